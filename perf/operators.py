@@ -108,7 +108,7 @@ def _quantise(x):
     x = x.float()
     m, e = torch.frexp(x.abs().amax(-1))
     k = torch.where(m <= 0.875, e - 9, e - 8).clamp(-126, 127)      # 448 = 0.875 * 2^9
-    k = torch.where(m == 0, torch.zeros_like(k), k)
+    k = torch.where(m == 0, torch.full_like(k, -126), k)
     codes = torch.ldexp(x, -k[..., None]).clamp(-448, 448).to(torch.float8_e4m3fn)
     return codes, (k + 127).to(torch.uint8)
 
