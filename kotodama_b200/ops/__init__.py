@@ -5,7 +5,7 @@ from __future__ import annotations
 
 import torch
 
-from .reference import TORCH_OPS, TorchOps
+from .reference import Fp8Pages, Int4Weight, TORCH_OPS, TorchOps
 
 _CUDA_OPS = None
 
@@ -21,4 +21,4 @@ def get_ops(device: torch.device | str):
     return _CUDA_OPS
 
 
-__all__ = ["get_ops", "TorchOps", "TORCH_OPS"]
+__all__ = ["get_ops", "Fp8Pages", "Int4Weight", "TorchOps", "TORCH_OPS"]

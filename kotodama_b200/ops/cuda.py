@@ -16,7 +16,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _build
-from .reference import DecodeWeight, Fp8Weight, TorchOps
+from .reference import DecodeWeight, Fp8Pages, Fp8Weight, Int4Weight, TorchOps
 
 _VP = ctypes.c_void_p
 _I = ctypes.c_int
@@ -26,6 +26,16 @@ _F = ctypes.c_float
 _FMT = {torch.float16: 0, torch.bfloat16: 1}
 _TYPE = {torch.bfloat16: 0, torch.float32: 1}      # activation type of kernels that exist for both
 _OUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+# arguments of the launchers that are called through CudaOps._launch: p address, i int, l long long, f float; the stream follows
+_CTYPE = {"p": _VP, "i": _I, "l": _LL, "f": _F}
+_ARGS = {
+    "kb_kv_append_fp8": "ppllppppp" + "iiil" + "ip",
+    "kb_kv_gather_fp8": "pppp" + "ii" + "piii" + "pppi" + "ppii" + "p",
+    "kb_tree_attn_plain": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fii" + "p",
+    "kb_gemm_int4": "pl" + "pp" + "pl" + "pl" + "iiii",
+}
 
 
 def _p(t: Optional[torch.Tensor]) -> _VP:
@@ -51,6 +61,7 @@ class CudaOps(TorchOps):
         self.mn_major = os.environ.get("KOTODAMA_MN_MAJOR", "1") == "1"   # MN-major GEMM operands (no transposes)
         self.launches = 0              # launches of kernels from this library
         self._status: dict[int, torch.Tensor] = {}
+        self._fns: dict = {}
         self.gemm_max_ctas = 0
         self.split_k_small_m = True
         self._splitk_ws: dict = {}
@@ -84,6 +95,23 @@ class CudaOps(TorchOps):
 
     def _call(self, fn: str, *args) -> None:
         self._rc(getattr(self.lib, fn)(*args), fn)
+
+    def _launch(self, fn: str, *args) -> None:
+        """A launcher called with plain numbers and addresses (its argument types are declared in ``_ARGS``); the stream is the current
+        one.  Cheaper on the host than wrapping every argument: the smallest operators are bound by it."""
+        f = self._fns.get(fn)
+        if f is None:
+            f = self._fns[fn] = getattr(self.lib, fn)
+            f.argtypes = [_CTYPE[c] for c in _ARGS[fn]] + [_VP]
+        self.launches += 1
+        rc = f(*args, torch.cuda.current_stream().cuda_stream)
+        if rc != 0:
+            raise KernelError(f"{fn}: launcher returned {rc}")
+
+    @staticmethod
+    def _on(t: torch.Tensor):
+        """The tensor's device made current, where it is not already (launches go to its stream)."""
+        return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
     def status(self, device: torch.device) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -290,7 +318,29 @@ class CudaOps(TorchOps):
         self._call("kb_pack_weight_tiles", _p(w), _LL(K), _p(packed), _I(N), _I(K), _st())
         return DecodeWeight(w, packed)
 
+    def _gemm_int4(self, a, b, out, residual, accumulate):
+        M, K = a.shape
+        N = b.shape[0]
+        if out is None:
+            out = torch.empty(M, N, device=a.device, dtype=a.dtype)
+        if accumulate and residual is not None:
+            raise KernelError("a product with 4-bit weights has one addend")
+        c = residual if residual is not None else (out if accumulate else None)
+        if (K != b.shape[1] or a.dtype != torch.bfloat16 or a.stride(1) != 1 or a.stride(0) % 8 or a.data_ptr() % 16 or out.shape != (M, N)
+                or any(t.dtype != a.dtype or t.stride(-1) != 1 or t.device != a.device for t in (out, c) if t is not None)
+                or b.packed.device != a.device or (c is not None and c.shape not in ((M, N), (1, N)))):
+            raise KernelError(f"4-bit product: bf16 rows of {b.shape[1]} numbers, 16-byte aligned, got {tuple(a.shape)} {a.dtype} {a.stride()}; "
+                              f"output and addend bf16 [{M}, {N}]")
+        if M:
+            with self._on(a):
+                self._launch("kb_gemm_int4", a.data_ptr(), a.stride(0), b.packed.data_ptr(), b.scales.data_ptr(),
+                             c.data_ptr() if c is not None else None, c.stride(0) if c is not None and c.shape[0] > 1 else 0, out.data_ptr(),
+                             out.stride(0), M, N, K, b.group)
+        return out
+
     def gemm_nt(self, a, b, out=None, residual=None, accumulate=False):
+        if isinstance(b, Int4Weight):
+            return self._gemm_int4(a, b, out, residual, accumulate)
         b_const = isinstance(b, DecodeWeight)
         if b_const:
             M, K = a.shape
@@ -502,6 +552,11 @@ class CudaOps(TorchOps):
         N = qkv.shape[0]
         out = torch.empty(N, (n_q + n_kv) * hd, device=qkv.device, dtype=qkv.dtype)
         rstd = torch.empty(N, n_q + n_kv, device=qkv.device, dtype=torch.float32)
+        if append is not None and isinstance(append[0], Fp8Pages):
+            self._rc(self.lib.kb_qknorm_rope_fwd(_p(qkv), _p(qw), _p(kw), _p(cos), _p(sin), _p(out), _p(rstd), _I(N), _I(seq_len), _I(n_q),
+                                                 _I(n_kv), _I(hd), _I(pos_offset), _F(eps), _p(positions), _st()), "kb_qknorm_rope_fwd")
+            self.kv_append(out[:, n_q * hd:], qkv[:, (n_q + n_kv) * hd:], *append)
+            return out, rstd
         if append is not None:
             k_pages, v_pages, slots = append
             rc = self.lib.kb_qknorm_rope_append(_p(qkv), _p(qw), _p(kw), _p(cos), _p(sin), _p(out), _p(rstd), _I(N),
@@ -658,12 +713,37 @@ class CudaOps(TorchOps):
 
     # ------------------------------------------------------------------ serving
     def kv_append(self, k, v, k_pages, v_pages, slots):
-        """Copy rows ``k[n], v[n]`` (``[N, n_kv*hd]`` views) into cache slot ``slots[n]`` (page*16 + offset)."""
+        """Copy rows ``k[n], v[n]`` (``[N, n_kv*hd]`` views) into cache slot ``slots[n]`` (page*16 + offset); with :class:`Fp8Pages`
+        quantised on the way (bf16 or fp32 rows)."""
+        if isinstance(k_pages, Fp8Pages):
+            return self._kv_append_fp8(k, v, k_pages, v_pages, slots)
         N, row = k.shape
         self._rc(self.lib.kb_kv_append(_p(k), _p(v), _LL(k.stride(0)), _LL(v.stride(0)), _p(k_pages), _p(v_pages),
                                        _p(slots), _I(N), _I(row), _I(k_pages.shape[-1]),
                                        _LL(k_pages.shape[0] * k_pages.shape[-2]), _p(self.status(k.device)), _st()),
                  "kb_kv_append")
+
+    def _kv_append_fp8(self, k, v, k_pages, v_pages, slots):
+        pages, n_kv, _, hd = k_pages.shape
+        N = self._fp8_pages(k_pages, v_pages, k, slots)
+        if (k.shape != (N, n_kv * hd) or v.shape != k.shape or slots.shape != (N,) or k.dtype not in _TYPE or v.dtype != k.dtype
+                or k.stride(1) != 1 or v.stride(1) != 1 or slots.dtype != torch.int64 or not slots.is_contiguous() or v.device != k.device):
+            raise KernelError(f"8-bit cache append: rows {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}, slots {tuple(slots.shape)} "
+                              f"{slots.dtype} for pages {tuple(k_pages.shape)}")
+        if N:
+            with self._on(k):
+                self._launch("kb_kv_append_fp8", k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k_pages.codes.data_ptr(),
+                             k_pages.exps.data_ptr(), v_pages.codes.data_ptr(), v_pages.exps.data_ptr(), slots.data_ptr(), N, n_kv, hd, pages * 16,
+                             _TYPE[k.dtype], self.status(k.device).data_ptr())
+
+    @staticmethod
+    def _fp8_pages(k_pages, v_pages, rows, *others) -> int:
+        """Checks that 8-bit pages belong together and lie where ``rows`` do; returns the number of rows."""
+        same = isinstance(v_pages, Fp8Pages) and k_pages.shape == v_pages.shape
+        if not same or k_pages.shape[2] != 16 or not all(t.is_contiguous() and t.device == rows.device for p in (k_pages, v_pages)
+                                                         for t in (p.codes, p.exps)) or any(t.device != rows.device for t in others):
+            raise KernelError("8-bit keys and values are dense pages of one shape, on the device of the rows")
+        return rows.shape[0]
 
     def paged_decode_attention(self, q, k_pages, v_pages, page_table, ctx_lens, max_ctx, n_q, n_kv, hd, split=512):
         """``q[B, n_q*hd]`` (one new token per request) against the paged cache; returns ``[B, n_q*hd]``."""
@@ -881,13 +961,33 @@ class CudaOps(TorchOps):
                    _st())
         return q, k, v
 
-    def kv_gather(self, k_pages, v_pages, page_table, seg_seq, seg_first, cu, total):
+    def kv_gather(self, k_pages, v_pages, page_table, seg_seq, seg_first, cu, total, dtype=torch.bfloat16):
+        if isinstance(k_pages, Fp8Pages):
+            return self._kv_gather_fp8(k_pages, v_pages, page_table, seg_seq, seg_first, cu, total, dtype)
         G, kd, vd = k_pages.shape[1], k_pages.shape[3], v_pages.shape[3]
         k = torch.empty(total, G, kd, device=k_pages.device, dtype=k_pages.dtype)
         v = torch.empty(total, G, vd, device=k_pages.device, dtype=k_pages.dtype)
         self._call("kb_kv_gather", _p(k_pages), _p(v_pages), _I(G), _I(kd), _I(vd), _p(page_table), _I(page_table.shape[0]), _I(page_table.shape[1]),
                    _I(k_pages.shape[0]), _p(seg_seq), _p(seg_first), _p(cu), _I(seg_seq.numel()), _p(k), _p(v), _I(total),
                    _I(_TYPE[k_pages.dtype]), _p(self.status(k_pages.device)), _st())
+        return k, v
+
+    def _kv_gather_fp8(self, k_pages, v_pages, page_table, seg_seq, seg_first, cu, total, dtype):
+        pages, G, _, hd = k_pages.shape
+        segs = seg_seq.numel()
+        self._fp8_pages(k_pages, v_pages, page_table, seg_seq, seg_first, cu)
+        if (dtype not in _TYPE or page_table.ndim != 2 or seg_first.numel() != segs or cu.numel() != segs + 1 or (total and not segs)
+                or any(t.dtype != torch.int32 or not t.is_contiguous() for t in (page_table, seg_seq, seg_first, cu))):
+            raise KernelError(f"8-bit cache rows are read as bf16 or fp32, by dense int32 tables: {dtype}, {segs} segments, "
+                              f"{seg_first.numel()} first positions, {cu.numel()} boundaries")
+        k = torch.empty(total, G, hd, device=page_table.device, dtype=dtype)
+        v = torch.empty_like(k)
+        if total:
+            with self._on(page_table):
+                self._launch("kb_kv_gather_fp8", k_pages.codes.data_ptr(), k_pages.exps.data_ptr(), v_pages.codes.data_ptr(),
+                             v_pages.exps.data_ptr(), G, hd, page_table.data_ptr(), page_table.shape[0], page_table.shape[1], pages,
+                             seg_seq.data_ptr(), seg_first.data_ptr(), cu.data_ptr(), segs, k.data_ptr(), v.data_ptr(), total, _TYPE[dtype],
+                             self.status(page_table.device).data_ptr())
         return k, v
 
     def paged_attention(self, q, k_pages, v_pages, page_table, ctx_lens, cu_seqlens, max_ctx, scale, softcap, chunk, gate, vdim, cols):
@@ -917,6 +1017,40 @@ class CudaOps(TorchOps):
                    _LL(gate.stride(0) if gate is not None else 0), _p(out), _I(N), _I(H), _I(vdim), _I(cols), _F(scale), _F(softcap), _I(chunk),
                    _I(_TYPE[q.dtype]), _p(self.status(q.device)), _st())
         return out
+
+    def paged_tree_attention(self, q, k_pages, v_pages, page_table, ctx_lens, cu_seqlens, max_q, max_ctx, scale, masks=None, out=None):
+        N, H, hd = q.shape
+        dev = q.device
+        fp8 = isinstance(k_pages, Fp8Pages)
+        B = ctx_lens.numel()
+        given = out is not None
+        res = out if given else torch.empty(N, H * hd, device=dev, dtype=q.dtype)
+        if fp8:
+            self._fp8_pages(k_pages, v_pages, q, page_table, ctx_lens)
+            kt, vt, ke, ve = k_pages.codes, v_pages.codes, k_pages.exps.data_ptr(), v_pages.exps.data_ptr()
+        else:
+            kt, vt, ke, ve = k_pages, v_pages, None, None
+            if (isinstance(v_pages, Fp8Pages) or kt.shape != vt.shape or kt.dtype != q.dtype or vt.dtype != q.dtype or not kt.is_contiguous()
+                    or not vt.is_contiguous() or kt.device != dev or vt.device != dev):
+                raise KernelError("keys and values are dense pages of one shape, of the queries' type and device")
+        if (q.dtype not in _TYPE or q.stride(2) != 1 or q.stride(1) != hd or kt.ndim != 4 or kt.shape[2] != 16 or kt.shape[3] != hd
+                or H % kt.shape[1] or res.shape != (N, H * hd) or res.dtype != q.dtype or res.stride(1) != 1 or res.device != dev):
+            raise KernelError(f"tree attention: queries {tuple(q.shape)} {q.dtype} {q.stride()} for pages {tuple(kt.shape)}, output "
+                              f"{tuple(res.shape)} {res.dtype}")
+        if (page_table.ndim != 2 or page_table.shape[0] != B or (cu_seqlens.numel() != B + 1 if cu_seqlens is not None else B > N)
+                or (masks is not None and (masks.shape != (N,) or masks.dtype != torch.int64 or not masks.is_contiguous() or masks.device != dev))
+                or any(t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev
+                       for t in (page_table, ctx_lens, cu_seqlens) if t is not None)):
+            raise KernelError(f"tree attention: {B} lengths, page lists {tuple(page_table.shape)}, boundaries "
+                              f"{None if cu_seqlens is None else tuple(cu_seqlens.shape)}, {N} rows; tables are dense int32, masks int64 per row")
+        if N == 0 or B == 0 or page_table.shape[1] == 0:
+            return res if given else res.zero_()
+        with self._on(q):
+            self._launch("kb_tree_attn_plain", q.data_ptr(), q.stride(0), kt.data_ptr(), ke, vt.data_ptr(), ve, page_table.data_ptr(),
+                         page_table.shape[1], kt.shape[0], ctx_lens.data_ptr(), cu_seqlens.data_ptr() if cu_seqlens is not None else None, B,
+                         masks.data_ptr() if masks is not None else None, res.data_ptr(), res.stride(0), N, H, kt.shape[1], hd, max_q, max_ctx,
+                         scale, int(not given), _TYPE[q.dtype], self.status(dev).data_ptr())
+        return res
 
     delta_short = 16        # most tokens of a sequence in one pass for which the recurrence is walked token by token
 

@@ -59,6 +59,83 @@ class DecodeWeight:
         return self.w.shape
 
 
+class Fp8Pages:
+    """Keys or values of a paged cache in 8 bits: e4m3 ``codes[pages, n_kv, 16, hd]`` and one power of two per row (token and KV
+    head), ``exps[pages, n_kv, 16]`` (uint8, biased by 127; 255 marks a row that held an infinity or a NaN).  A stored number is
+    ``code * 2^(exp - 127)``, with the smallest power (from 2^-126) that brings the row into the type's range.  Passing two of these where
+    the cache ops expect pages selects the 8-bit path."""
+
+    def __init__(self, codes: torch.Tensor, exps: torch.Tensor) -> None:
+        if codes.dtype != torch.float8_e4m3fn or exps.dtype != torch.uint8 or codes.ndim != 4 or codes.shape[:3] != exps.shape:
+            raise ValueError(f"8-bit pages are e4m3 codes [pages, n_kv, 16, hd] and uint8 exponents [pages, n_kv, 16], got "
+                             f"{codes.dtype} {tuple(codes.shape)}, {exps.dtype} {tuple(exps.shape)}")
+        self.codes, self.exps = codes, exps
+
+    @classmethod
+    def zeros(cls, pages: int, n_kv: int, hd: int, device: torch.device | str) -> "Fp8Pages":
+        return cls(torch.zeros(pages, n_kv, 16, hd, device=device, dtype=torch.float8_e4m3fn),
+                   torch.full((pages, n_kv, 16), 127, device=device, dtype=torch.uint8))
+
+    @property
+    def shape(self):
+        return self.codes.shape
+
+    @property
+    def device(self):
+        return self.codes.device
+
+    def rows(self, page: torch.Tensor, off: torch.Tensor) -> torch.Tensor:
+        """The fp32 rows ``[n, n_kv, hd]`` at places ``off`` of pages ``page``."""
+        c = self.codes.view(torch.uint8)[page, :, off].view(torch.float8_e4m3fn).float()
+        return torch.ldexp(c, self.exps[page, :, off].to(torch.int32)[..., None] - 127)
+
+
+def quant_pow2_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """``x[..., hd]`` -> e4m3 codes and biased exponents of :class:`Fp8Pages` (448 = 0.875 * 2^9, ties to even)."""
+    x = x.float()
+    top = x.abs().amax(-1)
+    m, e = torch.frexp(torch.where(torch.isfinite(top), top, torch.ones_like(top)))
+    k = torch.where(m <= 0.875, e - 9, e - 8).clamp(-126, 127)
+    k = torch.where(m == 0, torch.full_like(k, -126), k)
+    codes = _to_e4m3(torch.ldexp(x, -k[..., None]))
+    bad = ~torch.isfinite(top)
+    codes = torch.where(bad[..., None], torch.full_like(codes, float("nan"), dtype=torch.float32), codes.float()).to(torch.float8_e4m3fn)
+    return codes, torch.where(bad, torch.full_like(k, 255), k + 127).to(torch.uint8)
+
+
+class Int4Weight:
+    """A projection weight ``[N, K]`` in 4 bits: ``w[n, k] = scale[n, k // group] * (code[n, k] - 8)``, ``group`` 64 or 128.
+
+    ``packed`` (int32 ``[ceil(N / 16), ceil(K / 64), 32, 4]``) is in the order in which the tensor-core kernel consumes it: 512 contiguous
+    bytes hold a block of 16 rows and 64 inputs; word ``j`` of lane ``4 r + c`` has inputs ``16 c + 4 j .. + 3`` of row ``r`` in nibbles
+    0, 4, 2, 6 and of row ``r + 8`` in nibbles 1, 5, 3, 7.  Rows and inputs past the matrix have code 8.  ``scales`` (bf16
+    ``[ceil(N / 16), ceil(K / group), 8, 2]``) has rows ``r`` and ``r + 8`` side by side.  Made by :meth:`TorchOps.quant_int4`; passing one
+    where the NT product expects its weight selects the 4-bit path."""
+
+    def __init__(self, packed: torch.Tensor, scales: torch.Tensor, shape: tuple[int, int], group: int) -> None:
+        n, k = int(shape[0]), int(shape[1])
+        nt, kb = -(-n // 16), -(-k // 64)
+        if (n < 1 or k < 1 or k % 8 or group not in (64, 128) or packed.dtype != torch.int32 or scales.dtype != torch.bfloat16
+                or packed.shape != (nt, kb, 32, 4) or scales.shape != (nt, -(-k // group), 8, 2) or not packed.is_contiguous()
+                or not scales.is_contiguous() or packed.device != scales.device):
+            raise ValueError(f"4-bit weight {n} x {k}, group {group}: packed {packed.dtype} {tuple(packed.shape)}, scales {scales.dtype} "
+                             f"{tuple(scales.shape)} (inputs a multiple of 8, groups of 64 or 128)")
+        self.packed, self.scales, self.shape, self.group = packed, scales, torch.Size((n, k)), int(group)
+
+    def dense(self) -> torch.Tensor:
+        """The weight's values, fp32 ``[N, K]``."""
+        n, k = self.shape
+        nt, kb = self.packed.shape[:2]
+        shift = torch.tensor(_INT4_SHIFT, device=self.packed.device, dtype=torch.int32)
+        c = (self.packed.view(nt, kb, 8, 4, 4, 1, 1) >> shift) & 15                       # nt, kb, r, c, j, half, input
+        w = (c.permute(0, 5, 2, 1, 3, 4, 6).reshape(nt * 16, kb * 64)[:n, :k] - 8).float()
+        s = self.scales.float().permute(0, 3, 2, 1).reshape(nt * 16, -1)[:n]
+        return w * s.repeat_interleave(self.group, 1)[:, :k]
+
+
+_INT4_SHIFT = [[0, 16, 8, 24], [4, 20, 12, 28]]      # bit of input 0..3 of a word, rows r and r + 8
+
+
 def _to_e4m3(x: torch.Tensor) -> torch.Tensor:
     return x.clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
 
@@ -131,11 +208,41 @@ class TorchOps:
     def fp8_ok(self, *dims: int) -> bool:
         return all(d % 128 == 0 for d in dims)
 
+    # ------------------------------------------------------------------ 4-bit weights
+    def quant_int4(self, w: torch.Tensor, group: int = 128) -> Int4Weight:
+        """``w[N, K]`` (K a multiple of 8) in 4 bits: scale ``amax / 7`` per row and group, rounded to bf16 first so that the codes
+        fit the stored scale; ties to even."""
+        N, K = w.shape
+        if K % 8 or group not in (64, 128):
+            raise ValueError(f"4-bit weights take groups of 64 or 128 and inputs in eights, got {tuple(w.shape)}, group {group}")
+        nt, kb, ng = -(-N // 16), -(-K // 64), -(-K // group)
+        x = torch.zeros(nt * 16, ng * group, device=w.device, dtype=torch.float32)
+        x[:N, :K] = w.float()
+        x = x.view(nt * 16, ng, group)
+        scale = (x.abs().amax(-1) / 7.0).to(torch.bfloat16)
+        div = torch.where(scale == 0, torch.ones_like(scale), scale).float()
+        codes = torch.round(x / div[..., None]).clamp(-8, 7).to(torch.int64) + 8
+        c = codes.view(nt * 16, ng * group)[:, : kb * 64].reshape(nt, 2, 8, kb, 4, 4, 4).permute(0, 3, 2, 4, 5, 1, 6)
+        words = (c << torch.tensor(_INT4_SHIFT, device=w.device)).sum((-1, -2))                # nt, kb, r, c, j
+        packed = (words - ((words >> 31) << 32)).to(torch.int32).reshape(nt, kb, 32, 4).contiguous()
+        return Int4Weight(packed, scale.view(nt, 2, 8, ng).permute(0, 3, 2, 1).contiguous(), (N, K), group)
+
     # ------------------------------------------------------------------ GEMM
     def gemm_nt(self, a: torch.Tensor, b, out: Optional[torch.Tensor] = None,
                 residual: Optional[torch.Tensor] = None, accumulate: bool = False) -> torch.Tensor:
         """``a[M,K] @ b[N,K]^T (+ residual) -> [M,N]``; ``accumulate`` adds into ``out``.  ``b`` may be
-        an ``Fp8Weight``: the product then runs in block-scaled fp8."""
+        an ``Fp8Weight``: the product then runs in block-scaled fp8; or an ``Int4Weight``: 4-bit codes times the
+        activations, sums and scales in fp32."""
+        if isinstance(b, Int4Weight):
+            r = _f(a) @ b.dense().to(_f(a).dtype).t()
+            if residual is not None:
+                r = r + _f(residual)
+            if accumulate:
+                r = r + _f(out)
+            if out is None:
+                return r.to(a.dtype)
+            out.copy_(r)
+            return out
         if isinstance(b, DecodeWeight):
             b = b.w
         if isinstance(b, Fp8Weight):
@@ -624,10 +731,17 @@ class TorchOps:
 
     # ------------------------------------------------------------- serving
     def kv_append(self, k, v, k_pages, v_pages, slots) -> None:
-        """Copy rows ``k[n], v[n]`` (``[N, n_kv*hd]``) into cache slot ``slots[n]`` (= page*16 + offset)."""
+        """Copy rows ``k[n], v[n]`` (``[N, n_kv*hd]``) into cache slot ``slots[n]`` (= page*16 + offset; negative: dropped).  With
+        :class:`Fp8Pages` the rows are quantised on the way.  A slot is named once per call at most."""
         n_kv, hd = k_pages.shape[1], k_pages.shape[3]          # cache layout [pages, n_kv, 16, hd]
         ok = slots >= 0
         s = slots[ok]
+        if isinstance(k_pages, Fp8Pages):
+            for x, p in ((k, k_pages), (v, v_pages)):
+                codes, exps = quant_pow2_rows(x[ok].reshape(-1, n_kv, hd))
+                p.codes.view(torch.uint8)[s // 16, :, s % 16] = codes.view(torch.uint8)
+                p.exps[s // 16, :, s % 16] = exps
+            return
         k_pages[s // 16, :, s % 16] = k[ok].reshape(-1, n_kv, hd)
         v_pages[s // 16, :, s % 16] = v[ok].reshape(-1, n_kv, hd)
 
@@ -833,17 +947,73 @@ class TorchOps:
         v_pages[slots[ok] // 16, :, slots[ok] % 16] = v[ok]
         return (q, k, v) if keep else (q, None, None)
 
-    def kv_gather(self, k_pages, v_pages, page_table, seg_seq, seg_first, cu, total):
+    def kv_gather(self, k_pages, v_pages, page_table, seg_seq, seg_first, cu, total, dtype=torch.bfloat16):
         """Packed copies ``k, v[total, G, size]`` of cached rows: segment ``s`` holds positions ``seg_first[s] ..`` of sequence
-        ``seg_seq[s]`` in rows ``cu[s] .. cu[s + 1]``."""
+        ``seg_seq[s]`` in rows ``cu[s] .. cu[s + 1]``.  Rows of :class:`Fp8Pages` are returned as numbers of ``dtype``."""
         ks, vs = [], []
+        if isinstance(k_pages, Fp8Pages):
+            take = lambda p, page, off: p.rows(page, off).to(dtype)
+        else:
+            take = lambda p, page, off: p[page, :, off]
         cul = cu.tolist()
         for i, (b, f) in enumerate(zip(seg_seq.tolist(), seg_first.tolist())):
             t = torch.arange(f, f + cul[i + 1] - cul[i], device=k_pages.device)
             page = page_table[b, t // 16].long()
-            ks.append(k_pages[page, :, t % 16])
-            vs.append(v_pages[page, :, t % 16])
+            ks.append(take(k_pages, page, t % 16))
+            vs.append(take(v_pages, page, t % 16))
         return torch.cat(ks), torch.cat(vs)
+
+    def paged_tree_attention(self, q, k_pages, v_pages, page_table, ctx_lens, cu_seqlens, max_q, max_ctx, scale, masks=None, out=None):
+        """Attention of the drafted tokens of several sequences over the paged cache (bf16 pages or :class:`Fp8Pages`).
+
+        ``q[N, H, hd]``; sequence ``b`` owns rows ``cu_seqlens[b:b+2]`` (None: row ``b``), at most ``max_q`` and 64 of them.  Their keys and
+        values are already in the cache: they are the last of its ``ctx_lens[b]`` tokens (at most ``max_ctx``).  A row sees every token
+        in front of its sequence's rows, and of those rows the ones whose bits are set in ``masks[row]`` (int64, bit ``j`` =
+        row ``j`` of the sequence); without ``masks`` the ones up to itself.  What a row does not see does not reach it, whatever it
+        holds; a row that sees nothing is zero.  One row per sequence is plain decoding.
+
+        Returns ``[N, H * hd]``.  Rows behind the last sequence are zero, or left as they were in a given ``out``.  A sequence that
+        breaks these rules (more rows or tokens than it may have, fewer tokens than rows) gets zero rows, tokens on a page that is
+        not there are seen by no row; on CUDA both are recorded (status 6)."""
+        N, H, hd = q.shape
+        n_kv = k_pages.shape[1]
+        res = torch.zeros(N, H * hd, device=q.device, dtype=q.dtype) if out is None else out
+        cu = cu_seqlens.tolist() if cu_seqlens is not None else list(range(ctx_lens.numel() + 1))
+        num_pages = k_pages.shape[0]
+        take = lambda p, page, off: p.rows(page, off) if isinstance(p, Fp8Pages) else _f(p[page, :, off])
+        for b, n in enumerate(ctx_lens.tolist()):
+            lo, hi = max(cu[b], 0), min(cu[b + 1], N)
+            rows = cu[b + 1] - cu[b]
+            if hi <= lo:
+                continue
+            pages = page_table[b, : (max(n, 0) + 15) // 16].long()
+            if rows != hi - lo or rows > min(max_q, 64) or rows > n or n > min(max_ctx, page_table.shape[1] * 16):
+                res[lo:hi] = 0
+                continue
+            t = torch.arange(n, device=q.device)
+            there = ((pages >= 0) & (pages < num_pages))[t // 16]
+            page = pages[t // 16].clamp(0, num_pages - 1)
+            k, v = take(k_pages, page, t % 16), take(v_pages, page, t % 16)
+            j = t - (n - rows)
+            if masks is not None:
+                seen = (j[None, :] < 0) | ((masks[lo:hi, None] >> j.clamp_min(0)[None, :]) & 1 == 1)
+            else:
+                seen = j[None, :] <= torch.arange(rows, device=q.device)[:, None]
+            seen = seen & there
+            qf = _f(q[lo:hi]).reshape(rows, n_kv, H // n_kv, hd)
+            s = torch.einsum("ngrd,tgd->ngrt", qf, k.to(qf.dtype)) * scale
+            hide = ~seen[:, None, None, :]
+            s = s.masked_fill(hide, float("-inf"))
+            top = s.amax(-1, keepdim=True)
+            p = torch.exp(s - torch.where(top == float("-inf"), torch.zeros_like(top), top)).masked_fill(hide, 0.0)
+            total = p.sum(-1, keepdim=True)
+            p = p / torch.where(total == 0, torch.ones_like(total), total)
+            odd = ~torch.isfinite(v).all(-1).all(-1)                     # tokens whose values must not touch rows that do not see them
+            o = torch.einsum("ngrt,tgd->ngrd", p, torch.where(odd[:, None, None], torch.zeros_like(v), v).to(p.dtype))
+            for i in odd.nonzero().flatten().tolist():
+                o = torch.where(seen[:, i, None, None, None], o + p[..., i:i + 1] * v[i].to(p.dtype)[None, :, None, :], o)
+            res[lo:hi] = o.reshape(rows, H * hd).to(q.dtype)
+        return res
 
     def paged_attention(self, q, k_pages, v_pages, page_table, ctx_lens, cu_seqlens, max_ctx, scale, softcap, chunk, gate, vdim, cols):
         """``q[N, H, size]`` against the paged cache; sequence ``b`` owns rows ``cu_seqlens[b:b+2]`` (None: row ``b``), the last of

@@ -1,0 +1,232 @@
+"""8-bit paged cache, tree attention and 4-bit weights on the sm_100a kernels."""
+import math
+
+import pytest
+import torch
+
+import lowbit_cases as cases
+from kotodama_b200.ops import Fp8Pages, Int4Weight, get_ops
+from kotodama_b200.ops.cuda import KernelError
+from kotodama_b200.utils.guard import GuardRegions
+
+pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float32]
+
+
+def guarded(f):
+    ops = get_ops("cuda")
+    with GuardRegions() as g:
+        r = f(ops)
+        torch.cuda.synchronize()
+        assert not g.check()
+    return r
+
+
+# ------------------------------------------------------------------ 8-bit cache
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", cases.APPEND_CASES, ids=str)
+def test_append_is_exact(case, dtype):
+    guarded(lambda ops: cases.check_append(ops, "cuda", dtype, *case))
+    get_ops("cuda").check_status()
+
+
+def test_append_of_many_rows():
+    """Enough rows for the form with several rows per lane group: the same bytes as the plain back end's."""
+    from kotodama_b200.ops import TORCH_OPS
+    ops = get_ops("cuda")
+    n, n_kv, hd = 20011, 4, 128
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k = (torch.randn(n, n_kv * hd, device="cuda", generator=g) * torch.exp(torch.randn(n, 1, device="cuda", generator=g))).bfloat16()
+    v = torch.randn(n, n_kv * hd, device="cuda", generator=g).bfloat16()
+    slots = torch.randperm(n + 5, device="cuda", generator=g)[:n]
+    slots[7::100] = -1
+    got = [Fp8Pages.zeros(-(-(n + 5) // 16), n_kv, hd, "cuda") for _ in range(2)]
+    want = [Fp8Pages.zeros(-(-(n + 5) // 16), n_kv, hd, "cuda") for _ in range(2)]
+    ops.kv_append(k, v, *got, slots)
+    TORCH_OPS.kv_append(k, v, *want, slots)
+    for a, b in zip(got, want):
+        assert torch.equal(a.codes.view(torch.uint8), b.codes.view(torch.uint8)) and torch.equal(a.exps, b.exps)
+    ops.check_status()
+
+
+def test_rows_that_are_not_finite():
+    cases.check_append_not_finite(get_ops("cuda"), "cuda")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", cases.GATHER_CASES, ids=str)
+def test_gather_is_exact(case, dtype):
+    guarded(lambda ops: cases.check_gather(ops, "cuda", dtype, *case))
+    get_ops("cuda").check_status()
+
+
+def test_indices_out_of_range_are_reported():
+    ops = get_ops("cuda")
+    k = torch.randn(3, 64, device="cuda").bfloat16()
+    kp, vp = Fp8Pages.zeros(2, 1, 64, "cuda"), Fp8Pages.zeros(2, 1, 64, "cuda")
+    ops.kv_append(k, k, kp, vp, torch.tensor([0, 32, 5], device="cuda"))         # slot 32 of 32
+    with pytest.raises(KernelError, match="status 6"):
+        ops.check_status()
+    t = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    x, _ = ops.kv_gather(kp, vp, t(0, 9)[None], t(0), t(0), t(0, 20), 20)          # page 9 of 2
+    with pytest.raises(KernelError, match="status 6"):
+        ops.check_status()
+    assert bool((x[16:] == 0).all()) and bool((x[0] != 0).any())
+    ops.check_status()
+
+
+# ------------------------------------------------------------------ tree attention
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("case", cases.TREE_CASES + cases.TREE_PLAIN_CASES, ids=str)
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_tree_attention(case, fp8, dtype):
+    H, G, hd, sizes, lens, masked = case
+    guarded(lambda ops: cases.check_tree(ops, "cuda", H, G, hd, sizes, lens, fp8, dtype, masked))
+    get_ops("cuda").check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fp8", [False, True])
+def test_masked_tokens_that_are_not_finite(fp8, dtype):
+    cases.check_tree_masked_not_finite(get_ops("cuda"), "cuda", fp8, dtype)
+    cases.check_tree_masked_not_finite(get_ops("cuda"), "cuda", fp8, dtype, hd=64)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_bad_sequences(fp8):
+    ops = get_ops("cuda")
+    cases.check_tree_bad_sequences(ops, "cuda", fp8)
+    with pytest.raises(KernelError, match="status 6"):
+        ops.check_status()
+    ops.check_status()
+
+
+# ------------------------------------------------------------------ 4-bit weights
+@pytest.mark.parametrize("case", cases.INT4_QUANT_CASES, ids=str)
+def test_quantise_weights(case):
+    cases.check_quant_int4(get_ops("cuda"), "cuda", *case)
+
+
+@pytest.mark.parametrize("case", cases.INT4_CASES, ids=str)
+def test_products_with_4_bit_weights(case):
+    M, N, K, group, stride = case
+    guarded(lambda ops: cases.check_int4(ops, "cuda", torch.bfloat16, M, N, K, group, stride=stride))
+    get_ops("cuda").check_status()
+
+
+# ------------------------------------------------------------------ refusals
+def test_refusals():
+    ops = get_ops("cuda")
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    kp, vp = Fp8Pages.zeros(2, 1, 64, "cuda"), Fp8Pages.zeros(2, 1, 64, "cuda")
+    k = torch.randn(3, 64, device="cuda").bfloat16()
+    s = torch.arange(3, device="cuda")
+    for call in (lambda: ops.kv_append(k.half(), k.half(), kp, vp, s), lambda: ops.kv_append(k, k, kp, vp, s.int()),
+                 lambda: ops.kv_append(k, k, kp, vp, s[:2]), lambda: ops.kv_append(k[:, :32], k[:, :32], kp, vp, s),
+                 lambda: ops.kv_append(k, k, kp, Fp8Pages.zeros(3, 1, 64, "cuda"), s), lambda: ops.kv_append(k, k, kp, vp.codes, s),
+                 lambda: ops.kv_append(k, k.float(), kp, vp, s), lambda: ops.kv_append(k, k, kp, vp, s.cpu()),
+                 lambda: ops.kv_gather(kp, vp, i32(0)[None], i32(0), i32(0), i32(0, 4), 4, torch.float16),
+                 lambda: ops.kv_gather(kp, vp, i32(0)[None], i32(0), i32(0, 0), i32(0, 4), 4),
+                 lambda: ops.kv_gather(kp, vp, i32(0)[None].long(), i32(0), i32(0), i32(0, 4), 4)):
+        with pytest.raises(KernelError):
+            call()
+    q = torch.randn(2, 2, 64, device="cuda").bfloat16()
+    good = dict(q=q, k_pages=kp, v_pages=vp, page_table=i32(0)[None], ctx_lens=i32(8), cu_seqlens=i32(0, 2), max_q=2, max_ctx=8, scale=0.1)
+    ops.paged_tree_attention(**good)
+    page = torch.zeros(2, 1, 16, 64, device="cuda", dtype=torch.bfloat16)
+    for bad in (dict(q=q.half()), dict(q=q[:, :, :32]), dict(q=q.transpose(0, 1)), dict(v_pages=page), dict(k_pages=page), dict(ctx_lens=i32(8, 8)),
+                dict(cu_seqlens=i32(0, 1, 2)), dict(cu_seqlens=torch.tensor([0, 2], device="cuda")), dict(masks=s[:1]), dict(masks=i32(1, 1)),
+                dict(page_table=i32(0)), dict(out=q.view(2, 128).float()), dict(out=torch.empty(3, 128, device="cuda", dtype=torch.bfloat16)),
+                dict(k_pages=page.float(), v_pages=page.float()), dict(ctx_lens=torch.tensor([8], dtype=torch.int32))):
+        with pytest.raises(KernelError):
+            ops.paged_tree_attention(**{**good, **bad})
+    w = ops.quant_int4(torch.randn(32, 128, device="cuda"))
+    x = torch.randn(2, 128, device="cuda").bfloat16()
+    for call in (lambda: ops.gemm_nt(x.float(), w), lambda: ops.gemm_nt(x[:, :64], w), lambda: ops.gemm_nt(x.t().contiguous().t(), w),
+                 lambda: ops.gemm_nt(torch.randn(2, 132, device="cuda").bfloat16()[:, :128], w), lambda: ops.gemm_nt(x, w, out=x),
+                 lambda: ops.gemm_nt(x, w, residual=x), lambda: ops.gemm_nt(x, w, out=x[:, :32], residual=x[:, :32], accumulate=True),
+                 lambda: ops.gemm_nt(x, Int4Weight(w.packed.cpu(), w.scales.cpu(), (32, 128), 128))):
+        with pytest.raises(KernelError):
+            call()
+    ops.check_status()
+
+
+# ------------------------------------------------------------------ together, captured, on another stream
+def verification_step(ops, seed=0):
+    """What a server does to verify drafted tokens: 4-bit projections, 8-bit append, tree attention over the cache, 4-bit output
+    projection.  Returns a function that runs it on given inputs, and the inputs."""
+    H, G, hd, D, sizes, lens = 8, 2, 128, 512, [4, 1, 7], [37, 200, 64]
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    wqkv, wo = ops.quant_int4(rand((H + 2 * G) * hd, D) / 20), ops.quant_int4(rand(D, H * hd) / 20)
+    kp, vp = Fp8Pages.zeros(24, G, hd, "cuda"), Fp8Pages.zeros(24, G, hd, "cuda")
+    table = torch.arange(24, device="cuda", dtype=torch.int32).flip(0).view(3, 8)
+    table = torch.cat([table, table.new_zeros(3, 6)], 1)
+    table[1, :13] = torch.randperm(13, device="cuda", generator=g).int()                   # its own pages: 0 .. 12
+    table[0, :8], table[2, :8] = torch.arange(13, 21, device="cuda").int(), torch.tensor([21, 22, 23, 13 + 4, 13 + 5, 0, 0, 0], device="cuda").int()
+    ctx = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 4, 5, 12], dtype=torch.int32, device="cuda")
+    slot = lambda b, t: int(table[b, t // 16]) * 16 + t % 16
+    old = [slot(b, t) for b in range(3) for t in range(lens[b] - sizes[b])]
+    new = torch.tensor([slot(b, t) for b in range(3) for t in range(lens[b] - sizes[b], lens[b])], device="cuda")
+    rows = rand(len(old), 2 * G * hd).bfloat16()
+    ops.kv_append(rows[:, : G * hd], rows[:, G * hd:], kp, vp, torch.tensor(old, device="cuda"))
+    masks = cases.signed(cases.tree_masks(sizes, 3)).cuda()
+
+    def run(x):
+        qkv = ops.gemm_nt(x, wqkv)
+        ops.kv_append(qkv[:, H * hd:(H + G) * hd], qkv[:, (H + G) * hd:], kp, vp, new)
+        o = ops.paged_tree_attention(qkv[:, : H * hd].view(-1, H, hd), kp, vp, table, ctx, cu, 8, 256, 1 / math.sqrt(hd), masks)
+        return ops.gemm_nt(o, wo, residual=x)
+
+    def plain(x):
+        f = torch.float64
+        dense = [w.dense().to(f) for w in (wqkv, wo)]
+        qkv = (x.to(f) @ dense[0].t()).bfloat16()
+        o, _ = cases.plain_tree(qkv[:, : H * hd].reshape(-1, H, hd).cpu(), cases.plain_values(kp), cases.plain_values(vp), table.tolist(), lens,
+                                cu.tolist(), 1 / math.sqrt(hd), [m & (1 << 64) - 1 for m in masks.tolist()])
+        return o.reshape(12, -1).bfloat16().to(f) @ dense[1].t().cpu() + x.to(f).cpu()
+
+    return run, plain, [rand(12, D).bfloat16() for _ in range(3)]
+
+
+def test_verification_step():
+    ops = get_ops("cuda")
+    run, plain, xs = verification_step(ops)
+    for x in xs:
+        got = run(x)
+        want = plain(x)                              # reads the cache that run() wrote
+        # roundings to bf16 on the way (projection, attention, output): half a step each of the magnitudes they weigh
+        assert float((got.cpu().double() - want).norm() / want.norm()) < 3 * 2.0 ** -8
+    ops.check_status()
+
+
+def test_captured_and_replayed_on_another_stream():
+    """The step in a graph: replayed on new inputs it gives what the eager call gives; two graphs replayed in turn do not disturb one another."""
+    ops = get_ops("cuda")
+    steps = [verification_step(ops, s) for s in (0, 1)]
+    want = [[run(x).clone() for x in xs] for run, _, xs in steps]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = [run(xs[0]) for run, _, xs in steps]
+    side.synchronize()
+    assert all(torch.equal(a, w[0]) for a, w in zip(again, want))
+    graphs = []
+    for run, _, xs in steps:
+        x = xs[0].clone()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g), ops.dependent_launch():
+            y = run(x)
+        graphs.append((g, x, y))
+    streams = [torch.cuda.Stream() for _ in steps]
+    for i in range(3):
+        for (g, x, _), (_, _, xs), st in zip(graphs, steps, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                x.copy_(xs[i])
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, _, y), w in zip(graphs, want):
+            assert torch.equal(y, w[i])
+    ops.check_status()
