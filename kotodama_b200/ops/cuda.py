@@ -34,6 +34,7 @@ _ARGS = {
     "kb_kv_append_fp8": "ppllppppp" + "iiil" + "ip",
     "kb_kv_gather_fp8": "pppp" + "ii" + "piii" + "pppi" + "ppii" + "p",
     "kb_tree_attn_plain": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fii" + "p",
+    "kb_tree_attn": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fi" + "pl" + "p",
     "kb_gemm_int4": "pl" + "pp" + "pl" + "pl" + "iiii",
 }
 
@@ -83,6 +84,9 @@ class CudaOps(TorchOps):
                      "kb_route_blocked_grid"):
             if hasattr(self.lib, name):          # a library of the serving kernels alone does not have the training ones
                 getattr(self.lib, name).restype = _I
+        if hasattr(self.lib, "kb_tree_attn_floats"):
+            self._tree_floats = self.lib.kb_tree_attn_floats
+            self._tree_floats.restype = _LL
         for name in ("kb_delta_chunk_tt_bytes", "kb_delta_chunk_scalars"):
             if hasattr(self.lib, name):
                 getattr(self.lib, name).restype = _LL
@@ -1019,6 +1023,8 @@ class CudaOps(TorchOps):
         return out
 
     def paged_tree_attention(self, q, k_pages, v_pages, page_table, ctx_lens, cu_seqlens, max_q, max_ctx, scale, masks=None, out=None):
+        """bf16 queries with heads of 64 or 128 take the tensor-core kernel (``csrc/tree_attn_sm100.cu``); the 32-bit mode, other head
+        sizes and rows that are not 8-byte aligned the plain one (``csrc/tree_attn.cu``)."""
         N, H, hd = q.shape
         dev = q.device
         fp8 = isinstance(k_pages, Fp8Pages)
@@ -1045,6 +1051,18 @@ class CudaOps(TorchOps):
                               f"{None if cu_seqlens is None else tuple(cu_seqlens.shape)}, {N} rows; tables are dense int32, masks int64 per row")
         if N == 0 or B == 0 or page_table.shape[1] == 0:
             return res if given else res.zero_()
+        floats = 0
+        if q.dtype == torch.bfloat16 and q.stride(0) % 4 == 0 and res.stride(0) % 4 == 0 and (q.data_ptr() | res.data_ptr()) % 8 == 0:
+            floats = self._tree_floats(N, B, H, kt.shape[1], hd, max_q, max_ctx, kt.shape[0], int(fp8))
+        if floats:
+            work = torch.empty(floats, device=dev, dtype=torch.float32)
+            with self._on(q):
+                self._launch("kb_tree_attn", q.data_ptr(), q.stride(0), kt.data_ptr(), ke, vt.data_ptr(), ve, page_table.data_ptr(),
+                             page_table.shape[1], kt.shape[0], ctx_lens.data_ptr(), cu_seqlens.data_ptr() if cu_seqlens is not None else None, B,
+                             masks.data_ptr() if masks is not None else None, res.data_ptr(), res.stride(0), N, H, kt.shape[1], hd, max_q, max_ctx,
+                             scale, int(not given), work.data_ptr(), floats, self.status(dev).data_ptr())
+            self.launches += 1
+            return res
         with self._on(q):
             self._launch("kb_tree_attn_plain", q.data_ptr(), q.stride(0), kt.data_ptr(), ke, vt.data_ptr(), ve, page_table.data_ptr(),
                          page_table.shape[1], kt.shape[0], ctx_lens.data_ptr(), cu_seqlens.data_ptr() if cu_seqlens is not None else None, B,

@@ -429,3 +429,13 @@ def check_int4(ops, device, dtype, M, N, K, group, seed=0, stride=0):
 
 INT4_CASES = [(1, 16, 64, 64, 0), (1, 1, 8, 128, 0), (3, 40, 200, 128, 8), (8, 96, 512, 128, 0), (9, 33, 520, 64, 0), (17, 130, 1032, 128, 16),
               (33, 64, 64, 128, 0), (64, 48, 768, 64, 0), (65, 100, 1000, 128, 0), (130, 70, 136, 64, 8)]
+
+
+def tile_parts(total, grid):
+    """The line of ``total`` tiles as the tensor-core kernel cuts it (integer arithmetic of the kernel, for a check of its merge)."""
+    parts = min(grid, total)
+    return [(total * c // parts, total * (c + 1) // parts) for c in range(parts)]
+
+
+def part_of(tile, total, grid):
+    return ((tile + 1) * min(grid, total) - 1) // total

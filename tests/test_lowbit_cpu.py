@@ -63,3 +63,13 @@ def test_operands_that_are_no_pages_or_weights():
     for shape, group in (((4, 12), 64), ((4, 64), 32)):
         with pytest.raises(ValueError):
             TORCH_OPS.quant_int4(torch.randn(*shape), group)
+
+
+def test_the_cut_of_the_tiles():
+    """Every part has a tile, and the merge finds the part of a tile: all parts between a unit's first and last hold some of it."""
+    for total in list(range(1, 40)) + [295, 296, 297, 1000, 8192]:
+        for grid in (1, 2, 7, 8, 148, 296):
+            parts = cases.tile_parts(total, grid)
+            assert parts[0][0] == 0 and parts[-1][1] == total and all(a < b for a, b in parts) and all(p[1] == q[0] for p, q in zip(parts, parts[1:]))
+            for c, (a, b) in enumerate(parts):
+                assert all(cases.part_of(t, total, grid) == c for t in (a, (a + b) // 2, b - 1))
