@@ -21,31 +21,13 @@
 // Queries become f16 with a power of two per row taken out (exact down to 2^-24 of the row's largest).
 // bf16 pages: queries as they are, probabilities rounded to bf16 (2^-9 relative, like the other decode kernels).
 // Scores, maxima, sums and outputs are fp32.
-#include <cuda_fp8.h>
-
-#include "tc.cuh"
-
-typedef __nv_bfloat16 bf16;
+#include "tree_attn.cuh"
 
 namespace {
 
-constexpr int PAGE = 16, WARPS = 4, THREADS = WARPS * 32, MAX_B = 2048;
+using namespace tree;
 
-struct TreeParams {
-    const bf16* q;
-    long long q_stride;
-    const uint8_t *ke, *ve;                            // exponents of 8-bit pages
-    const int *table, *ctx_lens, *cu;
-    const long long* masks;
-    bf16* out;
-    long long out_stride;
-    float* part_o;                                     // [2 * grid][ROWS][HD]
-    float* part_ml;                                    // [2 * grid][ROWS][2]
-    int* uoff;                                         // [B + 1] tiles before each sequence, for the merge kernel
-    int max_pages, num_pages, B, N, H, G, n_kv, max_q, max_ctx;
-    float scale_log2;
-    int* status;
-};
+constexpr int WARPS = 4, THREADS = WARPS * 32;
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t* r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -66,27 +48,8 @@ __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, ui
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// four e4m3 codes -> two f16 pairs
-__device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t& hi) {
-    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(c));
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ float pow2_biased(int b) { return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 0x00400000u); }
-
 // A page's rows of one KV head, seen as [halves][16 rows][at most 128 bytes]: bf16 heads of 128 have two halves.
 __device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* m, uint64_t* bar, int row) { tc::tma_load_3d(dst, m, bar, 0, row, 0); }
-__device__ __forceinline__ void bulk_16(void* dst, const void* src, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(16), "r"(smem_u32(bar)) : "memory");
-}
-
 template <bool FP8, int HD, int MI>
 struct Cfg {
     static constexpr int ROWS = 16 * MI;
@@ -104,21 +67,6 @@ struct Cfg {
     static constexpr int EXPS = FP8 ? WARPS * NST * 2 * IT : 0;        // exponents of a stage: keys, then values
     static constexpr int FACT = FP8 ? WARPS * 2 * IT * 4 : 0;          // the step's factors as fp32
     static constexpr int SMEM = 1024 + RING + OBUF + EXPS + FACT;
-};
-
-// rows of a sequence and its tokens; 0 rows where it has none or breaks the rules
-__device__ __forceinline__ int2 span_of(const TreeParams& p, int b, bool report) {
-    const int c0 = p.cu ? p.cu[b] : b, c1 = p.cu ? p.cu[b + 1] : b + 1, n = c1 - c0, ctx = p.ctx_lens[b];
-    if (n <= 0) return make_int2(0, 0);
-    if (c0 < 0 || c1 > p.N || n > p.max_q || n > 64 || n > ctx || ctx > p.max_ctx || (ctx + PAGE - 1) / PAGE > p.max_pages) {
-        if (report && p.status) atomicMax(p.status, (int)KB_BAD_INDEX);
-        return make_int2(0, 0);
-    }
-    return make_int2(n, ctx);
-}
-
-struct Segment {                                       // a CTA's part of one unit
-    int b, h, rb, n, ctx, T, t0, t1;
 };
 
 template <bool FP8, int HD, int MI>
@@ -149,63 +97,11 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     }
     kb_dep_trigger();
     kb_dep_wait();
-    // ---- tiles before each sequence
-    {
-        const int per = (p.B + THREADS - 1) / THREADS;
-        int mine = 0;
-        for (int i = 0; i < per; ++i) {
-            const int b = threadIdx.x * per + i;
-            if (b >= p.B) break;
-            const int2 s = span_of(p, b, blockIdx.x == 0);
-            const int t = p.n_kv * ((s.x * p.G + C::ROWS - 1) / C::ROWS) * ((s.y + C::TILE - 1) / C::TILE);
-            uoff[b + 1] = t;
-            mine += t;
-        }
-        int s = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int v = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += v;
-        }
-        if (lane == 31) wsum[warp] = s;
-        __syncthreads();
-        int run = s - mine;
-        for (int w = 0; w < warp; ++w) run += wsum[w];
-        for (int i = 0; i < per; ++i) {
-            const int b = threadIdx.x * per + i;
-            if (b >= p.B) break;
-            run += uoff[b + 1];
-            uoff[b + 1] = run;
-        }
-        if (threadIdx.x == 0) uoff[0] = 0;
-        __syncthreads();
-        if (blockIdx.x == 0)
-            for (int i = threadIdx.x; i <= p.B; i += THREADS) p.uoff[i] = uoff[i];
-    }
-    const long long total = uoff[p.B];
-    const long long parts = min((long long)gridDim.x, total);      // every part has a tile: the merge reads all parts between a unit's ends
-    if (blockIdx.x >= parts) return;
-    const int lo = (int)(total * blockIdx.x / parts), hi = (int)(total * (blockIdx.x + 1) / parts);
-
-    auto segment = [&](int x) {                        // the unit of tile x, as far as this CTA has it from x on
-        int a = 0, z = p.B;
-        while (z - a > 1) {
-            const int m = (a + z) >> 1;
-            if (uoff[m] <= x) a = m; else z = m;
-        }
-        Segment s;
-        s.b = a;
-        const int2 sp = span_of(p, a, false);
-        s.n = sp.x;
-        s.ctx = sp.y;
-        s.T = (sp.y + C::TILE - 1) / C::TILE;
-        const int rel = x - uoff[a], unit = rel / s.T, rbs = (sp.x * p.G + C::ROWS - 1) / C::ROWS;
-        s.h = unit / rbs;
-        s.rb = unit % rbs;
-        s.t0 = rel - unit * s.T;
-        s.t1 = min(s.T, s.t0 + hi - x);
-        return s;
-    };
+    count_tiles<C::ROWS, C::TILE, THREADS>(p, uoff, wsum);
+    const int2 part = part_of_line(uoff[p.B]);
+    const int lo = part.x, hi = part.y;
+    if (lo >= hi) return;
+    auto segment = [&](int x) { return segment_at<C::ROWS, C::TILE>(p, uoff, x, hi); };
 
     // ---- producer side of this warp's ring: item k is this warp's step of tile lo + k
     uint8_t* ring = ring_all + (size_t)warp * C::NST * C::STAGE;
@@ -400,11 +296,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
                         for (int hf = 0; hf < 2; ++hf) {
                             const int i = min((row0 + mi * 16 + hf * 8 + r) / p.G, sg.n - 1);
-                            const unsigned long long mask = p.masks ? (unsigned long long)p.masks[c0 + i] : ~0ull >> (63 - i);
-                            const int d = base - prefix;                   // drafted index of the step's first token
-                            unsigned long long v = d >= 0 ? (d < 64 ? mask >> d : 0ull) : (mask << (-d < 64 ? -d : 0)) * (-d < 64);
-                            if (d < 0) v |= -d >= 64 ? ~0ull : (1ull << -d) - 1ull;
-                            seen[mi][hf] = v & valid;
+                            seen[mi][hf] = sees(p, c0, i, base - prefix) & valid;
 #pragma unroll
                             for (int j = 0; j < NT; ++j) {
                                 const uint32_t two = (uint32_t)(seen[mi][hf] >> (8 * j + 2 * qd)) & 3u;
@@ -761,20 +653,22 @@ EncodeFn encoder() {
     }
     return enc;
 }
-int page_map(CUtensorMap* m, const void* base, long long rows, int hd, bool fp8) {
+}  // namespace
+
+int tree::page_map(CUtensorMap* m, const void* base, long long rows, int hd, bool fp8, bool halves_apart) {
     const EncodeFn enc = encoder();
     if (!enc) return 100;
     const int row_bytes = fp8 ? hd : 2 * hd, in = row_bytes > 128 ? 128 : row_bytes, esz = fp8 ? 1 : 2;
     const cuuint64_t dims[3] = {(cuuint64_t)(in / esz), (cuuint64_t)rows, (cuuint64_t)(row_bytes / in)};
     const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)in};
-    const cuuint32_t box[3] = {(cuuint32_t)(in / esz), PAGE, (cuuint32_t)(row_bytes / in)}, one[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)(in / esz), PAGE, halves_apart ? 1u : (cuuint32_t)(row_bytes / in)}, one[3] = {1, 1, 1};
     const CUresult r = enc(m, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
                            one, CU_TENSOR_MAP_INTERLEAVE_NONE, in == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? 0 : 200 + (int)r;
 }
 
-int sm_count() {
+int tree::sm_count() {
     static int count[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
@@ -782,25 +676,43 @@ int sm_count() {
     return count[dev];
 }
 
+int tree::merge(const TreeParams& p, int hd, int rows, int tile, int grid, bool wide, int zero_tail, cudaStream_t st) {
+    const long long n = (long long)p.N * p.H;
+#define MERGE(HD_, W_)                                                                                                                  \
+    return kb_launch_dep(tree_merge_kernel<HD_, W_>, dim3((unsigned)((n + 8 / W_ - 1) / (8 / W_))), dim3(256), 0, st, p, rows, tile, grid, zero_tail)
+    if (hd == 128) {
+        if (wide) MERGE(128, 8);
+        MERGE(128, 1);
+    }
+    if (wide) MERGE(64, 8);
+    MERGE(64, 1);
+#undef MERGE
+}
+
+namespace {
+
 struct Plan {
-    int rows, tile, grid, wide_merge;
+    int rows, tile, grid;
+    bool wide;
 };
-// One CTA per tile, at most two per SM (what registers and shared memory admit).
+// Which kernel, and how many CTAs: one per tile, at most what fits the GPU at once (one per SM for the 128-row kernel, two for the
+// others).
 Plan plan_for(int B, int N, int n_kv, int G, int max_q, int max_ctx, bool fp8) {
     Plan pl;
-    pl.rows = max_q * G <= 16 ? 16 : 32;
-    pl.tile = WARPS * (fp8 ? 32 : 16);
+    const int most_rows = max_q * G;
+    pl.rows = most_rows <= 16 ? 16 : most_rows <= 32 ? 32 : 128;
+    pl.tile = pl.rows == 128 ? 128 : WARPS * (fp8 ? 32 : 16);
     const long long blocks = B + (long long)N * G / pl.rows;                            // units per KV head, at most
-    const long long one = (max_q * G + pl.rows - 1) / pl.rows;
+    const long long one = (most_rows + pl.rows - 1) / pl.rows;
     const long long units = n_kv * (blocks < B * one ? blocks : B * one), tiles = units * ((max_ctx + pl.tile - 1) / pl.tile);
-    const long long most = 2ll * sm_count();
+    const long long most = (pl.rows == 128 ? 1ll : 2ll) * sm_count();
     pl.grid = (int)(tiles < most ? tiles : most);
-    pl.wide_merge = pl.grid > 8 * units;               // parts per unit: one warp per row walks up to about eight of them
+    pl.wide = pl.grid > 8 * units;                     // parts per unit: one warp per row walks up to about eight of them
     return pl;
 }
 
 template <bool FP8, int HD, int MI>
-int launch_tree(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams& p, const Plan& pl, int zero_tail, cudaStream_t st) {
+int launch_tree(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams& p, const Plan& pl, cudaStream_t st) {
     static bool flags[64] = {};
     bool* set = kb_device_flag(flags);
     if (!set) return 7;
@@ -808,12 +720,7 @@ int launch_tree(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams
         if (cudaFuncSetAttribute(tree_attn_kernel<FP8, HD, MI>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<FP8, HD, MI>::SMEM) != cudaSuccess) return 7;
         *set = true;
     }
-    const int r = kb_launch_dep(tree_attn_kernel<FP8, HD, MI>, dim3(pl.grid), dim3(THREADS), Cfg<FP8, HD, MI>::SMEM, st, tmK, tmV, p);
-    if (r) return r;
-    const long long rows = (long long)p.N * p.H;
-    if (pl.wide_merge)
-        return kb_launch_dep(tree_merge_kernel<HD, 8>, dim3((unsigned)rows), dim3(256), 0, st, p, pl.rows, pl.tile, pl.grid, zero_tail);
-    return kb_launch_dep(tree_merge_kernel<HD, 1>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, pl.rows, pl.tile, pl.grid, zero_tail);
+    return kb_launch_dep(tree_attn_kernel<FP8, HD, MI>, dim3(pl.grid), dim3(THREADS), Cfg<FP8, HD, MI>::SMEM, st, tmK, tmV, p);
 }
 
 }  // namespace
@@ -843,8 +750,8 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
     const Plan pl = plan_for(B, N, n_kv, H / n_kv, max_q, max_ctx, fp8);
     CUtensorMap tmK, tmV;
     const long long rows = (long long)num_pages * n_kv * PAGE;
-    int r = page_map(&tmK, k, rows, hd, fp8);
-    if (!r) r = page_map(&tmV, v, rows, hd, fp8);
+    int r = page_map(&tmK, k, rows, hd, fp8, pl.rows == 128);
+    if (!r) r = page_map(&tmV, v, rows, hd, fp8, pl.rows == 128);
     if (r) return r;
     TreeParams p;
     p.q = (const bf16*)q;
@@ -871,14 +778,12 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
     p.max_ctx = max_ctx;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.status = status;
-#define TREE(F, D)                                                             \
-    {                                                                          \
-        if (pl.rows == 16) return launch_tree<F, D, 1>(tmK, tmV, p, pl, zero_tail, st); \
-        return launch_tree<F, D, 2>(tmK, tmV, p, pl, zero_tail, st);           \
-    }
-    if (fp8) {
-        if (hd == 128) TREE(true, 128) else TREE(true, 64)
-    }
-    if (hd == 128) TREE(false, 128) else TREE(false, 64)
+#define TREE(F, D) r = pl.rows == 16 ? launch_tree<F, D, 1>(tmK, tmV, p, pl, st) : launch_tree<F, D, 2>(tmK, tmV, p, pl, st)
+    if (pl.rows == 128) r = launch_tile(tmK, tmV, p, hd, fp8, pl.grid, st);
+    else if (fp8 && hd == 128) TREE(true, 128);
+    else if (fp8) TREE(true, 64);
+    else if (hd == 128) TREE(false, 128);
+    else TREE(false, 64);
 #undef TREE
+    return r ? r : merge(p, hd, pl.rows, pl.tile, pl.grid, pl.wide, zero_tail, st);
 }

@@ -310,13 +310,15 @@ TREE_CASES = [  # heads, kv heads, head size, rows per sequence, tokens per sequ
     (1, 1, 64, [1], [1], False), (4, 2, 128, [1, 1, 1], [1, 17, 300], False), (6, 2, 128, [5, 0, 3], [5, 9, 128], True),
     (3, 1, 64, [64], [64], True), (8, 8, 64, [2, 7], [130, 63], True), (24, 8, 128, [8], [301], True), (5, 1, 128, [13, 1], [257, 129], True),
     (16, 2, 128, [33], [65], False), (12, 4, 64, [16, 16], [1023, 31], True), (8, 1, 128, [64, 64], [640, 66], True),
+    (24, 2, 64, [3, 1, 6], [900, 3, 128], True), (64, 1, 128, [1, 2], [129, 384], False),
 ]
 TREE_PLAIN_CASES = [(2, 1, 80, [3, 1], [40, 7], True), (3, 3, 16, [1], [200], False), (4, 2, 256, [9], [77], True)]
 
 
-def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128):
-    """A drafted token whose keys or values are not finite reaches the rows that see it and no other."""
-    H, G, sizes, lens = 4, 2, [6, 2], [70, 33]
+def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128, H=4, G=2):
+    """A drafted token whose keys or values are not finite reaches the rows that see it and no other; of its values, in a row that sees
+    it, only the dimensions that are not finite are lost."""
+    sizes, lens = [6, 2], [70, 33]
     masks = [1, 3, 5, 11, 21, 33, 1, 3]
     c = tree_case(H, G, hd, sizes, lens, fp8, dtype, 11)
     clean = run_tree(ops, device, c, masks, 0.1).cpu()
@@ -337,11 +339,21 @@ def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128)
             rest = [0, 2, 4, 5, 6, 7]
             assert torch.equal(got[rest], clean[rest]), (name, what)
             assert not bool(torch.isfinite(got[hit]).all(-1).any()), (name, what)
+    if not fp8:
+        d = {**c, "v": c["v"].clone()}
+        d["v"][page, :, off, 3] = math.inf
+        got = run_tree(ops, device, d, masks, 0.1).cpu().view(-1, H, hd)
+        want, mass = plain_tree(c["q"], _dense(c["k"]), _dense(c["v"]), c["table"].tolist(), lens, c["cu"], 0.1, masks)
+        tol = tree_tolerance(c, want, mass, 0.1)
+        dims = [i for i in range(hd) if i != 3]
+        assert torch.equal(got[[0, 2, 4, 5, 6, 7]], clean.view(-1, H, hd)[[0, 2, 4, 5, 6, 7]])
+        assert bool((got[hit][..., 3] == math.inf).all())
+        assert bool(((got[hit].to(F64) - want[hit]).abs() <= tol[hit])[..., dims].all())
 
 
-def check_tree_bad_sequences(ops, device, fp8):
+def check_tree_bad_sequences(ops, device, fp8, H=4, G=2):
     """Sequences that break the rules get zero rows, tokens on pages that are not there are not seen; the other sequences are as ever."""
-    H, G, hd = 4, 2, 64
+    hd = 64
     c = tree_case(H, G, hd, [2, 3, 1, 2], [40, 2, 50, 90], fp8, torch.bfloat16, 5)      # 3 rows in 2 tokens
     c["table"][2, 1] = c["k"].shape[0]                              # page past the cache: tokens 16 .. 31 of sequence 2
     c["table"][2, 2] = -1

@@ -32,11 +32,13 @@ def test_tree_attention(case, fp8):
 @pytest.mark.parametrize("fp8", [False, True])
 def test_masked_tokens_that_are_not_finite(fp8):
     cases.check_tree_masked_not_finite(TORCH_OPS, "cpu", fp8, torch.float32)
+    cases.check_tree_masked_not_finite(TORCH_OPS, "cpu", fp8, torch.float32, 64, 32, 2)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
 def test_bad_sequences(fp8):
     cases.check_tree_bad_sequences(TORCH_OPS, "cpu", fp8)
+    cases.check_tree_bad_sequences(TORCH_OPS, "cpu", fp8, 64, 2)
 
 
 @pytest.mark.parametrize("case", cases.INT4_QUANT_CASES, ids=str)

@@ -87,15 +87,17 @@ def test_tree_attention(case, fp8, dtype):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fp8", [False, True])
-def test_masked_tokens_that_are_not_finite(fp8, dtype):
-    cases.check_tree_masked_not_finite(get_ops("cuda"), "cuda", fp8, dtype)
-    cases.check_tree_masked_not_finite(get_ops("cuda"), "cuda", fp8, dtype, hd=64)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H", [4, 10, 32])                # 12, 30 and 96 rows per KV head: the three forms of the kernel
+def test_masked_tokens_that_are_not_finite(fp8, dtype, hd, H):
+    cases.check_tree_masked_not_finite(get_ops("cuda"), "cuda", fp8, dtype, hd, H, 2)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-def test_bad_sequences(fp8):
+@pytest.mark.parametrize("H", [4, 16, 64])
+def test_bad_sequences(fp8, H):
     ops = get_ops("cuda")
-    cases.check_tree_bad_sequences(ops, "cuda", fp8)
+    cases.check_tree_bad_sequences(ops, "cuda", fp8, H, 2)
     with pytest.raises(KernelError, match="status 6"):
         ops.check_status()
     ops.check_status()
