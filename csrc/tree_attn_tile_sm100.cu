@@ -31,6 +31,7 @@ using namespace tree;
 constexpr int TT = 128, THREADS = 480;
 constexpr int W_VAL = 8, W_MMA = 12, W_K = 13, W_V = 14;
 constexpr float GROW = 8.0f;                           // log2 units
+constexpr int EMU = 2;                                 // of every 4 pairs of exponentials, this many run on the FMA pipe
 constexpr int HALF = TT * 128;                         // 128 tokens x 128 bytes: 16 KB
 
 template <bool FP8, int HD>
@@ -40,10 +41,11 @@ struct Lay {
     static constexpr int PIECE = TT * ROWB;            // one half of a staged tile
     static constexpr int KT = HALVES * PIECE;          // a staged tile of keys (or of values)
     static constexpr int VT = HD / 64 * HALF;          // a 16-bit value tile
-    static constexpr int KST = FP8 ? 4 : 3, RST = FP8 ? 3 : 2;       // stages of keys, of staged values (bf16: the operand tiles themselves)
-    static constexpr int RING = KST * KT + RST * KT + (FP8 ? 2 * VT : 0);
+    // stages of keys, of staged values, of value operand tiles (bf16: the staged tiles themselves)
+    static constexpr int KST = FP8 ? 4 : 3, RST = 3, VST = FP8 ? 2 : RST;
+    static constexpr int RING = KST * KT + RST * KT + (FP8 ? VST * VT : 0);
     static constexpr int EXPS = FP8 ? RST * 2 * TT : 0;
-    static constexpr int FACT = FP8 ? 2 * 2 * TT * 4 : 0;
+    static constexpr int FACT = FP8 ? VST * 2 * TT * 4 : 0;
     static constexpr int ROWBUF = 6 * TT * 4;
     static constexpr int SMEM = 1024 + RING + EXPS + FACT + ROWBUF;
 };
@@ -61,6 +63,13 @@ __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
 __device__ __forceinline__ float2 f16x2_to_float(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+// eight bf16 numbers of a query row (rows are 8-byte aligned)
+__device__ __forceinline__ uint4 ld_row(const bf16* p) {
+    const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 4);
+    return make_uint4(a.x, a.y, b.x, b.y);
+}
+__device__ __forceinline__ uint32_t largest(uint32_t two) { return max(two & 0x7fffu, (two >> 16) & 0x7fffu); }
 
 struct TileMeta {                                      // of an operand stage
     uint32_t valid[4], odd[4];                         // bits of the tile's tokens: exist; drafted with values that are not finite
@@ -81,10 +90,11 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     float* row_buf = reinterpret_cast<float*>(exps + L::EXPS + L::FACT);   // [2 parities][2 halves][TT] maxima, then [2 halves][TT] sums
     __shared__ int uoff[MAX_B + 1];
     __shared__ int wsum[THREADS / 32];
-    __shared__ uint64_t k_full[L::KST], k_empty[L::KST], r_full[L::RST], r_empty[L::RST], v_ready[2], pv_done[2], s_full[2], p_ready[2], q_ready[2],
+    __shared__ uint64_t k_full[L::KST], k_empty[L::KST], r_full[L::RST], r_empty[L::RST], v_ready[L::VST], pv_done[L::VST], s_full[2], p_ready[2], q_ready[2],
         xch, slow;
     __shared__ uint32_t there[L::RST];                 // bit per page of the staged values: loaded
-    __shared__ TileMeta meta[2];
+    __shared__ uint32_t there_k[8];                    // the same of key tile j % 8 (the softmax is less than eight tiles behind the loads)
+    __shared__ TileMeta meta[L::VST];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
@@ -92,9 +102,8 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::KST; ++i) { tc::mbar_init(&k_full[i], 1); tc::mbar_init(&k_empty[i], 1); }
         for (int i = 0; i < L::RST; ++i) { tc::mbar_init(&r_full[i], 1); tc::mbar_init(&r_empty[i], 4); }
+        for (int i = 0; i < L::VST; ++i) { tc::mbar_init(&v_ready[i], 4); tc::mbar_init(&pv_done[i], 1); }
         for (int i = 0; i < 2; ++i) {
-            tc::mbar_init(&v_ready[i], 4);
-            tc::mbar_init(&pv_done[i], 1);
             tc::mbar_init(&s_full[i], 1);
             tc::mbar_init(&p_ready[i], 8);
             tc::mbar_init(&q_ready[i], 4);
@@ -148,13 +157,14 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             fetch(j + 1);
             uint64_t* full = isv ? &r_full[st] : &k_full[st];
             if (isv && !FP8) {                         // the stage is the operand tile: free when its product has run
-                if (j >= 2) ok = tc::mbar_wait(&pv_done[st], (uint32_t)(use - 1) & 1u, abort_flag);
+                if (use > 0) ok = tc::mbar_wait(&pv_done[st], (uint32_t)(use - 1) & 1u, abort_flag);
             } else {
                 ok = tc::mbar_wait(isv ? &r_empty[st] : &k_empty[st], (uint32_t)(use & 1) ^ 1u, abort_flag);
             }
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             if (lane == 0) {
                 if (isv) there[st] = have;
+                else there_k[j % 8] = have;
                 tc::mbar_expect_tx(full, __popc(have) * (PAGE * L::ROW_BYTES + (FP8 && isv ? 2 * PAGE : 0)));
             }
             __syncwarp();
@@ -221,13 +231,13 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 o_len = og.t1 - og.t0;
                 o_at = 0;
             }
-            const int vs = j & 1;
-            ok = tc::mbar_wait(&v_ready[vs], (uint32_t)(j >> 1) & 1u, abort_flag) && tc::mbar_wait(&p_ready[vs], (uint32_t)(j >> 1) & 1u, abort_flag);
+            const int vs = j % L::VST;
+            ok = tc::mbar_wait(&v_ready[vs], (uint32_t)(j / L::VST) & 1u, abort_flag) && tc::mbar_wait(&p_ready[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag);
             if (!ok) break;
             tc::tc_fence_after();
             // a first tile overwrites O, unless the softmax warps have begun it (values that are not finite)
             const uint32_t acc = o_at > 0 || (meta[vs].odd[0] | meta[vs].odd[1] | meta[vs].odd[2] | meta[vs].odd[3]) ? 1u : 0u;
-            const uint32_t b_lo = dv.lo + vs * (L::VT >> 4), a = tmem0 + vs * 128;
+            const uint32_t b_lo = dv.lo + vs * (L::VT >> 4), a = tmem0 + (j & 1) * 128;
             if (tc::elect_one()) {
 #pragma unroll
                 for (int k = 0; k < TT / 16; ++k) tc::mma_f16_ts_h(tmem_oacc, a + 8 * k, b_lo + (k * 2048 >> 4), dv.hi, id_o, k == 0 ? acc : 1u);
@@ -247,41 +257,53 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             const bool live = R < sg.n * p.G;
             const bf16* src = p.q + (long long)((p.cu ? p.cu[sg.b] : sg.b) + (live ? R / p.G : 0)) * p.q_stride + (long long)(sg.h * p.G + (live ? R % p.G : 0)) * HD;
             const uint32_t dst = tmem_q + (seg & 1) * 64 + lane_base;
-            uint32_t w[HD / 2];
-#pragma unroll
-            for (int i = 0; i < HD / 4; ++i) {
-                const uint2 v = live ? *reinterpret_cast<const uint2*>(src + i * 4) : make_uint2(0u, 0u);
-                w[2 * i] = v.x;
-                w[2 * i + 1] = v.y;
-            }
             if constexpr (FP8) {
                 uint32_t big = 0;
 #pragma unroll
-                for (int i = 0; i < HD / 2; ++i) big = max(big, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+                for (int i = 0; i < HD / 8; ++i) {
+                    const uint4 v = live ? ld_row(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
+                    big = max(big, max(max(largest(v.x), largest(v.y)), max(largest(v.z), largest(v.w))));
+                }
                 // the largest number comes to [2^7, 2^8); a row that is not finite becomes NaN
                 const float inv = big >= 0x7f80u ? __uint_as_float(0x7fc00000u) : pow2_biased(min(254 - (int)(big >> 7) + 7, 254));
-                uint32_t q8[2][HD / 4];
 #pragma unroll
-                for (int i = 0; i < HD / 4; ++i) {
-                    uint32_t hi2[2], lo2[2];
+                for (int c = 0; c < HD / 32; ++c) {    // 32 numbers: eight columns of hi, eight of lo
+                    uint32_t hi8[8], lo8[8];
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float a = __uint_as_float(w[2 * i + e] << 16) * inv, b = __uint_as_float(w[2 * i + e] & 0xffff0000u) * inv;
-                        hi2[e] = e4m3x2(a, b);
-                        const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)hi2[e], __NV_E4M3)));
-                        lo2[e] = e4m3x2(a - back.x, b - back.y);
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 v = live ? ld_row(src + c * 32 + i * 8) : make_uint4(0u, 0u, 0u, 0u);
+                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            uint32_t h2[2], l2[2];
+#pragma unroll
+                            for (int z = 0; z < 2; ++z) {
+                                const float a = __uint_as_float(w[2 * e + z] << 16) * inv, b = __uint_as_float(w[2 * e + z] & 0xffff0000u) * inv;
+                                h2[z] = e4m3x2(a, b);
+                                const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h2[z], __NV_E4M3)));
+                                l2[z] = e4m3x2(a - back.x, b - back.y);
+                            }
+                            hi8[2 * i + e] = h2[0] | h2[1] << 16;
+                            lo8[2 * i + e] = l2[0] | l2[1] << 16;
+                        }
                     }
-                    q8[0][i] = hi2[0] | hi2[1] << 16;
-                    q8[1][i] = lo2[0] | lo2[1] << 16;
-                }
-#pragma unroll
-                for (int s = 0; s < 2; ++s) {
-                    if constexpr (HD == 128) tc::tmem_st32(dst + 32 * s, q8[s]);
-                    else tc::tmem_st16(dst + 32 * s, q8[s]);
+                    tc::tmem_st8(dst + 8 * c, hi8);
+                    tc::tmem_st8(dst + 32 + 8 * c, lo8);
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < HD / 2; c += 32) tc::tmem_st32(dst + c, w + c);
+                for (int c = 0; c < HD / 32; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint4 v = live ? ld_row(src + c * 32 + i * 8) : make_uint4(0u, 0u, 0u, 0u);
+                        w[4 * i] = v.x;
+                        w[4 * i + 1] = v.y;
+                        w[4 * i + 2] = v.z;
+                        w[4 * i + 3] = v.w;
+                    }
+                    tc::tmem_st16(dst + 16 * c, w);
+                }
             }
             tc::tmem_st_wait();
             tc::tc_fence_before();
@@ -291,20 +313,22 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         Segment sg = segment(0);
         int at = 0, seg = 0, loaded = 0, E = 0;        // tile within the segment, its number; segments whose queries are loaded
         for (int j = 0; j < n_tiles; ++j, ++at) {
-            const int vs = j & 1, rst = j % L::RST;
+            const int vs = j % L::VST, rst = j % L::RST;
             if (at == sg.t1 - sg.t0) {
                 sg = segment(j);
                 at = 0;
                 ++seg;
             }
-            if (j >= 2) ok = tc::mbar_wait(&pv_done[vs], (uint32_t)((j >> 1) - 1) & 1u, abort_flag);
+            // FP8: the operand stage is free when the product two tiles back has run
+            const bool ahead = at == 1 && loaded == seg + 1 && j - at + (sg.t1 - sg.t0) < n_tiles;
+            if (j >= 2 && (FP8 || loaded <= seg || ahead))
+                ok = tc::mbar_wait(&pv_done[(j - 2) % L::VST], (uint32_t)((j - 2) / L::VST) & 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            // queries of this unit, or of the next one once the products of the unit before this one (the buffer's last reader) have run
             if (loaded <= seg) {
                 load_queries(sg, seg);
                 loaded = seg + 1;
-            }
-            // the next unit's queries, once the products of the unit before this one (the buffer's last reader) have run
-            if (at == 1 && loaded == seg + 1 && j - at + (sg.t1 - sg.t0) < n_tiles) {
+            } else if (ahead) {
                 load_queries(segment(j - at + (sg.t1 - sg.t0)), seg + 1);
                 loaded = seg + 2;
             }
@@ -421,21 +445,19 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             float m_used = -INFINITY, l = 0.f;
             int E = 0;
             for (int at = 0; at < sg.t1 - sg.t0; ++at, ++j) {
-                const int vs = j & 1, base = (sg.t0 + at) * TT;
-                const uint32_t tmem_s = tmem0 + vs * 128 + lane_base;
-                const uint32_t phase = (uint32_t)(j >> 1) & 1u;
-                if (!tc::mbar_wait(&s_full[vs], phase, abort_flag)) { ok = false; break; }
+                const int vs = j % L::VST, base = (sg.t0 + at) * TT;
+                const uint32_t tmem_s = tmem0 + (j & 1) * 128 + lane_base;
+                if (!tc::mbar_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag)) { ok = false; break; }
                 tc::tc_fence_after();
-                // what exists is known with the value tile; without factors only the tiles at the end of a context ask
-                const bool drafts = base + TT > prefix;
-                if (!tc::mbar_wait(&v_ready[vs], phase, abort_flag)) { ok = false; break; }
+                // tiles with drafted tokens, with the end of the context, or with pages that are not there
+                const bool edge = base + TT > prefix || there_k[j % 8] != 0xffu;
+                if ((FP8 || edge) && !tc::mbar_wait(&v_ready[vs], (uint32_t)(j / L::VST) & 1u, abort_flag)) { ok = false; break; }
                 const TileMeta& mt = meta[vs];
-                const uint32_t odd_any = mt.odd[0] | mt.odd[1] | mt.odd[2] | mt.odd[3];
-                const unsigned long long exist = (unsigned long long)mt.valid[2 * hf] | (unsigned long long)mt.valid[2 * hf + 1] << 32;
-                const bool whole = (mt.valid[0] & mt.valid[1] & mt.valid[2] & mt.valid[3]) == 0xffffffffu;
+                uint32_t odd_any = 0;
+                unsigned long long seen = ~0ull;
                 float s[64];
                 float mx = -INFINITY;
-                unsigned long long seen = ~0ull;
+                if (edge) odd_any = mt.odd[0] | mt.odd[1] | mt.odd[2] | mt.odd[3];
                 if (live) {
                     tc::tmem_ld32(tmem_s + hf * 64, reinterpret_cast<uint32_t*>(s));
                     tc::tmem_ld32(tmem_s + hf * 64 + 32, reinterpret_cast<uint32_t*>(s + 32));
@@ -445,14 +467,17 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
                         for (int c = 0; c < 64; c += 4) {
                             const float4 f = *reinterpret_cast<const float4*>(kf + c);
-                            s[c] *= f.x;
-                            s[c + 1] *= f.y;
-                            s[c + 2] *= f.z;
-                            s[c + 3] *= f.w;
+                            const float2 a = __fmul2_rn(make_float2(s[c], s[c + 1]), make_float2(f.x, f.y));
+                            const float2 b = __fmul2_rn(make_float2(s[c + 2], s[c + 3]), make_float2(f.z, f.w));
+                            s[c] = a.x;
+                            s[c + 1] = a.y;
+                            s[c + 2] = b.x;
+                            s[c + 3] = b.y;
                         }
                     }
-                    if (drafts || !whole) {
-                        seen = sees(p, c0, row_i, base + hf * 64 - prefix) & exist;
+                    if (edge) {
+                        seen = sees(p, c0, row_i, base + hf * 64 - prefix) &
+                               ((unsigned long long)mt.valid[2 * hf] | (unsigned long long)mt.valid[2 * hf + 1] << 32);
 #pragma unroll
                         for (int c = 0; c < 64; ++c) s[c] = (uint32_t)(seen >> c) & 1u ? s[c] : -INFINITY;
                     }
@@ -469,27 +494,27 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 }
                 // (also orders "both halves have read their scores" before either writes P over them)
                 if (!exchange(&xch, n_x)) { ok = false; break; }
-                const int E_new = FP8 ? mt.E : 0;
                 if (live) {
+                    const int E_new = FP8 ? mt.E : 0;
                     mx = fmaxf(mx, row_buf[((j & 1) * 2 + (hf ^ 1)) * TT + r]) * scale;
                     const bool grow = mx > m_used + GROW;
                     if (at == 0) {
                         m_used = mx;
                         E = E_new;
                     } else if (__any_sync(0xffffffffu, grow) || (FP8 && E_new != E)) {
-                        if (!tc::mbar_wait(&pv_done[vs ^ 1], (uint32_t)((j - 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
+                        if (!tc::mbar_wait(&pv_done[(j - 1) % L::VST], (uint32_t)((j - 1) / L::VST) & 1u, abort_flag)) { ok = false; break; }
                         tc::tc_fence_after();
                         const float m_new = fmaxf(m_used, mx);
                         const float f = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
                         const float fo = FP8 ? f * exp2f((float)(E - E_new)) : f;
 #pragma unroll 1
-                        for (int c = 0; c < HD / 2; c += 32) {
-                            uint32_t o[32];
-                            tc::tmem_ld32(tmem_o + hf * (HD / 2) + c, o);
+                        for (int c = 0; c < HD / 2; c += 16) {
+                            uint32_t o[16];
+                            tc::tmem_ld16(tmem_o + hf * (HD / 2) + c, o);
                             tc::tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fo);
-                            tc::tmem_st32(tmem_o + hf * (HD / 2) + c, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fo);
+                            tc::tmem_st16(tmem_o + hf * (HD / 2) + c, o);
                         }
                         tc::tmem_st_wait();
                         l *= f;
@@ -498,32 +523,44 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                     }
                     const float mb = m_used == -INFINITY ? 0.f : m_used;
                     const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-mb, -mb);
+                    if (edge) {                                // exponentials of -infinity have to be zero
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2);
+                            s[c] = exp2f(x.x);
+                            s[c + 1] = exp2f(x.y);
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 64; c += 2) {
+                            const float2 e = attn::exp2_pair<EMU>(__ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2), c >> 1);
+                            s[c] = e.x;
+                            s[c + 1] = e.y;
+                        }
+                    }
                     float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                     const float* wf = fact + vs * 2 * TT + TT + hf * 64;
-                    const bool exact = drafts || !whole;       // exponentials of -infinity have to be zero
 #pragma unroll
-                    for (int q4 = 0; q4 < 2; ++q4) {
-                        uint32_t pk[16];
+                    for (int q4 = 0; q4 < 4; ++q4) {
+                        uint32_t pk[8];
 #pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            const float2 x = __ffma2_rn(make_float2(s[q4 * 32 + c], s[q4 * 32 + c + 1]), sc2, nm2);
-                            float2 e;
-                            if (exact) e = make_float2(exp2f(x.x), exp2f(x.y));
-                            else e = attn::exp2_pair<FP8 ? 2 : 0>(x, c >> 1);
-                            sum2[(c >> 1) & 1] = __fadd2_rn(sum2[(c >> 1) & 1], e);
+                        for (int c = q4 * 16; c < q4 * 16 + 16; c += 4) {
+                            float2 a = make_float2(s[c], s[c + 1]), b = make_float2(s[c + 2], s[c + 3]);
+                            sum2[0] = __fadd2_rn(sum2[0], a);
+                            sum2[1] = __fadd2_rn(sum2[1], b);
                             if constexpr (FP8) {
-                                const float2 w = *reinterpret_cast<const float2*>(wf + q4 * 32 + c);
-                                e = __fmul2_rn(e, w);
-                                pk[c >> 1] = pack_f16(e.x, e.y);
-                            } else {
-                                pk[c >> 1] = pack_bf16(e.x, e.y);
+                                const float4 w = *reinterpret_cast<const float4*>(wf + c);
+                                a = __fmul2_rn(a, make_float2(w.x, w.y));
+                                b = __fmul2_rn(b, make_float2(w.z, w.w));
+                                s[c] = a.x;                    // (kept for the pass below)
+                                s[c + 1] = a.y;
+                                s[c + 2] = b.x;
+                                s[c + 3] = b.y;
                             }
-                            if (odd_any) {                     // kept for the pass below
-                                s[q4 * 32 + c] = e.x;
-                                s[q4 * 32 + c + 1] = e.y;
-                            }
+                            pk[(c >> 1) & 7] = FP8 ? pack_f16(a.x, a.y) : pack_bf16(a.x, a.y);
+                            pk[((c >> 1) & 7) + 1] = FP8 ? pack_f16(b.x, b.y) : pack_bf16(b.x, b.y);
                         }
-                        tc::tmem_st16(tmem_s + hf * 32 + q4 * 16, pk);
+                        tc::tmem_st8(tmem_s + hf * 32 + q4 * 8, pk);
                     }
                     l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
                     tc::tmem_st_wait();
@@ -531,7 +568,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 if (odd_any) {
                     // ---- values that are not finite: rows that see the token get its products here, the others never meet it
                     uint8_t* op = sV + vs * L::VT;
-                    if (live && at > 0 && !tc::mbar_wait(&pv_done[vs ^ 1], (uint32_t)((j - 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
+                    if (live && at > 0 && !tc::mbar_wait(&pv_done[(j - 1) % L::VST], (uint32_t)((j - 1) / L::VST) & 1u, abort_flag)) { ok = false; break; }
                     tc::tc_fence_after();
                     bool begun = at > 0;
                     for (int tk = 0; tk < TT; ++tk) {
@@ -547,19 +584,19 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                         if (live) {
                             const float pv = row_buf[4 * TT + r];
 #pragma unroll 1
-                            for (int c = 0; c < HD / 2; c += 32) {
-                                uint32_t o[32];
-                                tc::tmem_ld32(tmem_o + hf * (HD / 2) + c, o);
+                            for (int c = 0; c < HD / 2; c += 16) {
+                                uint32_t o[16];
+                                tc::tmem_ld16(tmem_o + hf * (HD / 2) + c, o);
                                 tc::tmem_ld_wait();
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) {
+                                for (int i = 0; i < 16; ++i) {
                                     const int d = hf * (HD / 2) + c + i;
                                     const uint16_t bits = *reinterpret_cast<const uint16_t*>(op + (d >> 6) * HALF + tk * 128 + ((((d & 63) >> 3) ^ (tk & 7)) << 4) + (d & 7) * 2);
                                     const float v = FP8 ? f16x2_to_float(bits).x : __uint_as_float((uint32_t)bits << 16);
                                     const float was = begun ? __uint_as_float(o[i]) : 0.f;
                                     o[i] = __float_as_uint(pv < 0.f ? was : was + pv * v);
                                 }
-                                tc::tmem_st32(tmem_o + hf * (HD / 2) + c, o);
+                                tc::tmem_st16(tmem_o + hf * (HD / 2) + c, o);
                             }
                             tc::tmem_st_wait();
                         }
@@ -572,14 +609,14 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 }
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&p_ready[vs]);
+                if (lane == 0) tc::mbar_arrive(&p_ready[j & 1]);
             }
             if (!ok) break;
             // ---- the unit's rows, as far as this part has them
             row_buf[(4 + hf) * TT + r] = l;
             if (!exchange(&xch, n_x)) { ok = false; break; }
             l += row_buf[(4 + (hf ^ 1)) * TT + r];
-            if (!tc::mbar_wait(&pv_done[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, abort_flag)) { ok = false; break; }
+            if (!tc::mbar_wait(&pv_done[(j - 1) % L::VST], (uint32_t)((j - 1) / L::VST) & 1u, abort_flag)) { ok = false; break; }
             tc::tc_fence_after();
             if (live) {
                 const bool done = sg.t0 == 0 && sg.t1 == sg.T, mine = R < M;
