@@ -19,7 +19,7 @@ struct TreeParams {
     const long long* masks;
     bf16* out;
     long long out_stride;
-    float* part_o;                                     // [2 * grid][ROWS][HD]
+    float* part_o;                                     // [2 * grid][HD / 4][ROWS][4]
     float* part_ml;                                    // [2 * grid][ROWS][2]
     int* uoff;                                         // [B + 1] tiles before each sequence, for the merge kernel
     int max_pages, num_pages, B, N, H, G, n_kv, max_q, max_ctx;

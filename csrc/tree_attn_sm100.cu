@@ -510,8 +510,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         const bool done = sg.t0 == 0 && sg.t1 == sg.T;
         const long long slot = 2ll * blockIdx.x + (sg.t0 == 0);
         for (int i = threadIdx.x; i < C::ROWS * (HD / 4); i += THREADS) {
-            const int row = i / (HD / 4), d = (i % (HD / 4)) * 4, R = row0 + row;
-            if (R >= M) break;
+            const int row = i % C::ROWS, d = i / C::ROWS * 4, R = row0 + row;
+            if (R >= M) continue;
             const float4 a = *reinterpret_cast<const float4*>(obuf + row * C::OROW + d);
             const float4 z = *reinterpret_cast<const float4*>(obuf + (C::ROWS + row) * C::OROW + d);
             float4 v = make_float4(a.x + z.x, a.y + z.y, a.z + z.z, a.w + z.w);
@@ -528,7 +528,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 bf16* dst = p.out + (long long)(c0 + R / p.G) * p.out_stride + (long long)(sg.h * p.G + R % p.G) * HD + d;
                 *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
             } else {
-                *reinterpret_cast<float4*>(p.part_o + (slot * C::ROWS + row) * HD + d) = v;
+                *reinterpret_cast<float4*>(p.part_o + ((slot * (HD / 4) + d / 4) * C::ROWS + row) * 4) = v;
                 if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * C::ROWS + row) * 2) = make_float2(top, sum);
             }
         }
@@ -600,7 +600,10 @@ tree_merge_kernel(const TreeParams p, int ROWS, int TILE, int grid, int zero_tai
                 const long long at = (2ll * j + (j == first)) * ROWS + r;
                 ml[u] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
 #pragma unroll
-                for (int e = 0; e < EPL; e += 2) *reinterpret_cast<float2*>(&v[u][e]) = *reinterpret_cast<const float2*>(p.part_o + at * HD + lane * EPL + e);
+                for (int e = 0; e < EPL; e += 2) {
+                    const int d = lane * EPL + e;
+                    *reinterpret_cast<float2*>(&v[u][e]) = *reinterpret_cast<const float2*>(p.part_o + (((2ll * j + (j == first)) * (HD / 4) + d / 4) * ROWS + r) * 4 + d % 4);
+                }
             }
         }
 #pragma unroll
@@ -735,15 +738,15 @@ KB_API long long kb_tree_attn_floats(int N, int B, int H, int n_kv, int hd, int 
     return 2ll * pl.grid * pl.rows * (hd + 2) + B + 4;
 }
 
-// As kb_tree_attn_plain for bf16 and heads of 64 and 128; query rows 8-byte, output rows 8-byte aligned; `work` has kb_tree_attn_floats
+// As kb_tree_attn_plain for bf16 and heads of 64 and 128; query rows 16-byte, output rows 8-byte aligned; `work` has kb_tree_attn_floats
 // floats (16-byte aligned).
 KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const void* ke, const void* v, const void* ve, const int* table, int max_pages,
                         int num_pages, const int* ctx_lens, const int* cu, int B, const long long* masks, void* out, long long out_stride, int N,
                         int H, int n_kv, int hd, int max_q, int max_ctx, float scale, int zero_tail, float* work, long long work_floats, int* status,
                         cudaStream_t st) {
     const bool fp8 = ke != nullptr;
-    if ((ke == nullptr) != (ve == nullptr) || q_stride % 4 || out_stride % 4 || max_pages < 1 || num_pages < 1 || !status ||
-        ((uintptr_t)k | (uintptr_t)v | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)work) % 16 || ((uintptr_t)q | (uintptr_t)out) % 8)
+    if ((ke == nullptr) != (ve == nullptr) || q_stride % 8 || out_stride % 4 || max_pages < 1 || num_pages < 1 || !status ||
+        ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)work) % 16 || (uintptr_t)out % 8)
         return 5;
     const long long need = kb_tree_attn_floats(N, B, H, n_kv, hd, max_q, max_ctx, num_pages, fp8);
     if (need == 0 || work_floats < need) return 5;

@@ -2,22 +2,24 @@
 // tcgen05.  The work is cut as in tree_attn_sm100.cu (units of 128 rows, all units' tiles one line, equal parts, merge kernel); here a
 // part is walked by one CTA per SM with a role per warp:
 //
-//   warps 0-7    softmax: two threads per row, 64 token columns each (the row's maximum and sum cross through shared memory)
-//   warps 8-11   values: thread t owns token t of the tile.  Query rows -> tensor memory at the start of a unit; what of the tile exists;
-//                8-bit pages: factors of the tokens, codes of the values -> f16 operand tile
+//   warps 0-7    softmax: two groups of four, group g has the tiles of parity g; one thread per row
+//   warps 8-11   values: 8-bit pages -> f16 operand tile; places that hold no token -> zero.  Query rows -> shared memory, a unit ahead
 //   warp 12      MMA issue (the whole warp walks the loop, one elected lane issues)
 //   warps 13, 14 TMA of keys and values, a page per lane
+//   warp 15      what of a tile exists; 8-bit pages: factors of the keys, unit of the values
 //
-//   S = Q K^T    A = queries in tensor memory, B = key tile in shared memory (K-major)
+//   S = Q K^T    both operands K-major in shared memory, one accumulator per group
 //                bf16 pages: kind::f16.  8-bit pages: kind::f8f6f4 on the codes as they lie in the cache; a query row, a power of two
 //                taken out, is the sum of two e4m3 numbers, hi + lo, which together hold bf16's eight bits (down to 2^-10 of the row's
 //                largest; below that the error is at most 2^-18 of the largest) - two products at twice the rate of one in 16 bits.
-//   softmax      in fp32, lazy rescaling (O moves only when a row's maximum grows by more than 2^8); P back to tensor memory in 16 bits
-//   O += P V     A = P in tensor memory, B = value tile in shared memory (MN-major).  8-bit pages: P is f16 and carries the token's
-//                power of two relative to E, the unit's largest so far, times 2^6 (2^14 with the 2^8 of lazy rescaling), so that it keeps
-//                eleven bits down to 2^-20 and is off by at most 2^-31 below; O is in units of 2^(E - 6).
+//   softmax      in fp32, a row at a time in one pass: exponentials against the maximum so far, which is renewed only when a
+//                score exceeds it by more than 2^11 (2^40 where P is bf16); P back to tensor memory in 16 bits
+//   O += P V     A = P in tensor memory, B = value tile in shared memory (MN-major), one accumulator per group, so that the groups
+//                need nothing from one another before the end of a unit.  8-bit pages: P is f16 in units of 2^-4 (at most 2^15 with the
+//                2^11 of lazy maxima: eleven bits down to 2^-18, off by at most 2^-29 below); the values' f16 carry the token's power
+//                of two relative to E, the unit's largest so far (off by at most 2^-39 of the largest); O is in units of 2^(E - 6).
 //
-// S is double-buffered: the scores of the next tile exist before the softmax of the current one ends.  Query rows are double-buffered by unit.
+// The groups run out of step: one computes while the products of the other run.  Query rows are double-buffered by unit.
 // Tokens that do not exist are masked in S and zeroed in the value tile (whatever the cache holds there).  Values of drafted tokens that
 // are not finite must not meet the zero probabilities of rows that do not see them: such tokens are taken out of the value tile and
 // added row by row (never in normal use).  All waits are bounded (status word on timeout).
@@ -28,10 +30,9 @@ namespace {
 
 using namespace tree;
 
-constexpr int TT = 128, THREADS = 480;
-constexpr int W_VAL = 8, W_MMA = 12, W_K = 13, W_V = 14;
-constexpr float GROW = 8.0f;                           // log2 units
-constexpr int EMU = 2;                                 // of every 4 pairs of exponentials, this many run on the FMA pipe
+constexpr int TT = 128, THREADS = 512;
+constexpr int W_VAL = 8, W_MMA = 12, W_K = 13, W_V = 14, W_META = 15;
+constexpr int SLOTS = 8;                               // tiles that the notes on tiles reach ahead of the softmax, and more
 constexpr int HALF = TT * 128;                         // 128 tokens x 128 bytes: 16 KB
 
 template <bool FP8, int HD>
@@ -42,36 +43,81 @@ struct Lay {
     static constexpr int KT = HALVES * PIECE;          // a staged tile of keys (or of values)
     static constexpr int VT = HD / 64 * HALF;          // a 16-bit value tile
     // stages of keys, of staged values, of value operand tiles (bf16: the staged tiles themselves)
-    static constexpr int KST = FP8 ? 4 : 3, RST = 3, VST = FP8 ? 2 : RST;
-    static constexpr int RING = KST * KT + RST * KT + (FP8 ? VST * VT : 0);
+    static constexpr int KST = 2, RST = FP8 ? 3 : 2, VST = 2;
+    static constexpr int QT = FP8 ? 2 * KT : KT;       // query tile (8-bit pages: hi, lo)
+    static constexpr int RING = KST * KT + RST * KT + (FP8 ? VST * VT : 0) + 2 * QT;
     static constexpr int EXPS = FP8 ? RST * 2 * TT : 0;
-    static constexpr int FACT = FP8 ? VST * 2 * TT * 4 : 0;
-    static constexpr int ROWBUF = 6 * TT * 4;
+    static constexpr int FACT = FP8 ? SLOTS * TT * 4 : 0;
+    static constexpr int ROWBUF = 4 * TT * 4;
     static constexpr int SMEM = 1024 + RING + EXPS + FACT + ROWBUF;
 };
 
-__device__ __forceinline__ void mma_f8_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
+__device__ __forceinline__ void mma_f8_h(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "setp.ne.b32 p, %5, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], [%1], db, %4, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %2};\n\t"
+        "mov.b64 db, {%3, %4};\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], da, db, %5, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
         : "memory");
+}
+// Whether a phase is over, without the suspension of a wait: the MMA warp mostly finds its barriers passed.
+__device__ __forceinline__ bool passed(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
 }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
     return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 __device__ __forceinline__ float2 f16x2_to_float(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
-// eight bf16 numbers of a query row (rows are 8-byte aligned)
-__device__ __forceinline__ uint4 ld_row(const bf16* p) {
-    const uint2 a = *reinterpret_cast<const uint2*>(p), b = *reinterpret_cast<const uint2*>(p + 4);
-    return make_uint4(a.x, a.y, b.x, b.y);
-}
 __device__ __forceinline__ uint32_t largest(uint32_t two) { return max(two & 0x7fffu, (two >> 16) & 0x7fffu); }
 
-struct TileMeta {                                      // of an operand stage
+// Columns of tensor memory (a row per lane) times f: fp32 accumulators, packed probabilities.
+__device__ __noinline__ void scale_columns(uint32_t addr, int n, float f) {
+#pragma unroll 1
+    for (int c = 0; c < n; c += 32) {
+        uint32_t o[32];
+        tc::tmem_ld32(addr + c, o);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+        tc::tmem_st32(addr + c, o);
+    }
+    tc::tmem_st_wait();
+}
+template <bool F16>
+__device__ __noinline__ void scale_packed(uint32_t addr, int n, float f) {
+    tc::tmem_st_wait();
+#pragma unroll 1
+    for (int c = 0; c < n; c += 16) {
+        uint32_t o[16];
+        tc::tmem_ld16(addr + c, o);
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const float2 v = F16 ? f16x2_to_float(o[i]) : make_float2(__uint_as_float(o[i] << 16), __uint_as_float(o[i] & 0xffff0000u));
+            o[i] = F16 ? pack_f16(v.x * f, v.y * f) : pack_bf16(v.x * f, v.y * f);
+        }
+        tc::tmem_st16(addr + c, o);
+    }
+    tc::tmem_st_wait();
+}
+
+struct TileMeta {
     uint32_t valid[4], odd[4];                         // bits of the tile's tokens: exist; drafted with values that are not finite
     int E;                                             // biased exponent of the output's unit (8-bit pages)
 };
@@ -86,30 +132,33 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     uint8_t* sR = sK + L::KST * L::KT;                                 // staged values
     uint8_t* sV = FP8 ? sR + L::RST * L::KT : sR;                      // value operand tiles
     uint8_t* exps = smem + L::RING;                                    // [RST][2][TT] exponents of keys and values
-    float* fact = reinterpret_cast<float*>(exps + L::EXPS);            // [2][2][TT] factors of scores and probabilities
-    float* row_buf = reinterpret_cast<float*>(exps + L::EXPS + L::FACT);   // [2 parities][2 halves][TT] maxima, then [2 halves][TT] sums
+    float* fact = reinterpret_cast<float*>(exps + L::EXPS);            // [SLOTS][TT] factors of scores
+    uint8_t* sQ = smem + L::RING - 2 * L::QT;                          // two query tiles, staged like keys
+    float* row_buf = reinterpret_cast<float*>(exps + L::EXPS + L::FACT);   // [2 groups][TT] maxima, then sums
     __shared__ int uoff[MAX_B + 1];
     __shared__ int wsum[THREADS / 32];
-    __shared__ uint64_t k_full[L::KST], k_empty[L::KST], r_full[L::RST], r_empty[L::RST], v_ready[L::VST], pv_done[L::VST], s_full[2], p_ready[2], q_ready[2],
-        xch, slow;
+    __shared__ uint64_t k_full[L::KST], k_empty[L::KST], r_full[L::RST], r_empty[L::RST], v_ready[L::VST], f_ready[SLOTS], pv_done[L::VST], s_full[2], p_ready[2], q_ready[2],
+        xch, slow[2];
     __shared__ uint32_t there[L::RST];                 // bit per page of the staged values: loaded
-    __shared__ uint32_t there_k[8];                    // the same of key tile j % 8 (the softmax is less than eight tiles behind the loads)
-    __shared__ TileMeta meta[L::VST];
+    __shared__ uint32_t there_k[SLOTS];                // the same of key tile j % SLOTS
+    __shared__ TileMeta meta[SLOTS];                   // of tile j at j % SLOTS
     __shared__ uint32_t tmem_slot;
+    __shared__ int unit_E[2];
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < L::KST; ++i) { tc::mbar_init(&k_full[i], 1); tc::mbar_init(&k_empty[i], 1); }
-        for (int i = 0; i < L::RST; ++i) { tc::mbar_init(&r_full[i], 1); tc::mbar_init(&r_empty[i], 4); }
+        for (int i = 0; i < L::RST; ++i) { tc::mbar_init(&r_full[i], 1); tc::mbar_init(&r_empty[i], 5); }
         for (int i = 0; i < L::VST; ++i) { tc::mbar_init(&v_ready[i], 4); tc::mbar_init(&pv_done[i], 1); }
+        for (int i = 0; i < SLOTS; ++i) tc::mbar_init(&f_ready[i], 1);
         for (int i = 0; i < 2; ++i) {
             tc::mbar_init(&s_full[i], 1);
-            tc::mbar_init(&p_ready[i], 8);
+            tc::mbar_init(&p_ready[i], 4);
             tc::mbar_init(&q_ready[i], 4);
+            tc::mbar_init(&slow[i], 4);
         }
         tc::mbar_init(&xch, 8);
-        tc::mbar_init(&slow, 8);
         abort_word = 0;
         tc::fence_barrier_init();
         tc::prefetch_tmap(&tmK);
@@ -124,7 +173,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     tc::tc_fence_before();
     count_tiles<TT, TT, THREADS>(p, uoff, wsum);       // (has the block's barriers)
     tc::tc_fence_after();
-    const uint32_t tmem0 = tmem_slot, tmem_oacc = tmem0 + 256, tmem_q = tmem0 + 384;       // S: two times 128 columns; Q: two times 64
+    const uint32_t tmem0 = tmem_slot, tmem_oacc = tmem0 + 256;             // S: two times 128 columns; O: two times HD
     const int2 part = part_of_line(uoff[p.B]);
     const int lo = part.x, n_tiles = part.y - part.x;
     auto segment = [&](int j) { return segment_at<TT, TT>(p, uoff, lo + j, lo + n_tiles); };
@@ -164,7 +213,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             if (lane == 0) {
                 if (isv) there[st] = have;
-                else there_k[j % 8] = have;
+                else there_k[j % SLOTS] = have;
                 tc::mbar_expect_tx(full, __popc(have) * (PAGE * L::ROW_BYTES + (FP8 && isv ? 2 * PAGE : 0)));
             }
             __syncwarp();
@@ -188,33 +237,40 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         // ------------------------------------------------------------ products
         const uint32_t id_s = FP8 ? (1u << 4) | (uint32_t)(TT >> 3) << 17 | (uint32_t)(TT >> 4) << 24 : tc::instr_desc_f16(TT, TT, 1, 1, 0, 0);
         const uint32_t id_o = tc::instr_desc_f16(TT, HD, FP8 ? 0 : 1, FP8 ? 0 : 1, 0, 1);
-        tc::DescHalves dk = tc::smem_desc_halves(smem_u32(sK), 16, L::ROWB * 8);
-        if (L::ROWB == 64) dk.hi = (dk.hi & ~(7u << 29)) | 4u << 29;       // rows of 64 bytes: 64-byte swizzle
+        tc::DescHalves dk = tc::smem_desc_halves(smem_u32(sK), 16, L::ROWB * 8), dq = tc::smem_desc_halves(smem_u32(sQ), 16, L::ROWB * 8);
+        if (L::ROWB == 64) dq.hi = dk.hi = (dk.hi & ~(7u << 29)) | 4u << 29;       // rows of 64 bytes: 64-byte swizzle
         const tc::DescHalves dv = tc::smem_desc_halves(smem_u32(sV), HALF, 1024);
         Segment sg = segment(0);
         int s_left = sg.t1 - sg.t0, s_seg = 0;         // tiles of the segment that S is at; its number
+        bool s_new = true;                             // its queries have not been waited for
+        auto wait = [&](uint64_t* bar, uint32_t parity) { return passed(bar, parity) || tc::mbar_wait(bar, parity, abort_flag); };
         auto scores = [&](int j) {                     // S(j): waits for its queries and keys
             if (s_left == 0) {
                 sg = segment(j);
                 s_left = sg.t1 - sg.t0;
                 ++s_seg;
+                s_new = true;
             }
             --s_left;
             const int st = j % L::KST;
-            if (!tc::mbar_wait(&q_ready[s_seg & 1], (uint32_t)(s_seg >> 1) & 1u, abort_flag)) return false;
-            if (!tc::mbar_wait(&k_full[st], (uint32_t)(j / L::KST) & 1u, abort_flag)) return false;
+            if (s_new && !wait(&q_ready[s_seg & 1], (uint32_t)(s_seg >> 1) & 1u)) return false;
+            s_new = false;
+            if (!wait(&k_full[st], (uint32_t)(j / L::KST) & 1u)) return false;
             tc::tc_fence_after();
-            const uint32_t b_lo = dk.lo + st * (L::KT >> 4), aq = tmem_q + (s_seg & 1) * 64, d = tmem0 + (j & 1) * 128;
+            const uint32_t b_lo = dk.lo + st * (L::KT >> 4), a_lo = dq.lo + (s_seg & 1) * (L::QT >> 4), d = tmem0 + (j & 1) * 128;
             if (tc::elect_one()) {
                 if constexpr (FP8) {
 #pragma unroll
-                    for (int k = 0; k < HD / 32; ++k) mma_f8_ts(d, aq + 8 * k, b_lo + (k * 32 >> 4), dk.hi, id_s, k != 0);
+                    for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int k = 0; k < HD / 32; ++k) mma_f8_ts(d, aq + 32 + 8 * k, b_lo + (k * 32 >> 4), dk.hi, id_s, 1u);
+                        for (int k = 0; k < HD / 32; ++k)
+                            mma_f8_h(d, a_lo + ((i * L::KT + k * 32) >> 4), dq.hi, b_lo + (k * 32 >> 4), dk.hi, id_s, (i | k) != 0);
                 } else {
 #pragma unroll
-                    for (int k = 0; k < HD / 16; ++k)
-                        tc::mma_f16_ts_h(d, aq + 8 * k, b_lo + (((k >> 2) * HALF + (k & 3) * 32) >> 4), dk.hi, id_s, k != 0);
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint32_t off = ((k >> 2) * HALF + (k & 3) * 32) >> 4;
+                        tc::mma_f16_h(d, a_lo + off, dq.hi, b_lo + off, dk.hi, id_s, k != 0);
+                    }
                 }
                 tc::tc_commit(&s_full[j & 1]);
                 tc::tc_commit(&k_empty[st]);
@@ -232,15 +288,16 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 o_at = 0;
             }
             const int vs = j % L::VST;
-            ok = tc::mbar_wait(&v_ready[vs], (uint32_t)(j / L::VST) & 1u, abort_flag) && tc::mbar_wait(&p_ready[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag);
+            ok = wait(&v_ready[vs], (uint32_t)(j / L::VST) & 1u) && wait(&p_ready[j & 1], (uint32_t)(j >> 1) & 1u);
             if (!ok) break;
             tc::tc_fence_after();
-            // a first tile overwrites O, unless the softmax warps have begun it (values that are not finite)
-            const uint32_t acc = o_at > 0 || (meta[vs].odd[0] | meta[vs].odd[1] | meta[vs].odd[2] | meta[vs].odd[3]) ? 1u : 0u;
+            // a group's first tile overwrites its O, unless the softmax warps have begun it (values that are not finite)
+            const TileMeta& mt = meta[j % SLOTS];
+            const uint32_t acc = o_at > 1 || (mt.odd[0] | mt.odd[1] | mt.odd[2] | mt.odd[3]) ? 1u : 0u;
             const uint32_t b_lo = dv.lo + vs * (L::VT >> 4), a = tmem0 + (j & 1) * 128;
             if (tc::elect_one()) {
 #pragma unroll
-                for (int k = 0; k < TT / 16; ++k) tc::mma_f16_ts_h(tmem_oacc, a + 8 * k, b_lo + (k * 2048 >> 4), dv.hi, id_o, k == 0 ? acc : 1u);
+                for (int k = 0; k < TT / 16; ++k) tc::mma_f16_ts_h(tmem_oacc + (j & 1) * HD, a + 8 * k, b_lo + (k * 2048 >> 4), dv.hi, id_o, k == 0 ? acc : 1u);
                 tc::tc_commit(&pv_done[vs]);
             }
             __syncwarp();
@@ -248,31 +305,92 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             if (j + 2 < n_tiles) ok = scores(j + 2);
         }
         if (!ok && lane == 0) atomicMax(p.status, (int)KB_TIMEOUT_MMA);
+    } else if (warp == W_META) {
+        // ------------------------------------------------------------ what of a tile exists, which drafted tokens are odd, factors
+        Segment sg = segment(0);
+        int first = 0;                                 // tile at which sg begins
+        uint32_t E = 0;
+        for (int j = 0; j < n_tiles; ++j) {
+            if (j - first == sg.t1 - sg.t0) {
+                sg = segment(j);
+                first = j;
+            }
+            const int rst = j % L::RST;
+            // (slot j % SLOTS is free: the load of tile j waited for the conversion, and with it the product, of tiles less than SLOTS back)
+            ok = tc::mbar_wait(&r_full[rst], (uint32_t)(j / L::RST) & 1u, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            const int base = (sg.t0 + j - first) * TT, prefix = sg.ctx - sg.n;
+            const uint32_t have = there[rst];
+            const bool edge = have != 0xffu || base + TT > prefix;
+            const uint8_t* e = exps + rst * 2 * TT;
+            TileMeta& mt = meta[j % SLOTS];
+            uint32_t top = 0;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {              // 32 tokens at a time
+                const int t = w * 32 + lane, tok = base + t;
+                const bool valid = !edge || (tok < sg.ctx && (have >> (t / PAGE) & 1u));
+                if constexpr (FP8) {
+                    fact[(j % SLOTS) * TT + t] = pow2_biased(e[t]);
+                    const uint32_t ev = e[TT + t];
+                    if (valid && ev != 255u) top = max(top, ev);
+                }
+                uint32_t vword = 0xffffffffu, oword = 0u;
+                if (edge) {
+                    vword = __ballot_sync(0xffffffffu, valid);
+                    const uint8_t* raw = sR + rst * L::KT + t * L::ROWB;
+                    bool bad = false;
+                    if (valid && tok >= prefix)
+                        for (int h = 0; h < L::HALVES; ++h)
+                            for (int c = 0; c < L::ROWB / 16; ++c) {
+                                const uint4 v = *reinterpret_cast<const uint4*>(raw + h * L::PIECE + c * 16);
+                                const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                                for (int q = 0; q < 4; ++q)
+                                    bad |= FP8 ? __vcmpeq4(x[q] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u : __vcmpeq2(x[q] & 0x7f807f80u, 0x7f807f80u) != 0u;
+                            }
+                    oword = __ballot_sync(0xffffffffu, bad);
+                }
+                if (lane == 0) {
+                    mt.valid[w] = vword;
+                    mt.odd[w] = oword;
+                }
+            }
+            if constexpr (FP8) {                       // the unit of the output: largest exponent of the unit's values so far
+                top = __reduce_max_sync(0xffffffffu, top);
+                E = j == first ? top : max(E, top);
+                if (lane == 0) mt.E = (int)E;
+            }
+            __syncwarp();
+            if (lane == 0) {
+                tc::mbar_arrive(&f_ready[j % SLOTS]);
+                if (FP8) tc::mbar_arrive(&r_empty[rst]);
+            }
+        }
+        if (!ok && lane == 0) atomicMax(p.status, (int)KB_TIMEOUT_TMA);
     } else if (warp >= W_VAL) {
         // ------------------------------------------------------------ values: thread = token of the tile, and = query row
         const int t = threadIdx.x - W_VAL * 32;
-        const uint32_t lane_base = (uint32_t)((warp - W_VAL) * 32) << 16;
         auto load_queries = [&](const Segment& sg, int seg) {
             const int R = sg.rb * TT + t;
             const bool live = R < sg.n * p.G;
             const bf16* src = p.q + (long long)((p.cu ? p.cu[sg.b] : sg.b) + (live ? R / p.G : 0)) * p.q_stride + (long long)(sg.h * p.G + (live ? R % p.G : 0)) * HD;
-            const uint32_t dst = tmem_q + (seg & 1) * 64 + lane_base;
+            uint8_t* dst = sQ + (seg & 1) * L::QT + t * L::ROWB;
+            const int sw = L::ROWB == 128 ? t & 7 : (t >> 1) & 3;
+            uint4 v[HD / 8];
+#pragma unroll
+            for (int i = 0; i < HD / 8; ++i) v[i] = live ? *reinterpret_cast<const uint4*>(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
             if constexpr (FP8) {
                 uint32_t big = 0;
 #pragma unroll
-                for (int i = 0; i < HD / 8; ++i) {
-                    const uint4 v = live ? ld_row(src + i * 8) : make_uint4(0u, 0u, 0u, 0u);
-                    big = max(big, max(max(largest(v.x), largest(v.y)), max(largest(v.z), largest(v.w))));
-                }
+                for (int i = 0; i < HD / 8; ++i) big = max(big, max(max(largest(v[i].x), largest(v[i].y)), max(largest(v[i].z), largest(v[i].w))));
                 // the largest number comes to [2^7, 2^8); a row that is not finite becomes NaN
                 const float inv = big >= 0x7f80u ? __uint_as_float(0x7fc00000u) : pow2_biased(min(254 - (int)(big >> 7) + 7, 254));
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {    // 32 numbers: eight columns of hi, eight of lo
-                    uint32_t hi8[8], lo8[8];
+                for (int c = 0; c < HD / 16; ++c) {    // sixteen numbers: a chunk of hi, a chunk of lo
+                    uint32_t hi4[4], lo4[4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint4 v = live ? ld_row(src + c * 32 + i * 8) : make_uint4(0u, 0u, 0u, 0u);
-                        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t w[4] = {v[2 * c + i].x, v[2 * c + i].y, v[2 * c + i].z, v[2 * c + i].w};
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
                             uint32_t h2[2], l2[2];
@@ -283,35 +401,23 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                                 const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h2[z], __NV_E4M3)));
                                 l2[z] = e4m3x2(a - back.x, b - back.y);
                             }
-                            hi8[2 * i + e] = h2[0] | h2[1] << 16;
-                            lo8[2 * i + e] = l2[0] | l2[1] << 16;
+                            hi4[2 * i + e] = h2[0] | h2[1] << 16;
+                            lo4[2 * i + e] = l2[0] | l2[1] << 16;
                         }
                     }
-                    tc::tmem_st8(dst + 8 * c, hi8);
-                    tc::tmem_st8(dst + 32 + 8 * c, lo8);
+                    *reinterpret_cast<uint4*>(dst + ((c ^ sw) << 4)) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
+                    *reinterpret_cast<uint4*>(dst + L::KT + ((c ^ sw) << 4)) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
                 }
             } else {
 #pragma unroll
-                for (int c = 0; c < HD / 32; ++c) {
-                    uint32_t w[16];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint4 v = live ? ld_row(src + c * 32 + i * 8) : make_uint4(0u, 0u, 0u, 0u);
-                        w[4 * i] = v.x;
-                        w[4 * i + 1] = v.y;
-                        w[4 * i + 2] = v.z;
-                        w[4 * i + 3] = v.w;
-                    }
-                    tc::tmem_st16(dst + 16 * c, w);
-                }
+                for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * HALF + (((c & 7) ^ sw) << 4)) = v[c];
             }
-            tc::tmem_st_wait();
-            tc::tc_fence_before();
+            tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(&q_ready[seg & 1]);
         };
         Segment sg = segment(0);
-        int at = 0, seg = 0, loaded = 0, E = 0;        // tile within the segment, its number; segments whose queries are loaded
+        int at = 0, seg = 0, loaded = 0;               // tile within the segment, its number; segments whose queries are loaded
         for (int j = 0; j < n_tiles; ++j, ++at) {
             const int vs = j % L::VST, rst = j % L::RST;
             if (at == sg.t1 - sg.t0) {
@@ -319,86 +425,70 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 at = 0;
                 ++seg;
             }
-            // FP8: the operand stage is free when the product two tiles back has run
-            const bool ahead = at == 1 && loaded == seg + 1 && j - at + (sg.t1 - sg.t0) < n_tiles;
-            if (j >= 2 && (FP8 || loaded <= seg || ahead))
-                ok = tc::mbar_wait(&pv_done[(j - 2) % L::VST], (uint32_t)((j - 2) / L::VST) & 1u, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             // queries of this unit, or of the next one once the products of the unit before this one (the buffer's last reader) have run
-            if (loaded <= seg) {
-                load_queries(sg, seg);
-                loaded = seg + 1;
-            } else if (ahead) {
-                load_queries(segment(j - at + (sg.t1 - sg.t0)), seg + 1);
-                loaded = seg + 2;
-            }
-            ok = tc::mbar_wait(&r_full[rst], (uint32_t)(j / L::RST) & 1u, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            const int base = (sg.t0 + at) * TT, prefix = sg.ctx - sg.n, tok = base + t;
-            const uint32_t have = there[rst];
-            const bool valid = tok < sg.ctx && (have >> (t / PAGE) & 1u);
-            const bool edge = have != 0xffu || base + TT > prefix;
-            uint8_t* raw = sR + rst * L::KT;
-            uint8_t* op = sV + vs * L::VT;
-            uint32_t vword = 0xffffffffu, oword = 0u;
-            if (edge) {
-                vword = __ballot_sync(0xffffffffu, valid);
-                bool bad = false;
-                if (valid && tok >= prefix)
-                    for (int h = 0; h < L::HALVES; ++h)
-                        for (int c = 0; c < L::ROWB / 16; ++c) {
-                            const uint4 v = *reinterpret_cast<const uint4*>(raw + h * L::PIECE + t * L::ROWB + c * 16);
-                            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                            for (int q = 0; q < 4; ++q)
-                                bad |= FP8 ? __vcmpeq4(w[q] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u : __vcmpeq2(w[q] & 0x7f807f80u, 0x7f807f80u) != 0u;
-                        }
-                oword = __ballot_sync(0xffffffffu, bad);
-            }
-            if constexpr (FP8) {
-                // the unit of the output: largest exponent of the values so far (every warp finds it from all 128 tokens)
-                const uint8_t* e = exps + rst * 2 * TT;
-                uint32_t top = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int x = e[TT + i * 32 + lane], tk = base + i * 32 + lane;
-                    if (x != 255 && (!edge || (tk < sg.ctx && (have >> (2 * i + (lane >> 4)) & 1u)))) top = max(top, (uint32_t)x);
+            const bool ahead = at == 1 && loaded == seg + 1 && j - at + (sg.t1 - sg.t0) < n_tiles;
+            if (loaded <= seg || ahead) {
+                if (j >= 2) ok = tc::mbar_wait(&pv_done[(j - 2) % L::VST], (uint32_t)((j - 2) / L::VST) & 1u, abort_flag);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                if (loaded <= seg) {
+                    load_queries(sg, seg);
+                    loaded = seg + 1;
+                } else {
+                    load_queries(segment(j - at + (sg.t1 - sg.t0)), seg + 1);
+                    loaded = seg + 2;
                 }
-                top = __reduce_max_sync(0xffffffffu, top);
-                E = at == 0 ? (int)top : max(E, (int)top);
-                const int ek = e[t], ev = e[TT + t], w = min(ev - E, 0) + 6 + 127;
-                fact[vs * 2 * TT + t] = pow2_biased(ek);
-                fact[vs * 2 * TT + TT + t] = !valid || w <= 0 ? 0.f : ev == 255 ? 1.f : __uint_as_float((uint32_t)w << 23);
+            }
+            ok = tc::mbar_wait(&f_ready[j % SLOTS], (uint32_t)(j / SLOTS) & 1u, abort_flag);
+            // the operand stage is free when the product two tiles back has run
+            if (FP8 && ok && j >= 2) ok = tc::mbar_wait(&pv_done[vs], (uint32_t)((j - 2) / L::VST) & 1u, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            const TileMeta& mt = meta[j % SLOTS];
+            const uint32_t vword = mt.valid[warp - W_VAL];
+            uint8_t* op = sV + vs * L::VT;
+            if constexpr (FP8) {
+                // the token's factor, an f16 power of two of at most 2^6 (twice)
+                const uint8_t* raw = sR + rst * L::KT;
+                const int ev = exps[rst * 2 * TT + TT + t], w = ev == 255 ? 0 : min(ev - mt.E, 0) + 6;
+                const uint32_t one = !(vword >> lane & 1u) || w < -24 ? 0u : w >= -14 ? (uint32_t)(w + 15) << 10 : 1u << (w + 24);
+                const uint32_t mine = one | one << 16;
                 // codes -> f16: a warp takes whole rows, 16 codes per lane, so that loads and stores use all banks
                 constexpr int CH = HD / 16, RPW = 32 / CH;     // chunks per row, rows per warp step
                 const int c = lane % CH;
+                constexpr int U = 4;                           // rows in flight
+#pragma unroll 1
+                for (int i0 = 0; i0 < 32 / RPW; i0 += U) {
+                    uint4 v[U];
 #pragma unroll
-                for (int i = 0; i < 32 / RPW; ++i) {
-                    const int row = (warp - W_VAL) * 32 + i * RPW + lane / CH;
-                    const int sw = HD == 128 ? row & 7 : (row >> 1) & 3;
-                    uint4 v = *reinterpret_cast<const uint4*>(raw + row * L::ROWB + ((c ^ sw) << 4));
-                    if (edge && !(vword >> (row & 31) & 1u)) v = make_uint4(0u, 0u, 0u, 0u);
-                    uint4 a, b;
-                    codes_to_f16(v.x, a.x, a.y);
-                    codes_to_f16(v.y, a.z, a.w);
-                    codes_to_f16(v.z, b.x, b.y);
-                    codes_to_f16(v.w, b.z, b.w);
-                    uint8_t* dst = op + (c >> 2) * HALF + row * 128;
-                    const int c0 = (c & 3) * 2, flip = (c >> 2) & 1;       // the two halves of a row share banks: store them in opposite order
-                    *reinterpret_cast<uint4*>(dst + (((c0 + flip) ^ (row & 7)) << 4)) = flip ? b : a;
-                    *reinterpret_cast<uint4*>(dst + (((c0 + 1 - flip) ^ (row & 7)) << 4)) = flip ? a : b;
+                    for (int u = 0; u < U; ++u) {
+                        const int row = (warp - W_VAL) * 32 + (i0 + u) * RPW + lane / CH;
+                        v[u] = *reinterpret_cast<const uint4*>(raw + row * L::ROWB + ((c ^ (HD == 128 ? row & 7 : (row >> 1) & 3)) << 4));
+                    }
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int row = (warp - W_VAL) * 32 + (i0 + u) * RPW + lane / CH;
+                        const uint32_t f = __shfl_sync(0xffffffffu, mine, row & 31);
+                        if (!(vword >> (row & 31) & 1u)) v[u] = make_uint4(0u, 0u, 0u, 0u);
+                        uint4 a, b;
+                        codes_to_f16(v[u].x, a.x, a.y);
+                        codes_to_f16(v[u].y, a.z, a.w);
+                        codes_to_f16(v[u].z, b.x, b.y);
+                        codes_to_f16(v[u].w, b.z, b.w);
+                        a = make_uint4(mul_f16x2(a.x, f), mul_f16x2(a.y, f), mul_f16x2(a.z, f), mul_f16x2(a.w, f));
+                        b = make_uint4(mul_f16x2(b.x, f), mul_f16x2(b.y, f), mul_f16x2(b.z, f), mul_f16x2(b.w, f));
+                        uint8_t* dst = op + (c >> 2) * HALF + row * 128;
+                        const int c0 = (c & 3) * 2, flip = (c >> 2) & 1;   // the two halves of a row share banks: store them in opposite order
+                        *reinterpret_cast<uint4*>(dst + (((c0 + flip) ^ (row & 7)) << 4)) = flip ? b : a;
+                        *reinterpret_cast<uint4*>(dst + (((c0 + 1 - flip) ^ (row & 7)) << 4)) = flip ? a : b;
+                    }
                 }
-            } else if (edge && !valid) {
+                tc::fence_proxy_async();
+            } else if (vword != 0xffffffffu) {
+                if (!(vword >> lane & 1u))
 #pragma unroll
-                for (int h = 0; h < L::HALVES; ++h)
-                    for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(op + h * HALF + t * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    for (int h = 0; h < L::HALVES; ++h)
+                        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(op + h * HALF + t * 128 + c * 16) = make_uint4(0u, 0u, 0u, 0u);
+                tc::fence_proxy_async();
             }
-            if (lane == 0) {
-                meta[vs].valid[warp - W_VAL] = vword;
-                meta[vs].odd[warp - W_VAL] = oword;
-                meta[vs].E = E;
-            }
-            tc::fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
                 tc::mbar_arrive(&v_ready[vs]);
@@ -407,9 +497,10 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         }
         if (!ok && lane == 0) atomicMax(p.status, (int)KB_TIMEOUT_TMA);
     } else {
-        // ------------------------------------------------------------ softmax: two threads per row
-        const int hf = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16, tmem_o = tmem_oacc + lane_base;
+        // ------------------------------------------------------------ softmax: a thread per row, tiles of parity g
+        const int g = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tmem_s = tmem0 + g * 128 + lane_base, tmem_o = tmem_oacc + g * HD + lane_base;
         uint32_t n_slow = 0, n_x = 0;
         auto exchange = [&](uint64_t* bar, uint32_t& count) {
             __syncwarp();
@@ -418,149 +509,114 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             ++count;
             return good;
         };
-        int j = 0;
-        while (j < n_tiles && ok) {
-            const Segment sg = segment(j);
-            const int M = sg.n * p.G, R = sg.rb * TT + r, c0 = p.cu ? p.cu[sg.b] : sg.b, prefix = sg.ctx - sg.n;
+        // log2 units: the maximum is renewed when a score exceeds it by more than GROW; P is in units of 2^-SHIFT.  f16 holds 2^(GROW + SHIFT)
+        constexpr float GROW = FP8 ? 11.f : 40.f, SHIFT = FP8 ? 4.f : 0.f;
+        int j0 = 0;
+        while (j0 < n_tiles && ok) {
+            const Segment sg = segment(j0);
+            const int len = sg.t1 - sg.t0, M = sg.n * p.G, R = sg.rb * TT + r, c0 = p.cu ? p.cu[sg.b] : sg.b, prefix = sg.ctx - sg.n;
             const bool live = sg.rb * TT + (warp & 3) * 32 < M;            // the warp has rows
-            const int row_i = min(R, M - 1) / p.G;
+            const int row_i = min(R, M - 1) / p.G, row_g = min(R, M - 1) % p.G;
             float scale = p.scale_log2;
             if constexpr (FP8) {                       // the power of two that load_queries took out of this row
                 if (live) {
-                    const bf16* src = p.q + (long long)(c0 + row_i) * p.q_stride + (long long)(sg.h * p.G + min(R, M - 1) % p.G) * HD + hf * (HD / 2);
+                    const bf16* src = p.q + (long long)(c0 + row_i) * p.q_stride + (long long)(sg.h * p.G + row_g) * HD;
                     uint32_t big = 0;
 #pragma unroll
                     for (int i = 0; i < HD / 8; ++i) {
-                        const uint2 v = *reinterpret_cast<const uint2*>(src + i * 4);
-                        big = max(big, max(max(v.x & 0x7fffu, (v.x >> 16) & 0x7fffu), max(v.y & 0x7fffu, (v.y >> 16) & 0x7fffu)));
+                        const uint4 v = *reinterpret_cast<const uint4*>(src + i * 8);
+                        big = max(big, max(max(largest(v.x), largest(v.y)), max(largest(v.z), largest(v.w))));
                     }
-                    row_buf[(4 + hf) * TT + r] = __uint_as_float(big);
+                    scale *= pow2_biased(254 - min(254 - (int)(big >> 7) + 7, 254));       // 1 / inv of load_queries
                 }
-                if (!exchange(&xch, n_x)) { ok = false; break; }
-                const uint32_t big = max(__float_as_uint(row_buf[4 * TT + r]), __float_as_uint(row_buf[5 * TT + r]));
-                // 1 / inv of load_queries; exact, both are powers of two
-                scale *= pow2_biased(254 - min(254 - (int)(big >> 7) + 7, 254));
-                if (!exchange(&xch, n_x)) { ok = false; break; }           // both have read before the sums are written there
             }
             float m_used = -INFINITY, l = 0.f;
             int E = 0;
-            for (int at = 0; at < sg.t1 - sg.t0; ++at, ++j) {
-                const int vs = j % L::VST, base = (sg.t0 + at) * TT;
-                const uint32_t tmem_s = tmem0 + (j & 1) * 128 + lane_base;
-                if (!tc::mbar_wait(&s_full[j & 1], (uint32_t)(j >> 1) & 1u, abort_flag)) { ok = false; break; }
+            bool begun = false;                        // the group has had a tile of this segment
+            for (int at = (g ^ j0) & 1; at < len; at += 2) {
+                const int j = j0 + at, vs = j % L::VST, base = (sg.t0 + at) * TT;
+                if (!tc::mbar_wait(&s_full[g], (uint32_t)(j >> 1) & 1u, abort_flag)) { ok = false; break; }
                 tc::tc_fence_after();
                 // tiles with drafted tokens, with the end of the context, or with pages that are not there
-                const bool edge = base + TT > prefix || there_k[j % 8] != 0xffu;
-                if ((FP8 || edge) && !tc::mbar_wait(&v_ready[vs], (uint32_t)(j / L::VST) & 1u, abort_flag)) { ok = false; break; }
-                const TileMeta& mt = meta[vs];
+                const bool edge = base + TT > prefix || there_k[j % SLOTS] != 0xffu;
+                if ((FP8 || edge) && !tc::mbar_wait(&f_ready[j % SLOTS], (uint32_t)(j / SLOTS) & 1u, abort_flag)) { ok = false; break; }
+                const TileMeta& mt = meta[j % SLOTS];
                 uint32_t odd_any = 0;
-                unsigned long long seen = ~0ull;
-                float s[64];
-                float mx = -INFINITY;
-                if (edge) odd_any = mt.odd[0] | mt.odd[1] | mt.odd[2] | mt.odd[3];
-                if (live) {
-                    tc::tmem_ld32(tmem_s + hf * 64, reinterpret_cast<uint32_t*>(s));
-                    tc::tmem_ld32(tmem_s + hf * 64 + 32, reinterpret_cast<uint32_t*>(s + 32));
-                    tc::tmem_ld_wait();
-                    if constexpr (FP8) {
-                        const float* kf = fact + vs * 2 * TT + hf * 64;
+                unsigned long long seen[2] = {~0ull, ~0ull};
+                if (edge) {
+                    odd_any = mt.odd[0] | mt.odd[1] | mt.odd[2] | mt.odd[3];
 #pragma unroll
-                        for (int c = 0; c < 64; c += 4) {
-                            const float4 f = *reinterpret_cast<const float4*>(kf + c);
-                            const float2 a = __fmul2_rn(make_float2(s[c], s[c + 1]), make_float2(f.x, f.y));
-                            const float2 b = __fmul2_rn(make_float2(s[c + 2], s[c + 3]), make_float2(f.z, f.w));
-                            s[c] = a.x;
-                            s[c + 1] = a.y;
-                            s[c + 2] = b.x;
-                            s[c + 3] = b.y;
-                        }
-                    }
-                    if (edge) {
-                        seen = sees(p, c0, row_i, base + hf * 64 - prefix) &
-                               ((unsigned long long)mt.valid[2 * hf] | (unsigned long long)mt.valid[2 * hf + 1] << 32);
-#pragma unroll
-                        for (int c = 0; c < 64; ++c) s[c] = (uint32_t)(seen >> c) & 1u ? s[c] : -INFINITY;
-                    }
-                    float mx8[8];
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) mx8[i] = fmaxf(s[2 * i], s[2 * i + 1]);
-#pragma unroll
-                    for (int c = 16; c < 64; c += 16) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) mx8[i] = attn::fmax3(mx8[i], s[c + 2 * i], s[c + 2 * i + 1]);
-                    }
-                    mx = attn::fmax3(attn::fmax3(mx8[0], mx8[1], mx8[2]), attn::fmax3(mx8[3], mx8[4], mx8[5]), fmaxf(mx8[6], mx8[7]));
-                    row_buf[((j & 1) * 2 + hf) * TT + r] = mx;
+                    for (int hf = 0; hf < 2; ++hf)
+                        seen[hf] = sees(p, c0, row_i, base + hf * 64 - prefix) &
+                                   ((unsigned long long)mt.valid[2 * hf] | (unsigned long long)mt.valid[2 * hf + 1] << 32);
                 }
-                // (also orders "both halves have read their scores" before either writes P over them)
-                if (!exchange(&xch, n_x)) { ok = false; break; }
                 if (live) {
+                    const float* kf = fact + (j % SLOTS) * TT;
                     const int E_new = FP8 ? mt.E : 0;
-                    mx = fmaxf(mx, row_buf[((j & 1) * 2 + (hf ^ 1)) * TT + r]) * scale;
-                    const bool grow = mx > m_used + GROW;
-                    if (at == 0) {
-                        m_used = mx;
-                        E = E_new;
-                    } else if (__any_sync(0xffffffffu, grow) || (FP8 && E_new != E)) {
-                        if (!tc::mbar_wait(&pv_done[(j - 1) % L::VST], (uint32_t)((j - 1) / L::VST) & 1u, abort_flag)) { ok = false; break; }
-                        tc::tc_fence_after();
-                        const float m_new = fmaxf(m_used, mx);
-                        const float f = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
-                        const float fo = FP8 ? f * exp2f((float)(E - E_new)) : f;
-#pragma unroll 1
-                        for (int c = 0; c < HD / 2; c += 16) {
-                            uint32_t o[16];
-                            tc::tmem_ld16(tmem_o + hf * (HD / 2) + c, o);
-                            tc::tmem_ld_wait();
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * fo);
-                            tc::tmem_st16(tmem_o + hf * (HD / 2) + c, o);
-                        }
-                        tc::tmem_st_wait();
-                        l *= f;
-                        m_used = m_new;
-                        E = E_new;
-                    }
-                    const float mb = m_used == -INFINITY ? 0.f : m_used;
-                    const float2 sc2 = make_float2(scale, scale), nm2 = make_float2(-mb, -mb);
-                    if (edge) {                                // exponentials of -infinity have to be zero
-#pragma unroll
-                        for (int c = 0; c < 64; c += 2) {
-                            const float2 x = __ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2);
-                            s[c] = exp2f(x.x);
-                            s[c + 1] = exp2f(x.y);
-                        }
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < 64; c += 2) {
-                            const float2 e = attn::exp2_pair<EMU>(__ffma2_rn(make_float2(s[c], s[c + 1]), sc2, nm2), c >> 1);
-                            s[c] = e.x;
-                            s[c + 1] = e.y;
-                        }
-                    }
+                    if (FP8 && begun && E_new != E) scale_columns(tmem_o, HD, exp2f((float)(E - E_new)));
+                    E = E_new;
+                    const float2 sc2 = make_float2(scale, scale);
                     float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-                    const float* wf = fact + vs * 2 * TT + TT + hf * 64;
+                    // 32 columns at a time.  The loop stays rolled: unrolled, the instruction cache is what bounds this kernel
+#pragma unroll 1
+                    for (int q = 0; q < 4; ++q) {
+                        float x[32];
+                        tc::tmem_ld32(tmem_s + 32 * q, reinterpret_cast<uint32_t*>(x));
+                        tc::tmem_ld_wait();
+                        if constexpr (FP8) {
 #pragma unroll
-                    for (int q4 = 0; q4 < 4; ++q4) {
-                        uint32_t pk[8];
-#pragma unroll
-                        for (int c = q4 * 16; c < q4 * 16 + 16; c += 4) {
-                            float2 a = make_float2(s[c], s[c + 1]), b = make_float2(s[c + 2], s[c + 3]);
-                            sum2[0] = __fadd2_rn(sum2[0], a);
-                            sum2[1] = __fadd2_rn(sum2[1], b);
-                            if constexpr (FP8) {
-                                const float4 w = *reinterpret_cast<const float4*>(wf + c);
-                                a = __fmul2_rn(a, make_float2(w.x, w.y));
-                                b = __fmul2_rn(b, make_float2(w.z, w.w));
-                                s[c] = a.x;                    // (kept for the pass below)
-                                s[c + 1] = a.y;
-                                s[c + 2] = b.x;
-                                s[c + 3] = b.y;
+                            for (int i = 0; i < 32; i += 4) {
+                                const float4 f = *reinterpret_cast<const float4*>(kf + 32 * q + i);
+                                const float2 u = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(f.x, f.y));
+                                const float2 v = __fmul2_rn(make_float2(x[i + 2], x[i + 3]), make_float2(f.z, f.w));
+                                x[i] = u.x;
+                                x[i + 1] = u.y;
+                                x[i + 2] = v.x;
+                                x[i + 3] = v.y;
                             }
-                            pk[(c >> 1) & 7] = FP8 ? pack_f16(a.x, a.y) : pack_bf16(a.x, a.y);
-                            pk[((c >> 1) & 7) + 1] = FP8 ? pack_f16(b.x, b.y) : pack_bf16(b.x, b.y);
                         }
-                        tc::tmem_st8(tmem_s + hf * 32 + q4 * 8, pk);
+                        const uint32_t sees32 = (uint32_t)(seen[q >> 1] >> (32 * (q & 1)));
+                        if (edge) {                    // what is not seen
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) x[i] = sees32 >> i & 1u ? x[i] : -INFINITY;
+                        }
+                        float m4[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) m4[i] = attn::fmax3(x[3 * i], x[3 * i + 1], x[3 * i + 2]);
+#pragma unroll
+                        for (int i = 12; i < 28; i += 8) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) m4[e] = attn::fmax3(m4[e], x[i + 2 * e], x[i + 2 * e + 1]);
+                        }
+                        m4[0] = attn::fmax3(m4[0], x[28], x[29]);
+                        m4[1] = attn::fmax3(m4[1], x[30], x[31]);
+                        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
+                        if (__any_sync(0xffffffffu, mx > m_used + GROW)) {
+                            // move to the new maximum what has been summed against the old one: O (S(j) follows the product of the
+                            // group's last tile, so O is complete), the sum, and this tile's probabilities so far
+                            const float m_new = fmaxf(m_used, mx), f = m_new == -INFINITY ? 1.f : exp2f(m_used - m_new);
+                            if (begun) scale_columns(tmem_o, HD, f);
+                            if (q > 0) scale_packed<FP8>(tmem_s, 16 * q, f);
+                            l *= f;
+                            sum2[0] = __fmul2_rn(sum2[0], make_float2(f, f));
+                            sum2[1] = __fmul2_rn(sum2[1], make_float2(f, f));
+                            m_used = m_new;
+                        }
+                        const float mb = m_used == -INFINITY ? -SHIFT : m_used - SHIFT;
+                        const float2 nm2 = make_float2(-mb, -mb);
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            const float2 y = __ffma2_rn(make_float2(x[i], x[i + 1]), sc2, nm2);
+                            x[i] = exp2f(y.x);
+                            x[i + 1] = exp2f(y.y);
+                        }
+                        uint32_t pk[16];
+#pragma unroll
+                        for (int i = 0; i < 32; i += 2) {
+                            sum2[(i >> 1) & 1] = __fadd2_rn(sum2[(i >> 1) & 1], make_float2(x[i], x[i + 1]));
+                            pk[i >> 1] = FP8 ? pack_f16(x[i], x[i + 1]) : pack_bf16(x[i], x[i + 1]);
+                        }
+                        tc::tmem_st16(tmem_s + 16 * q, pk);        // over the scores of columns that this thread has read
                     }
                     l += (sum2[0].x + sum2[0].y) + (sum2[1].x + sum2[1].y);
                     tc::tmem_st_wait();
@@ -568,84 +624,100 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 if (odd_any) {
                     // ---- values that are not finite: rows that see the token get its products here, the others never meet it
                     uint8_t* op = sV + vs * L::VT;
-                    if (live && at > 0 && !tc::mbar_wait(&pv_done[(j - 1) % L::VST], (uint32_t)((j - 1) / L::VST) & 1u, abort_flag)) { ok = false; break; }
-                    tc::tc_fence_after();
-                    bool begun = at > 0;
-                    for (int tk = 0; tk < TT; ++tk) {
+                    if (!tc::mbar_wait(&v_ready[vs], (uint32_t)(j / L::VST) & 1u, abort_flag)) { ok = false; break; }
+                    bool have_o = begun;
+                    for (int tk = 0; tk < TT && live; ++tk) {
                         if (!(mt.odd[tk >> 5] >> (tk & 31) & 1u)) continue;
-                        if (live && hf == tk >> 6) {
-                            float mine = 0.f;
+                        uint32_t two = 0, pk[16];
+                        tc::tmem_ld16(tmem_s + (tk >> 5) * 16, pk);
+                        tc::tmem_ld_wait();
 #pragma unroll
-                            for (int c = 0; c < 64; ++c)
-                                if (c == (tk & 63)) mine = s[c];
-                            row_buf[4 * TT + r] = seen >> (tk & 63) & 1ull ? mine : -1.f;
-                        }
-                        if (!exchange(&slow, n_slow)) { ok = false; break; }
-                        if (live) {
-                            const float pv = row_buf[4 * TT + r];
+                        for (int c = 0; c < 16; ++c)
+                            if (c == ((tk >> 1) & 15)) two = pk[c];
+                        two = tk & 1 ? two >> 16 : two & 0xffffu;
+                        const float pv = FP8 ? f16x2_to_float(two).x : __uint_as_float(two << 16);
+                        const bool sees_it = seen[tk >> 6] >> (tk & 63) & 1ull;
 #pragma unroll 1
-                            for (int c = 0; c < HD / 2; c += 16) {
-                                uint32_t o[16];
-                                tc::tmem_ld16(tmem_o + hf * (HD / 2) + c, o);
-                                tc::tmem_ld_wait();
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t o[16];
+                            tc::tmem_ld16(tmem_o + c, o);
+                            tc::tmem_ld_wait();
 #pragma unroll
-                                for (int i = 0; i < 16; ++i) {
-                                    const int d = hf * (HD / 2) + c + i;
-                                    const uint16_t bits = *reinterpret_cast<const uint16_t*>(op + (d >> 6) * HALF + tk * 128 + ((((d & 63) >> 3) ^ (tk & 7)) << 4) + (d & 7) * 2);
-                                    const float v = FP8 ? f16x2_to_float(bits).x : __uint_as_float((uint32_t)bits << 16);
-                                    const float was = begun ? __uint_as_float(o[i]) : 0.f;
-                                    o[i] = __float_as_uint(pv < 0.f ? was : was + pv * v);
-                                }
-                                tc::tmem_st16(tmem_o + hf * (HD / 2) + c, o);
+                            for (int i = 0; i < 16; ++i) {
+                                const int d = c + i;
+                                const uint16_t bits = *reinterpret_cast<const uint16_t*>(op + (d >> 6) * HALF + tk * 128 + ((((d & 63) >> 3) ^ (tk & 7)) << 4) + (d & 7) * 2);
+                                const float v = FP8 ? f16x2_to_float(bits).x : __uint_as_float((uint32_t)bits << 16);
+                                const float was = have_o ? __uint_as_float(o[i]) : 0.f;
+                                o[i] = __float_as_uint(sees_it ? was + pv * v : was);
                             }
-                            tc::tmem_st_wait();
+                            tc::tmem_st16(tmem_o + c, o);
                         }
-                        begun = true;
-                        if (!exchange(&slow, n_slow)) { ok = false; break; }
-                        if (warp == 0 && lane < HD / 8) *reinterpret_cast<uint4*>(op + (lane >> 3) * HALF + tk * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+                        tc::tmem_st_wait();
+                        have_o = true;
                     }
-                    if (!ok) break;
+                    if (!exchange(&slow[g], n_slow)) { ok = false; break; }        // the group's rows have read the tokens
+                    for (int tk = warp & 3; tk < TT; tk += 4)
+                        if ((mt.odd[tk >> 5] >> (tk & 31) & 1u) && lane < HD / 8)
+                            *reinterpret_cast<uint4*>(op + (lane >> 3) * HALF + tk * 128 + (lane & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
                     tc::fence_proxy_async();
                 }
+                begun = true;
                 tc::tc_fence_before();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive(&p_ready[j & 1]);
+                if (lane == 0) tc::mbar_arrive(&p_ready[g]);
             }
             if (!ok) break;
-            // ---- the unit's rows, as far as this part has them
-            row_buf[(4 + hf) * TT + r] = l;
+            // ---- the unit's rows, as far as this part has them: the groups' results together
+            row_buf[g * TT + r] = m_used;
+            row_buf[(2 + g) * TT + r] = FP8 ? l * 0.0625f : l;
+            if (lane == 0 && (warp & 3) == 0) unit_E[g] = E;
             if (!exchange(&xch, n_x)) { ok = false; break; }
-            l += row_buf[(4 + (hf ^ 1)) * TT + r];
-            if (!tc::mbar_wait(&pv_done[(j - 1) % L::VST], (uint32_t)((j - 1) / L::VST) & 1u, abort_flag)) { ok = false; break; }
+            const int j_last = j0 + len - 1;
+            if (!tc::mbar_wait(&pv_done[j_last % L::VST], (uint32_t)(j_last / L::VST) & 1u, abort_flag)) { ok = false; break; }
             tc::tc_fence_after();
             if (live) {
                 const bool done = sg.t0 == 0 && sg.t1 == sg.T, mine = R < M;
                 const long long slot = 2ll * blockIdx.x + (sg.t0 == 0);
-                float unit = 1.f;
-                if constexpr (FP8) unit = pow2_biased(E) * 0.015625f;      // 2^(E - 127 - 6)
-                if (done) unit *= l == 0.f ? 0.f : 1.f / l;
-                bf16* dst = p.out + (long long)(c0 + row_i) * p.out_stride + (long long)(sg.h * p.G + min(R, M - 1) % p.G) * HD + hf * (HD / 2);
-                float* part_o = p.part_o + (slot * TT + r) * HD + hf * (HD / 2);
+                const float m0 = row_buf[r], m1 = row_buf[TT + r], m = fmaxf(m0, m1), mb = m == -INFINITY ? 0.f : m;
+                float f0 = exp2f(m0 - mb), f1 = exp2f(m1 - mb);
+                // (a sum without a maximum is zero, or NaN and has to get through)
+                const float sum = (m0 == -INFINITY ? row_buf[2 * TT + r] : row_buf[2 * TT + r] * f0) +
+                                  (m1 == -INFINITY ? row_buf[3 * TT + r] : row_buf[3 * TT + r] * f1);
+                if constexpr (FP8) {                   // 2^(E - 127 - 6) and the 2^4 of P
+                    f0 *= pow2_biased(unit_E[0]) * 9.765625e-4f;
+                    f1 *= pow2_biased(unit_E[1]) * 9.765625e-4f;
+                }
+                if (done) {
+                    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                    f0 *= inv;
+                    f1 *= inv;
+                }
+                const bool has0 = len > 1 || (j0 & 1) == 0, has1 = len > 1 || (j0 & 1) == 1;       // what a group without a tile left in O is not its
+                bf16* dst = p.out + (long long)(c0 + row_i) * p.out_stride + (long long)(sg.h * p.G + row_g) * HD + g * (HD / 2);
+                float* part_o = p.part_o + (slot * (HD / 4) + g * (HD / 8)) * TT * 4 + r * 4;      // [HD / 4][rows][4]: a warp's stores are whole lines
 #pragma unroll 1
-                for (int c = 0; c < HD / 2; c += 32) {
-                    uint32_t o[32];
-                    tc::tmem_ld32(tmem_o + hf * (HD / 2) + c, o);
+                for (int c = 0; c < HD / 2; c += 16) {
+                    uint32_t a[16], b[16];
+                    tc::tmem_ld16(tmem_oacc + lane_base + g * (HD / 2) + c, a);
+                    tc::tmem_ld16(tmem_oacc + HD + lane_base + g * (HD / 2) + c, b);
                     tc::tmem_ld_wait();
                     if (mine) {
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4) {
+                        for (int i = 0; i < 16; i += 4) {
                             float v[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(o[i + e]) * unit;
+                            for (int e = 0; e < 4; ++e)
+                                v[e] = (has0 ? __uint_as_float(a[i + e]) * f0 : 0.f) + (has1 ? __uint_as_float(b[i + e]) * f1 : 0.f);
                             if (done) *reinterpret_cast<uint2*>(dst + c + i) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
-                            else *reinterpret_cast<float4*>(part_o + c + i) = make_float4(v[0], v[1], v[2], v[3]);
+                            else *reinterpret_cast<float4*>(part_o + (long long)((c + i) >> 2) * TT * 4) = make_float4(v[0], v[1], v[2], v[3]);
                         }
                     }
                 }
-                if (mine && !done && hf == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * TT + r) * 2) = make_float2(m_used, l);
+                if (mine && !done && g == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * TT + r) * 2) = make_float2(m, sum);
             }
-            tc::tc_fence_before();                     // O is read before the next unit's first product (ordered by its p_ready)
-            if (!exchange(&xch, n_x)) { ok = false; break; }               // and the sums before the next unit writes there
+            tc::tc_fence_before();                     // O is read before the next unit's first products (ordered by their p_ready)
+            if (!exchange(&xch, n_x)) { ok = false; break; }
+            j0 += len;
         }
         if (!ok && lane == 0) atomicMax(p.status, (int)KB_TIMEOUT_EPI);
     }

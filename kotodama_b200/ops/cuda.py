@@ -1024,7 +1024,7 @@ class CudaOps(TorchOps):
 
     def paged_tree_attention(self, q, k_pages, v_pages, page_table, ctx_lens, cu_seqlens, max_q, max_ctx, scale, masks=None, out=None):
         """bf16 queries with heads of 64 or 128 take the tensor-core kernel (``csrc/tree_attn_sm100.cu``); the 32-bit mode, other head
-        sizes and rows that are not 8-byte aligned the plain one (``csrc/tree_attn.cu``)."""
+        sizes and query rows that are not 16-byte aligned the plain one (``csrc/tree_attn.cu``)."""
         N, H, hd = q.shape
         dev = q.device
         fp8 = isinstance(k_pages, Fp8Pages)
@@ -1052,7 +1052,7 @@ class CudaOps(TorchOps):
         if N == 0 or B == 0 or page_table.shape[1] == 0:
             return res if given else res.zero_()
         floats = 0
-        if q.dtype == torch.bfloat16 and q.stride(0) % 4 == 0 and res.stride(0) % 4 == 0 and (q.data_ptr() | res.data_ptr()) % 8 == 0:
+        if q.dtype == torch.bfloat16 and q.stride(0) % 8 == 0 and res.stride(0) % 4 == 0 and q.data_ptr() % 16 == 0 and res.data_ptr() % 8 == 0:
             floats = self._tree_floats(N, B, H, kt.shape[1], hd, max_q, max_ctx, kt.shape[0], int(fp8))
         if floats:
             work = torch.empty(floats, device=dev, dtype=torch.float32)
