@@ -1,4 +1,4 @@
-// Shared pieces of the tensor-core tree attention kernels (tree_attn_sm100.cu: tiles of 16 and 32 query rows on mma.sync,
+// Shared pieces of the tensor-core tree attention kernels (tree_attn_sm100.cu: tiles of 16 query rows on mma.sync,
 // tree_attn_tile_sm100.cu: tiles of 128 rows on tcgen05): parameters, the cut of the work, the merge of partial results.
 #pragma once
 #include <cuda_fp8.h>
@@ -9,18 +9,18 @@ typedef __nv_bfloat16 bf16;
 
 namespace tree {
 
-constexpr int PAGE = 16, MAX_B = 2048;
+constexpr int PAGE = 16, MAX_B = 1024;
 
 struct TreeParams {
     const bf16* q;
     long long q_stride;
-    const uint8_t *ke, *ve;                            // exponents of 8-bit pages
+    const uint8_t *k, *v, *ke, *ve;                    // pages, and exponents of 8-bit pages
     const int *table, *ctx_lens, *cu;
     const long long* masks;
     bf16* out;
     long long out_stride;
-    float* part_o;                                     // [2 * grid][HD / 4][ROWS][4]
-    float* part_ml;                                    // [2 * grid][ROWS][2]
+    float* part_o;                                     // [2 * workers][ROWS][HD], or [2 * workers][HD / 4][ROWS][4] (128 rows)
+    float* part_ml;                                    // [2 * workers][ROWS][2]
     int* uoff;                                         // [B + 1] tiles before each sequence, for the merge kernel
     int max_pages, num_pages, B, N, H, G, n_kv, max_q, max_ctx;
     float scale_log2;
@@ -40,9 +40,17 @@ __device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t&
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(c));
 }
 __device__ __forceinline__ float pow2_biased(int b) { return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 0x00400000u); }
-__device__ __forceinline__ void bulk_16(void* dst, const void* src, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(smem_u32(dst)), "l"(src), "r"(16), "r"(smem_u32(bar)) : "memory");
+// Pages are fetched 16 bytes per thread.  (A TMA copy costs ~150 cycles of its engine whatever its size: blocks of 2 KB, a page of one
+// head, reached 3.4 TB/s over the GPU, 16-byte copies by the threads 6.8.)
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// Arrives on `bar` when this thread's copies so far have landed (counted among the barrier's arrivals).
+__device__ __forceinline__ void copy_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // rows of a sequence and its tokens; 0 rows where it has none or breaks the rules
@@ -56,7 +64,7 @@ __device__ __forceinline__ int2 span_of(const TreeParams& p, int b, bool report)
     return make_int2(n, ctx);
 }
 
-struct Segment {                                       // a CTA's part of one unit
+struct Segment {                                       // a worker's part of one unit
     int b, h, rb, n, ctx, T, t0, t1;
 };
 // The unit of tile x, as far as a part that ends at `hi` has it from x on.
@@ -114,12 +122,12 @@ __device__ __forceinline__ void count_tiles(const TreeParams& p, int* uoff, int*
     if (blockIdx.x == 0)
         for (int i = threadIdx.x; i <= p.B; i += THREADS) p.uoff[i] = uoff[i];
 }
-// This block's part [lo, hi) of the line of tiles (empty where there are more blocks than tiles: every part that exists has a tile, since
-// the merge reads all parts between a unit's first and last).
-__device__ __forceinline__ int2 part_of_line(long long total) {
-    const long long parts = min((long long)gridDim.x, total);
-    if ((long long)blockIdx.x >= parts) return make_int2(0, 0);
-    return make_int2((int)(total * blockIdx.x / parts), (int)(total * (blockIdx.x + 1) / parts));
+// The part [lo, hi) of the line of tiles that worker `w` of `workers` has (empty where there are more workers than tiles: every part that
+// exists has a tile, since the merge reads all parts between a unit's first and last).
+__device__ __forceinline__ int2 part_of_line(long long total, int w, int workers) {
+    const long long parts = min((long long)workers, total);
+    if (w >= parts) return make_int2(0, 0);
+    return make_int2((int)(total * w / parts), (int)(total * (w + 1) / parts));
 }
 // Bits of `width` <= 64 tokens from position `base` on that drafted row i sees (bit t: token base + t), existing or not.
 __device__ __forceinline__ unsigned long long sees(const TreeParams& p, int c0, int i, int d) {      // d = base - prefix
@@ -131,10 +139,7 @@ __device__ __forceinline__ unsigned long long sees(const TreeParams& p, int c0, 
 
 // Host side, in tree_attn_sm100.cu.
 int sm_count();
-int page_map(CUtensorMap* m, const void* base, long long rows, int hd, bool fp8, bool halves_apart);
-// Puts the parts of the units together; `wide`: eight warps per row instead of one.
-int merge(const TreeParams& p, int hd, int rows, int tile, int grid, bool wide, int zero_tail, cudaStream_t st);
 // The 128-row kernel (tree_attn_tile_sm100.cu).
-int launch_tile(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams& p, int hd, bool fp8, int grid, cudaStream_t st);
+int launch_tile(const TreeParams& p, int hd, bool fp8, int grid, cudaStream_t st);
 
 }  // namespace tree

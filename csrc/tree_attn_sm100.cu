@@ -3,31 +3,30 @@
 //
 // What bounds it.  A cached row is used by the (drafted token, query head) rows of its KV head only - 1 to a few hundred - so the
 // cache's bytes bound the call, and above ~100 rows the tensor cores do.  Each (sequence, KV head) has its n * G query rows as the
-// M side of `mma.sync.m16n8k16` tiles (ROWS = 16 or 32 of them per unit of work), cached tokens are the N side of the score product and
-// the K side of the output product; probabilities go from accumulators to operands in registers.
+// M side of `mma.sync.m16n8k16` tiles (16 of them per unit of work), cached tokens are the N side of the score product and the K side of
+// the output product; probabilities go from accumulators to operands in registers.  Calls with more than 16 rows per KV head take
+// tree_attn_tile_sm100.cu.
 //
-// Work.  A unit is (sequence, KV head, block of ROWS rows); its tiles are TILE tokens of the context.  All units' tiles form one line
-// that is cut into equal parts, one per CTA, so that ragged contexts and one long context load the GPU alike.  A CTA walks its part:
-// a unit that lies inside it is finished there, the others leave partial results (unnormalised output, maximum, sum per row)
-// that the merge kernel puts together.  A CTA has at most two such partial units: the one it enters with (slot 0) and the one it leaves with (slot 1).
-//
-// Inside a CTA the four warps share the rows and split the tokens: warp w has tokens w * IT .. of every tile, in a ring of its own that
-// TMA fills page by page (128- or 64-byte swizzle), so nothing in the loop waits for another warp; every cached number is
-// converted once per CTA.  The warps' results meet in shared memory at the end of a unit.
+// Work.  A unit is (sequence, KV head, block of rows); its tiles are TILE tokens of the context.  All units' tiles form one line
+// that is cut into equal parts, one per worker, so that ragged contexts and one long context load the GPU alike.  Here a worker is a
+// warp (in tree_attn_tile_sm100.cu a CTA): it copies its tiles into a ring of its own, 16 bytes per lane, and waits for no other warp.
+// A unit that lies inside a part is finished there, the others leave partial results (unnormalised output, maximum, sum per row)
+// that the merge kernel puts together.  A worker has at most two such partial units: the one it enters with (slot 0) and the one it
+// leaves with (slot 1).
 //
 // 8-bit pages.  Codes become f16 (exact) on the way to the tensor cores.  Keys: the score's accumulator is scaled by the token's power of two.
-// Values: the probability is scaled by the token's power of two relative to E, the largest seen so far by the warp, times 2^14, and
-// rounded to f16; the output is kept in units of 2^(E - 14).  So a probability keeps f16's eleven bits down to 2^-28 of the largest.
+// Values: the probability is scaled by the token's power of two relative to E, the largest seen so far by the warp, times 2^4, and
+// rounded to f16; the output is kept in units of 2^(E - 4).  Maxima are renewed when a score exceeds them by 2^11, so f16's largest is
+// 2^15, and a probability keeps eleven bits down to 2^-18 of the maximum and is off by at most 2^-29 below.
 // Queries become f16 with a power of two per row taken out (exact down to 2^-24 of the row's largest).
-// bf16 pages: queries as they are, probabilities rounded to bf16 (2^-9 relative, like the other decode kernels).
-// Scores, maxima, sums and outputs are fp32.
+// bf16 pages: queries as they are, probabilities rounded to bf16.  Scores, maxima, sums and outputs are fp32.
 #include "tree_attn.cuh"
 
 namespace {
 
 using namespace tree;
 
-constexpr int WARPS = 4, THREADS = WARPS * 32;
+constexpr int WARPS = 4, THREADS = WARPS * 32, CTAS = 3;     // CTAs per SM: what registers and shared memory admit
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t* r) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -48,65 +47,61 @@ __device__ __forceinline__ void mma(float* d, const uint32_t* a, uint32_t b0, ui
                      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// A page's rows of one KV head, seen as [halves][16 rows][at most 128 bytes]: bf16 heads of 128 have two halves.
-__device__ __forceinline__ void tma_page(void* dst, const CUtensorMap* m, uint64_t* bar, int row) { tc::tma_load_3d(dst, m, bar, 0, row, 0); }
-template <bool FP8, int HD, int MI>
+template <bool FP8, int HD>
 struct Cfg {
-    static constexpr int ROWS = 16 * MI;
-    static constexpr int IT = FP8 ? 32 : 16;           // tokens of a warp's step
-    static constexpr int PAGES = IT / PAGE;
-    static constexpr int TILE = WARPS * IT;
+    static constexpr int ROWS = 16;
+    static constexpr int TILE = FP8 || HD == 64 ? 32 : 16;     // tokens of a step
+    static constexpr int PAGES = TILE / PAGE;
     static constexpr int ROW_BYTES = FP8 ? HD : 2 * HD;
     static constexpr int PAGE_BYTES = PAGE * ROW_BYTES;
     static constexpr int STAGE = 2 * PAGES * PAGE_BYTES;               // keys, then values
-    static constexpr int NST = HD == 128 ? 2 : 4;
-    static constexpr int OPAD = FP8 ? 16 : 8;
-    static constexpr int OROW = HD + OPAD;
+    static constexpr int NST = FP8 && HD == 64 ? 4 : 2;
+    // Where 16-byte piece `i` of a page's rows goes: rows of 64, 128 or 256 bytes (two halves of 128), each group of eight 16-byte places
+    // of the banks permuted by the row, so that ldmatrix meets all banks.
+    __device__ static __forceinline__ uint32_t place(int i) {
+        if (ROW_BYTES == 64) return (i >> 2) * 64 + (((i & 3) ^ ((i >> 3) & 3)) << 4);
+        if (ROW_BYTES == 128) return (i >> 3) * 128 + (((i & 7) ^ ((i >> 3) & 7)) << 4);
+        return ((i >> 3) & 1) * 2048 + (i >> 4) * 128 + (((i & 7) ^ ((i >> 4) & 7)) << 4);
+    }
     static constexpr int RING = WARPS * NST * STAGE;
-    static constexpr int OBUF = 2 * ROWS * OROW * 4;
-    static constexpr int EXPS = FP8 ? WARPS * NST * 2 * IT : 0;        // exponents of a stage: keys, then values
-    static constexpr int FACT = FP8 ? WARPS * 2 * IT * 4 : 0;          // the step's factors as fp32
-    static constexpr int SMEM = 1024 + RING + OBUF + EXPS + FACT;
+    static constexpr int EXPS = FP8 ? WARPS * NST * 2 * TILE : 0;      // exponents of a stage: keys, then values
+    static constexpr int FACT = FP8 ? WARPS * 2 * TILE * 4 : 0;        // the step's factors as fp32
+    static constexpr int SMEM = RING + EXPS + FACT;
 };
 
-template <bool FP8, int HD, int MI>
-__global__ void __launch_bounds__(THREADS, 2)
-tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeParams p) {
-    using C = Cfg<FP8, HD, MI>;
-    constexpr int IT = C::IT, NT = IT / 8, KS = HD / 16;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* ring_all = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    float* obuf = reinterpret_cast<float*>(ring_all + C::RING);
-    uint8_t* exps_all = ring_all + C::RING + C::OBUF;
+template <bool FP8, int HD>
+__global__ void __launch_bounds__(THREADS, CTAS)
+tree_attn_kernel(const TreeParams p) {
+    using C = Cfg<FP8, HD>;
+    constexpr int TILE = C::TILE, NT = TILE / 8, KS = HD / 16;
+    // log2 units: when a maximum is renewed; 8-bit pages: probabilities carry 2^UP, and f16 holds 2^(GROW + UP)
+    constexpr int UP = 4;
+    constexpr float GROW = FP8 ? 11.f : 20.f;
+    extern __shared__ __align__(128) uint8_t ring_all[];
+    uint8_t* exps_all = ring_all + C::RING;
     float* fact_all = reinterpret_cast<float*>(exps_all + C::EXPS);
     __shared__ int uoff[MAX_B + 1];
     __shared__ int wsum[WARPS];
-    __shared__ uint64_t full[WARPS][C::NST];
     __shared__ uint32_t there[WARPS][C::NST];          // bit per page of a stage: loaded
-    __shared__ float wm[2][WARPS][C::ROWS], wl[2][WARPS][C::ROWS];
-    __shared__ int we[2][WARPS];
-    __shared__ int abort_flag;
+    __shared__ float2 wml[WARPS][C::ROWS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, qd = lane & 3;
-    if (threadIdx.x == 0) {
-        for (int w = 0; w < WARPS; ++w)
-            for (int s = 0; s < C::NST; ++s) tc::mbar_init(&full[w][s], 1);
-        abort_flag = 0;
-        tc::fence_barrier_init();
-        tc::prefetch_tmap(&tmK);
-        tc::prefetch_tmap(&tmV);
-    }
-    kb_dep_trigger();
     kb_dep_wait();
-    count_tiles<C::ROWS, C::TILE, THREADS>(p, uoff, wsum);
-    const int2 part = part_of_line(uoff[p.B]);
+    kb_dep_trigger();
+    count_tiles<C::ROWS, TILE, THREADS>(p, uoff, wsum);
+    const int worker = blockIdx.x * WARPS + warp;
+    const int2 part = part_of_line(uoff[p.B], worker, gridDim.x * WARPS);
     const int lo = part.x, hi = part.y;
-    if (lo >= hi) return;
-    auto segment = [&](int x) { return segment_at<C::ROWS, C::TILE>(p, uoff, x, hi); };
+    if (uoff[p.B] == 0) return;
+    auto segment = [&](int x) { return segment_at<C::ROWS, TILE>(p, uoff, x, hi); };
 
-    // ---- producer side of this warp's ring: item k is this warp's step of tile lo + k
+    // ---- this warp's ring: item k is tile lo + k
     uint8_t* ring = ring_all + (size_t)warp * C::NST * C::STAGE;
-    uint8_t* exps = exps_all + warp * C::NST * 2 * IT;
-    Segment ps = segment(lo);
+    uint8_t* exps = exps_all + warp * C::NST * 2 * TILE;
+    const Segment unit = segment(min(lo, uoff[p.B] - 1));      // the first unit of the part
+    Segment ps = unit;
+    // Whether the block's four parts lie in one unit: their results then meet in shared memory, and the merge has a quarter of the parts.
+    const int2 cta_first = part_of_line(uoff[p.B], blockIdx.x * WARPS, gridDim.x * WARPS), cta_last = part_of_line(uoff[p.B], blockIdx.x * WARPS + WARPS - 1, gridDim.x * WARPS);
+    const bool together = cta_last.y > 0 && cta_first.x >= lo - unit.t0 && cta_last.y <= lo - unit.t0 + unit.T;
     int px = lo, pfirst = lo;                          // next tile to issue; tile at which ps begins
     int next_page = -1;                                // lane l < PAGES: page number of the next item (fetched one item ahead)
     auto fetch_page = [&]() {
@@ -115,119 +110,102 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             ps = segment(px);
             pfirst = px;
         }
-        const int tok = (ps.t0 + px - pfirst) * C::TILE + warp * IT + lane * PAGE;
+        const int tok = (ps.t0 + px - pfirst) * TILE + lane * PAGE;
         next_page = -2;                                // nothing to load
         if (lane < C::PAGES && tok < ps.ctx) next_page = p.table[(long long)ps.b * p.max_pages + tok / PAGE];
     };
     fetch_page();
     auto issue = [&]() {                               // loads item px, then looks up the page numbers of the one after it
-        if (px >= hi) return;
-        const int st = (px - lo) % C::NST;
-        const bool good = next_page >= 0 && next_page < p.num_pages;
-        if (lane < C::PAGES && next_page != -2 && !good && p.status) atomicMax(p.status, (int)KB_BAD_INDEX);
-        const uint32_t have = __ballot_sync(0xffffffffu, lane < C::PAGES && good);
-        if (lane == 0) {
-            there[warp][st] = have;
-            tc::mbar_expect_tx(&full[warp][st], __popc(have) * (2 * C::PAGE_BYTES + (FP8 ? 2 * PAGE : 0)));
-        }
-        __syncwarp();
-        if (lane < C::PAGES && good) {
-            uint8_t* dst = ring + (size_t)st * C::STAGE + lane * C::PAGE_BYTES;
-            const long long cell = (long long)next_page * p.n_kv + ps.h;
-            tma_page(dst, &tmK, &full[warp][st], (int)(cell * PAGE));
-            tma_page(dst + C::PAGES * C::PAGE_BYTES, &tmV, &full[warp][st], (int)(cell * PAGE));
-            if constexpr (FP8) {
-                uint8_t* e = exps + st * 2 * IT + lane * PAGE;
-                bulk_16(e, p.ke + cell * PAGE, &full[warp][st]);
-                bulk_16(e + IT, p.ve + cell * PAGE, &full[warp][st]);
+        if (px < hi) {
+            const int st = (px - lo) % C::NST;
+            const bool good = next_page >= 0 && next_page < p.num_pages;
+            if (lane < C::PAGES && next_page != -2 && !good && p.status) atomicMax(p.status, (int)KB_BAD_INDEX);
+            const uint32_t have = __ballot_sync(0xffffffffu, lane < C::PAGES && good);
+            if (lane == 0) there[warp][st] = have;
+            const uint32_t dst = smem_u32(ring + (size_t)st * C::STAGE);
+#pragma unroll
+            for (int pg = 0; pg < C::PAGES; ++pg) {
+                if (!(have >> pg & 1u)) continue;
+                const long long cell = (long long)__shfl_sync(0xffffffffu, next_page, pg) * p.n_kv + ps.h;
+                const uint8_t *k = p.k + cell * C::PAGE_BYTES + lane * 16, *v = p.v + cell * C::PAGE_BYTES + lane * 16;
+#pragma unroll
+                for (int i = 0; i < C::PAGE_BYTES / 512; ++i) {
+                    const uint32_t at = dst + pg * C::PAGE_BYTES + C::place(i * 32 + lane);
+                    copy16(at, k + i * 512);
+                    copy16(at + C::PAGES * C::PAGE_BYTES, v + i * 512);
+                }
+                if (FP8 && lane < 2) copy16(smem_u32(exps + st * 2 * TILE + lane * TILE + pg * PAGE), (lane ? p.ve : p.ke) + cell * PAGE);
             }
+            ++px;
+            fetch_page();
         }
-        ++px;
-        fetch_page();
+        copy_commit();                                 // (an empty group behind the last item: the count of groups goes on)
     };
     for (int i = 0; i < C::NST; ++i) issue();
 
-    bool ok = true;
-    int parity = 0;
     for (int x = lo; x < hi;) {
         const Segment sg = segment(x);
         const int row0 = sg.rb * C::ROWS, M = sg.n * p.G, prefix = sg.ctx - sg.n;
         const int c0 = p.cu ? p.cu[sg.b] : sg.b;
         // ---- the unit's queries as A fragments
-        uint32_t qa[MI][KS][4];
-        float rs[MI][2];                               // scores of rows r, r + 8 in log2 units per accumulator unit
+        uint32_t qa[KS][4];
+        float rs[2];                                   // scores of rows r, r + 8 in log2 units per accumulator unit
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-            uint2 raw[2][KS];
+        for (int hf = 0; hf < 2; ++hf) {
+            const int R = row0 + hf * 8 + r;
+            const bf16* src = p.q + (long long)(c0 + R / p.G) * p.q_stride + (long long)(sg.h * p.G + R % p.G) * HD;
+            uint2 raw[KS];
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                const int R = row0 + mi * 16 + hf * 8 + r;
-                const bf16* src = p.q + (long long)(c0 + R / p.G) * p.q_stride + (long long)(sg.h * p.G + R % p.G) * HD;
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    raw[hf][ks] = make_uint2(0u, 0u);
-                    if (R < M) {
-                        if constexpr (FP8) raw[hf][ks] = *reinterpret_cast<const uint2*>(src + ks * 16 + 4 * qd);
-                        else raw[hf][ks] = make_uint2(*reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * qd),
-                                                      *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + 2 * qd));
-                    }
+            for (int ks = 0; ks < KS; ++ks) {
+                raw[ks] = make_uint2(0u, 0u);
+                if (R < M) {
+                    if constexpr (FP8) raw[ks] = *reinterpret_cast<const uint2*>(src + ks * 16 + 4 * qd);
+                    else raw[ks] = make_uint2(*reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * qd), *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + 2 * qd));
                 }
-                rs[mi][hf] = p.scale_log2;
-                if constexpr (FP8) {                   // take a power of two out of the row, then f16
-                    uint32_t big = 0;
+            }
+            rs[hf] = p.scale_log2;
+            if constexpr (FP8) {                       // take a power of two out of the row, then f16
+                uint32_t big = 0;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks)
-                        big = max(big, max(max(raw[hf][ks].x & 0x7fffu, (raw[hf][ks].x >> 16) & 0x7fffu),
-                                           max(raw[hf][ks].y & 0x7fffu, (raw[hf][ks].y >> 16) & 0x7fffu)));
-                    big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
-                    big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                    const int e = min(max((int)(big >> 7), 1), 253);       // biased exponent of the largest number
-                    const float inv = pow2_biased(254 - e);
-                    rs[mi][hf] = p.scale_log2 * pow2_biased(e);
+                for (int ks = 0; ks < KS; ++ks) big = max(big, max(max(raw[ks].x & 0x7fffu, (raw[ks].x >> 16) & 0x7fffu), max(raw[ks].y & 0x7fffu, (raw[ks].y >> 16) & 0x7fffu)));
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
+                big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
+                const int e = min(max((int)(big >> 7), 1), 253);           // biased exponent of the largest number
+                const float inv = pow2_biased(254 - e);
+                rs[hf] = p.scale_log2 * pow2_biased(e);
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const uint32_t a = raw[hf][ks].x, b = raw[hf][ks].y;
-                        raw[hf][ks].x = pack_f16(__uint_as_float(a << 16) * inv, __uint_as_float(a & 0xffff0000u) * inv);
-                        raw[hf][ks].y = pack_f16(__uint_as_float(b << 16) * inv, __uint_as_float(b & 0xffff0000u) * inv);
-                    }
-                }
+                for (int ks = 0; ks < KS; ++ks)
+                    raw[ks] = make_uint2(pack_f16(__uint_as_float(raw[ks].x << 16) * inv, __uint_as_float(raw[ks].x & 0xffff0000u) * inv),
+                                         pack_f16(__uint_as_float(raw[ks].y << 16) * inv, __uint_as_float(raw[ks].y & 0xffff0000u) * inv));
             }
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                qa[mi][ks][0] = raw[0][ks].x;
-                qa[mi][ks][1] = raw[1][ks].x;
-                qa[mi][ks][2] = raw[0][ks].y;
-                qa[mi][ks][3] = raw[1][ks].y;
+                qa[ks][hf] = raw[ks].x;
+                qa[ks][2 + hf] = raw[ks].y;
             }
         }
-        float o[MI][HD / 8][4], m[MI][2], l[MI][2];
+        float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
         int E = 0;                                     // biased exponent of the output's unit
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi) {
-#pragma unroll
-            for (int j = 0; j < HD / 8; ++j) o[mi][j][0] = o[mi][j][1] = o[mi][j][2] = o[mi][j][3] = 0.f;
-            m[mi][0] = m[mi][1] = -INFINITY;
-            l[mi][0] = l[mi][1] = 0.f;
-        }
+        for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         for (int t = sg.t0; t < sg.t1; ++t, ++x) {
-            const int k = x - lo, st = k % C::NST;
-            if (ok && !tc::mbar_wait(&full[warp][st], (uint32_t)(k / C::NST) & 1u, &abort_flag)) ok = false;
-            ok = __shfl_sync(0xffffffffu, (int)ok, 0);
-            const int base = t * C::TILE + warp * IT;
+            const int st = (x - lo) % C::NST;
+            copy_wait<C::NST - 1>();
+            __syncwarp();
+            const int base = t * TILE;
             const uint32_t have = there[warp][st];
-            if (ok && have) {
+            if (have) {
                 const uint32_t kb = smem_u32(ring + (size_t)st * C::STAGE), vb = kb + C::PAGES * C::PAGE_BYTES;
                 uint32_t valid = 0;                    // tokens of the step that exist
 #pragma unroll
                 for (int i = 0; i < C::PAGES; ++i) valid |= (have >> i & 1u) * (0xffffu << (16 * i));
-                if (base + IT > sg.ctx) valid &= 0xffffffffu >> (32 - (sg.ctx - base));
-                const bool whole = valid == (IT == 32 ? 0xffffffffu : 0xffffu);
-                const bool drafts = base + IT > prefix;
-                float* fk = fact_all + warp * 2 * IT;
+                if (base + TILE > sg.ctx) valid &= 0xffffffffu >> (32 - (sg.ctx - base));
+                const bool whole = valid == (TILE == 32 ? 0xffffffffu : 0xffffu), drafts = base + TILE > prefix;
+                float* fk = fact_all + warp * 2 * TILE;
                 float grow = 1.f;                      // factor of the output's change of unit
                 if constexpr (FP8) {
-                    const uint8_t* e = exps + st * 2 * IT;
-                    const int ek = e[lane], ev = e[IT + lane];
+                    const uint8_t* e = exps + st * 2 * TILE;
+                    const int ek = e[lane], ev = e[TILE + lane];
                     const bool counts = (valid >> lane & 1u) && ev != 255;
                     const int top = (int)__reduce_max_sync(0xffffffffu, counts ? (unsigned)ev : 0u);
                     if (top > E) {
@@ -235,20 +213,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                         E = top;
                     }
                     fk[lane] = pow2_biased(ek);
-                    const int w = min(ev - E, 0) + 14 + 127;
-                    fk[IT + lane] = counts ? (w > 0 ? __uint_as_float((uint32_t)w << 23) : 0.f) : 1.f;
+                    const int w = min(ev - E, 0) + UP + 127;
+                    fk[TILE + lane] = counts ? (w > 0 ? __uint_as_float((uint32_t)w << 23) : 0.f) : 1.f;
                     __syncwarp();
                 }
                 // ---- scores
-                float s[MI][NT][4];
+                float s[NT][4];
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) s[mi][j][0] = s[mi][j][1] = s[mi][j][2] = s[mi][j][3] = 0.f;
+                for (int j = 0; j < NT; ++j) s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
                 if constexpr (FP8) {
-                    const int tok = (lane >> 3) * 8 + (lane & 7);          // ldmatrix: matrix lane / 8 = tokens of n tile lane / 8
-                    const uint32_t row = kb + tok * HD;
-                    const int sw = HD == 128 ? tok & 7 : (tok >> 1) & 3;
+                    const uint32_t row = kb + lane * HD;                   // ldmatrix: matrix i holds the tokens of n tile i
+                    const int sw = HD == 128 ? lane & 7 : (lane >> 1) & 3;
 #pragma unroll
                     for (int ks = 0; ks < KS; ++ks) {
                         uint32_t c[4];
@@ -257,60 +232,53 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                         for (int j = 0; j < 4; ++j) {
                             uint32_t b0, b1;
                             codes_to_f16(c[j], b0, b1);
-#pragma unroll
-                            for (int mi = 0; mi < MI; ++mi) mma<true>(s[mi][j], qa[mi][ks], b0, b1);
+                            mma<true>(s[j], qa[ks], b0, b1);
                         }
                     }
                 } else {
                     const int tok = (lane & 7) + (lane >> 4) * 8, sub = (lane >> 3) & 1;
 #pragma unroll
-                    for (int ks = 0; ks < KS; ++ks) {
-                        const int ch = ks * 2 + sub;
-                        uint32_t b[4];
-                        ldsm_x4(kb + (ch >> 3) * 2048 + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4), b);
+                    for (int pg = 0; pg < C::PAGES; ++pg)
 #pragma unroll
-                        for (int mi = 0; mi < MI; ++mi) {
-                            mma<false>(s[mi][0], qa[mi][ks], b[0], b[1]);
-                            mma<false>(s[mi][1], qa[mi][ks], b[2], b[3]);
+                        for (int ks = 0; ks < KS; ++ks) {
+                            const int ch = ks * 2 + sub;
+                            uint32_t b[4];
+                            ldsm_x4(kb + pg * C::PAGE_BYTES + (ch >> 3) * 2048 + tok * 128 + (((ch & 7) ^ (tok & 7)) << 4), b);
+                            mma<false>(s[2 * pg], qa[ks], b[0], b[1]);
+                            mma<false>(s[2 * pg + 1], qa[ks], b[2], b[3]);
                         }
-                    }
                 }
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
                     float2 f = make_float2(1.f, 1.f);
                     if constexpr (FP8) f = *reinterpret_cast<const float2*>(fk + 8 * j + 2 * qd);
-#pragma unroll
-                    for (int mi = 0; mi < MI; ++mi) {
-                        s[mi][j][0] *= f.x * rs[mi][0];
-                        s[mi][j][1] *= f.y * rs[mi][0];
-                        s[mi][j][2] *= f.x * rs[mi][1];
-                        s[mi][j][3] *= f.y * rs[mi][1];
-                    }
+                    s[j][0] *= f.x * rs[0];
+                    s[j][1] *= f.y * rs[0];
+                    s[j][2] *= f.x * rs[1];
+                    s[j][3] *= f.y * rs[1];
                 }
                 // ---- what is not seen: places that hold no token, and drafted tokens the row's mask does not name
                 uint32_t odd = 0;                      // drafted tokens whose values are not finite: kept out of the product
-                unsigned long long seen[MI][2];        // bit t: the row sees token t of the step (only where something is hidden)
+                uint32_t seen[2] = {0u, 0u};           // bit t: the row sees token t of the step (only where something is hidden)
                 if (!whole || drafts) {
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
+                    for (int hf = 0; hf < 2; ++hf) {
+                        const int i = min((row0 + hf * 8 + r) / p.G, sg.n - 1);
+                        seen[hf] = (uint32_t)sees(p, c0, i, base - prefix) & valid;
 #pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            const int i = min((row0 + mi * 16 + hf * 8 + r) / p.G, sg.n - 1);
-                            seen[mi][hf] = sees(p, c0, i, base - prefix) & valid;
-#pragma unroll
-                            for (int j = 0; j < NT; ++j) {
-                                const uint32_t two = (uint32_t)(seen[mi][hf] >> (8 * j + 2 * qd)) & 3u;
-                                if (!(two & 1u)) s[mi][j][2 * hf] = -INFINITY;
-                                if (!(two & 2u)) s[mi][j][2 * hf + 1] = -INFINITY;
-                            }
+                        for (int j = 0; j < NT; ++j) {
+                            const uint32_t two = seen[hf] >> (8 * j + 2 * qd);
+                            if (!(two & 1u)) s[j][2 * hf] = -INFINITY;
+                            if (!(two & 2u)) s[j][2 * hf + 1] = -INFINITY;
                         }
+                    }
                     if (drafts) {
                         bool bad = false;
-                        if (lane < IT && (valid >> lane & 1u) && base + lane >= prefix) {
-                            const uint8_t* row = ring + (size_t)st * C::STAGE + C::PAGES * C::PAGE_BYTES + (lane / PAGE) * C::PAGE_BYTES;
-                            const int tr = lane % PAGE;
+                        if (lane < TILE && (valid >> lane & 1u) && base + lane >= prefix) {
+                            const uint8_t* page = ring + (size_t)st * C::STAGE + (C::PAGES + lane / PAGE) * C::PAGE_BYTES;
+#pragma unroll 1
                             for (int c = 0; c < C::ROW_BYTES / 16; ++c) {
-                                const uint4 v = *reinterpret_cast<const uint4*>(FP8 ? row + tr * HD + c * 16 : row + (c >> 3) * 2048 + tr * 128 + (c & 7) * 16);
+                                const uint4 v = *reinterpret_cast<const uint4*>(page + C::place((lane % PAGE) * (C::ROW_BYTES / 16) + c));
                                 const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                                 for (int q = 0; q < 4; ++q)
@@ -320,79 +288,95 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                         odd = __ballot_sync(0xffffffffu, bad);
                     }
                 }
-                // ---- online softmax
-                uint32_t pa[MI][IT / 16][4];
-                bool still = true;
-                float f[MI][2];
+                // ---- softmax against a maximum that is renewed only when a score exceeds it by more than GROW
+                float mx[2];
 #pragma unroll
-                for (int mi = 0; mi < MI; ++mi)
+                for (int hf = 0; hf < 2; ++hf) {
+                    mx[hf] = fmaxf(s[0][2 * hf], s[0][2 * hf + 1]);
+#pragma unroll
+                    for (int j = 1; j < NT; ++j) mx[hf] = fmaxf(mx[hf], fmaxf(s[j][2 * hf], s[j][2 * hf + 1]));
+                }
+                if (__any_sync(0xffffffffu, mx[0] > m[0] + GROW || mx[1] > m[1] + GROW || (FP8 && grow != 1.f))) {
+                    float f[2];
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
-                        float mx = -INFINITY;
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) mx = fmaxf(mx, fmaxf(s[mi][j][2 * hf], s[mi][j][2 * hf + 1]));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                        const float mn = fmaxf(m[mi][hf], mx), at = mn == -INFINITY ? 0.f : mn;
-                        const float g = exp2f(m[mi][hf] - at);
-                        m[mi][hf] = mn;
-                        float sum = 0.f;
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            s[mi][j][2 * hf] = exp2f(s[mi][j][2 * hf] - at);
-                            s[mi][j][2 * hf + 1] = exp2f(s[mi][j][2 * hf + 1] - at);
-                            sum += s[mi][j][2 * hf] + s[mi][j][2 * hf + 1];
-                        }
-                        l[mi][hf] = l[mi][hf] * g + sum;
-                        f[mi][hf] = g * grow;
-                        still = still && f[mi][hf] == 1.f;
+                        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+                        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+                        const float mn = fmaxf(m[hf], mx[hf]);
+                        f[hf] = mn == -INFINITY ? 1.f : exp2f(m[hf] - mn);
+                        m[hf] = mn;
+                        l[hf] *= f[hf];
+                        f[hf] *= grow;
                     }
-                if (!__all_sync(0xffffffffu, still)) {
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                        for (int j = 0; j < HD / 8; ++j) {
-                            o[mi][j][0] *= f[mi][0];
-                            o[mi][j][1] *= f[mi][0];
-                            o[mi][j][2] *= f[mi][1];
-                            o[mi][j][3] *= f[mi][1];
-                        }
+                    for (int j = 0; j < HD / 8; ++j) {
+                        o[j][0] *= f[0];
+                        o[j][1] *= f[0];
+                        o[j][2] *= f[1];
+                        o[j][3] *= f[1];
+                    }
                 }
+                uint32_t pa[TILE / 16][4];
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    if constexpr (FP8) {
-                        const float2 w = *reinterpret_cast<const float2*>(fk + IT + 8 * j + 2 * qd);
+                for (int hf = 0; hf < 2; ++hf) {
+                    const float at = m[hf] == -INFINITY ? 0.f : m[hf];
 #pragma unroll
-                        for (int mi = 0; mi < MI; ++mi) {
-                            s[mi][j][0] *= w.x;
-                            s[mi][j][1] *= w.y;
-                            s[mi][j][2] *= w.x;
-                            s[mi][j][3] *= w.y;
+                    for (int j = 0; j < NT; ++j) {
+                        float a = exp2f(s[j][2 * hf] - at), z = exp2f(s[j][2 * hf + 1] - at);
+                        l[hf] += a + z;
+                        if constexpr (FP8) {
+                            const float2 w = *reinterpret_cast<const float2*>(fk + TILE + 8 * j + 2 * qd);
+                            a *= w.x;
+                            z *= w.y;
                         }
+                        s[j][2 * hf] = a;
+                        s[j][2 * hf + 1] = z;
+                        pa[j >> 1][(j & 1) * 2 + hf] = FP8 ? pack_f16(a, z) : pack_bf16(a, z);
                     }
+                }
+                if (!whole || odd) {
+                    // Values that must not enter the product: what the cache holds in places without a token, and drafted tokens that
+                    // are not finite - those are added row by row (never in normal use)
+                    uint8_t* pages = ring + (size_t)st * C::STAGE + C::PAGES * C::PAGE_BYTES;
+#pragma unroll 1
+                    for (uint32_t left = odd; left; left &= left - 1u) {
+                        const int tk = __ffs(left) - 1, src = (lane & ~3) | ((tk & 7) >> 1), tr = tk % PAGE;
+                        const uint8_t* page = pages + (tk / PAGE) * C::PAGE_BYTES;
+                        float pv[2];
 #pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
+                        for (int hf = 0; hf < 2; ++hf) {
+                            float mine = 0.f;
 #pragma unroll
-                        for (int hf = 0; hf < 2; ++hf)
-                            pa[mi][j >> 1][(j & 1) * 2 + hf] = FP8 ? pack_f16(s[mi][j][2 * hf], s[mi][j][2 * hf + 1])
-                                                                   : pack_bf16(s[mi][j][2 * hf], s[mi][j][2 * hf + 1]);
+                            for (int j = 0; j < NT; ++j)
+                                if (j == tk >> 3) mine = tk & 1 ? s[j][2 * hf + 1] : s[j][2 * hf];
+                            pv[hf] = __shfl_sync(0xffffffffu, mine, src);
+                        }
+#pragma unroll
+                        for (int j = 0; j < HD / 8; ++j)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int d = FP8 ? (j >> 1) * 16 + 4 * qd + 2 * e + (j & 1) : 8 * j + 2 * qd + e, byte = FP8 ? d : 2 * d;
+                                const uint8_t* at = page + C::place(tr * (C::ROW_BYTES / 16) + byte / 16) + byte % 16;
+                                const float v = FP8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(*at, __NV_E4M3))) : __bfloat162float(*reinterpret_cast<const bf16*>(at));
+                                if (seen[0] >> tk & 1u) o[j][e] += pv[0] * v;
+                                if (seen[1] >> tk & 1u) o[j][2 + e] += pv[1] * v;
+                            }
+                    }
+                    __syncwarp();
+                    if (lane < TILE && !(valid >> lane & ~(odd >> lane) & 1u))
+#pragma unroll 1
+                        for (int c = 0; c < C::ROW_BYTES / 16; ++c)
+                            *reinterpret_cast<uint4*>(pages + (lane / PAGE) * C::PAGE_BYTES + C::place((lane % PAGE) * (C::ROW_BYTES / 16) + c)) = make_uint4(0u, 0u, 0u, 0u);
+                    __syncwarp();
                 }
                 // ---- output
-                const uint32_t use = valid & ~odd;
-                const bool cut = !whole || odd;
                 const int vtok = (lane & 7) + ((lane >> 3) & 1) * 8, vsub = lane >> 4;
 #pragma unroll
-                for (int kk = 0; kk < IT / 16; ++kk) {
-                    uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;     // tokens 2 qd, 2 qd + 1 (+ 8) of the page, 16 bits each
-                    if (cut) {
-                        const uint32_t a = use >> (16 * kk + 2 * qd), z = use >> (16 * kk + 8 + 2 * qd);
-                        keep0 = (a & 1u ? 0xffffu : 0u) | (a & 2u ? 0xffff0000u : 0u);
-                        keep1 = (z & 1u ? 0xffffu : 0u) | (z & 2u ? 0xffff0000u : 0u);
-                    }
+                for (int kk = 0; kk < TILE / 16; ++kk) {
+                    const uint32_t page = vb + kk * C::PAGE_BYTES;
                     if constexpr (FP8) {
-                        const int tok = kk * 16 + vtok;
-                        const uint32_t row = vb + tok * HD;
-                        const int sw = HD == 128 ? tok & 7 : (tok >> 1) & 3;
+                        const uint32_t row = page + vtok * HD;
+                        const int sw = HD == 128 ? vtok & 7 : (vtok >> 1) & 3;
 #pragma unroll
                         for (int c = 0; c < HD / 16; c += 2) {
                             uint32_t v[4];
@@ -400,13 +384,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 #pragma unroll
                             for (int i = 0; i < 2; ++i) {
                                 uint32_t e0, o0, e1, o1;                   // even and odd head dimensions of the chunk
-                                codes_to_f16(__byte_perm(v[2 * i] & keep0, 0, 0x3120), e0, o0);
-                                codes_to_f16(__byte_perm(v[2 * i + 1] & keep1, 0, 0x3120), e1, o1);
-#pragma unroll
-                                for (int mi = 0; mi < MI; ++mi) {
-                                    mma<true>(o[mi][2 * (c + i)], pa[mi][kk], e0, e1);
-                                    mma<true>(o[mi][2 * (c + i) + 1], pa[mi][kk], o0, o1);
-                                }
+                                codes_to_f16(__byte_perm(v[2 * i], 0, 0x3120), e0, o0);
+                                codes_to_f16(__byte_perm(v[2 * i + 1], 0, 0x3120), e1, o1);
+                                mma<true>(o[2 * (c + i)], pa[kk], e0, e1);
+                                mma<true>(o[2 * (c + i) + 1], pa[kk], o0, o1);
                             }
                         }
                     } else {
@@ -414,163 +395,117 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                         for (int j = 0; j < HD / 16; ++j) {
                             const int ch = j * 2 + vsub;
                             uint32_t v[4];
-                            ldsm_x4_t(vb + (ch >> 3) * 2048 + vtok * 128 + (((ch & 7) ^ (vtok & 7)) << 4), v);
-#pragma unroll
-                            for (int mi = 0; mi < MI; ++mi) {
-                                mma<false>(o[mi][2 * j], pa[mi][kk], v[0] & keep0, v[1] & keep1);
-                                mma<false>(o[mi][2 * j + 1], pa[mi][kk], v[2] & keep0, v[3] & keep1);
-                            }
+                            ldsm_x4_t(page + (ch >> 3) * 2048 + vtok * 128 + (((ch & 7) ^ (vtok & 7)) << 4), v);
+                            mma<false>(o[2 * j], pa[kk], v[0], v[1]);
+                            mma<false>(o[2 * j + 1], pa[kk], v[2], v[3]);
                         }
                     }
-                }
-                for (uint32_t left = odd; left; left &= left - 1u) {       // rare: rows that see such a token get its products one by one
-                    const int tk = __ffs(left) - 1, src = (lane & ~3) | ((tk & 7) >> 1);
-                    const uint8_t* row = ring + (size_t)st * C::STAGE + C::PAGES * C::PAGE_BYTES + (tk / PAGE) * C::PAGE_BYTES;
-                    const int tr = tk % PAGE;
-#pragma unroll
-                    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            float mine = 0.f;
-#pragma unroll
-                            for (int j = 0; j < NT; ++j)
-                                if (j == tk >> 3) mine = tk & 1 ? s[mi][j][2 * hf + 1] : s[mi][j][2 * hf];
-                            const float pv = __shfl_sync(0xffffffffu, mine, src);
-                            if (!(seen[mi][hf] >> tk & 1ull)) continue;
-#pragma unroll
-                            for (int j = 0; j < HD / 8; ++j)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    float v;
-                                    if constexpr (FP8) {
-                                        const int d = (j >> 1) * 16 + 4 * qd + 2 * e + (j & 1), c = d >> 4;
-                                        const int sw = HD == 128 ? tr & 7 : (tr >> 1) & 3;
-                                        v = __half2float(__half(__nv_cvt_fp8_to_halfraw(row[tr * HD + ((c ^ sw) << 4) + (d & 15)], __NV_E4M3)));
-                                    } else {
-                                        const int d = 8 * j + 2 * qd + e, c = d >> 3;
-                                        v = __bfloat162float(*reinterpret_cast<const bf16*>(row + (c >> 3) * 2048 + tr * 128 + (((c & 7) ^ (tr & 7)) << 4) + (d & 7) * 2));
-                                    }
-                                    o[mi][j][2 * hf + e] += pv * v;
-                                }
-                        }
                 }
             }
             __syncwarp();                              // every lane has read the stage
-            if (ok) {
-                tc::fence_proxy_async();
-                issue();
-            }
+            issue();
         }
-        // ---- the warps' results meet
+        // ---- the unit's rows, as far as this warp has them
+        const bool done = !together && sg.t0 == 0 && sg.t1 == sg.T;
+        const long long slot = 2ll * worker + (sg.t0 == 0);
+        float* part_o = p.part_o + slot * C::ROWS * HD;
+        if (together) {                                // the ring is idle now: [16][HD] floats at its start
+            copy_wait<0>();
+            __syncwarp();
+            part_o = reinterpret_cast<float*>(ring);
+        }
 #pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
+        for (int hf = 0; hf < 2; ++hf) {
+            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 1);
+            l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
+            const int row = hf * 8 + r, R = row0 + row;
+            if (R >= M) continue;
+            float g = FP8 ? pow2_biased(E) * (1.f / (1 << UP)) : 1.f;      // 2^(E - 127 - UP)
+            if (done) g *= l[hf] == 0.f ? 0.f : 1.f / l[hf];
+            bf16* dst = p.out + (long long)(c0 + R / p.G) * p.out_stride + (long long)(sg.h * p.G + R % p.G) * HD;
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {
-                l[mi][hf] += __shfl_xor_sync(0xffffffffu, l[mi][hf], 1);
-                l[mi][hf] += __shfl_xor_sync(0xffffffffu, l[mi][hf], 2);
-                if (qd == 0) {
-                    wm[parity][warp][mi * 16 + hf * 8 + r] = m[mi][hf];
-                    wl[parity][warp][mi * 16 + hf * 8 + r] = l[mi][hf];
+            for (int j = 0; j < HD / 8; ++j) {
+                if constexpr (FP8) {                   // dimensions 4 qd .. 4 qd + 3 of a chunk of 16: evens in one tile, odds in the other
+                    if (j & 1) continue;
+                    const int d = j * 8 + 4 * qd;
+                    const float a = o[j][2 * hf] * g, b = o[j + 1][2 * hf] * g, c = o[j][2 * hf + 1] * g, e = o[j + 1][2 * hf + 1] * g;
+                    if (done) *reinterpret_cast<uint2*>(dst + d) = make_uint2(pack_bf16(a, b), pack_bf16(c, e));
+                    else *reinterpret_cast<float4*>(part_o + row * HD + d) = make_float4(a, b, c, e);
+                } else {
+                    const int d = j * 8 + 2 * qd;
+                    const float a = o[j][2 * hf] * g, b = o[j][2 * hf + 1] * g;
+                    if (done) *reinterpret_cast<uint32_t*>(dst + d) = pack_bf16(a, b);
+                    else *reinterpret_cast<float2*>(part_o + row * HD + d) = make_float2(a, b);
                 }
             }
-        if (lane == 0) we[parity][warp] = E;
-        __syncthreads();
-        const float unit = FP8 ? pow2_biased(E) * 6.103515625e-05f : 1.f;              // 2^(E - 127 - 14)
-        float* buf = obuf + (warp & 1) * C::ROWS * C::OROW;
-#pragma unroll
-        for (int turn = 0; turn < 2; ++turn) {
-            if ((warp >> 1) == turn) {
-#pragma unroll
-                for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-                    for (int hf = 0; hf < 2; ++hf) {
-                        const int row = mi * 16 + hf * 8 + r;
-                        float top = wm[parity][0][row];
-#pragma unroll
-                        for (int w = 1; w < WARPS; ++w) top = fmaxf(top, wm[parity][w][row]);
-                        const float g = m[mi][hf] == -INFINITY ? 0.f : exp2f(m[mi][hf] - top) * unit;
-                        const bool none = m[mi][hf] == -INFINITY && l[mi][hf] == 0.f;   // (a NaN sum has to get through)
-                        float* dst = buf + row * C::OROW;
-#pragma unroll
-                        for (int j = 0; j < HD / 8; ++j) {
-                            const int d0 = FP8 ? (j >> 1) * 16 + 4 * qd + (j & 1) : 8 * j + 2 * qd, d1 = d0 + (FP8 ? 2 : 1);
-                            const float a = none ? 0.f : o[mi][j][2 * hf] * g, z = none ? 0.f : o[mi][j][2 * hf + 1] * g;
-                            if (turn == 0) {
-                                dst[d0] = a;
-                                dst[d1] = z;
-                            } else {
-                                dst[d0] += a;
-                                dst[d1] += z;
-                            }
-                        }
-                    }
-            }
-            __syncthreads();
-        }
-        const bool done = sg.t0 == 0 && sg.t1 == sg.T;
-        const long long slot = 2ll * blockIdx.x + (sg.t0 == 0);
-        for (int i = threadIdx.x; i < C::ROWS * (HD / 4); i += THREADS) {
-            const int row = i % C::ROWS, d = i / C::ROWS * 4, R = row0 + row;
-            if (R >= M) continue;
-            const float4 a = *reinterpret_cast<const float4*>(obuf + row * C::OROW + d);
-            const float4 z = *reinterpret_cast<const float4*>(obuf + (C::ROWS + row) * C::OROW + d);
-            float4 v = make_float4(a.x + z.x, a.y + z.y, a.z + z.z, a.w + z.w);
-            float top = wm[parity][0][row], sum = 0.f;
-#pragma unroll
-            for (int w = 1; w < WARPS; ++w) top = fmaxf(top, wm[parity][w][row]);
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) {
-                const float mw = wm[parity][w][row], lw = wl[parity][w][row];
-                sum += mw == -INFINITY ? lw : lw * exp2f(mw - top);          // lw is 0 or NaN where there is no maximum
-            }
-            if (done) {
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
-                bf16* dst = p.out + (long long)(c0 + R / p.G) * p.out_stride + (long long)(sg.h * p.G + R % p.G) * HD + d;
-                *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
-            } else {
-                *reinterpret_cast<float4*>(p.part_o + ((slot * (HD / 4) + d / 4) * C::ROWS + row) * 4) = v;
-                if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * C::ROWS + row) * 2) = make_float2(top, sum);
+            if (!done && qd == 0) {
+                if (together) wml[warp][row] = make_float2(m[hf], l[hf]);
+                else *reinterpret_cast<float2*>(p.part_ml + (slot * C::ROWS + row) * 2) = make_float2(m[hf], l[hf]);
             }
         }
-        parity ^= 1;
     }
-    if (!ok) {
-        // a copy did not arrive in time: report, and let copies in flight land before the shared memory goes
-        if (lane == 0) {
-            atomicMax(p.status, (int)KB_TIMEOUT_TMA);
-            const uint64_t t0 = global_timer_ns();
-            while (global_timer_ns() - t0 < 2000000ull) {}
+    copy_wait<0>();
+    if (!together) return;
+    __syncthreads();
+    const int x0 = cta_first.x - (lo - unit.t0), x1 = cta_last.y - (lo - unit.t0);     // the block's tiles of the unit
+    const bool done = x0 == 0 && x1 == unit.T;
+    const long long slot = 2ll * blockIdx.x * WARPS + (x0 == 0);
+    const int M = unit.n * p.G - unit.rb * C::ROWS, c0 = p.cu ? p.cu[unit.b] : unit.b;
+    for (int i = threadIdx.x; i < min(M, C::ROWS) * (HD / 4); i += THREADS) {
+        const int row = i / (HD / 4), d = i % (HD / 4) * 4;
+        float top = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, wml[w][row].x);
+        const float at = top == -INFINITY ? 0.f : top;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float2 ml = wml[w][row];
+            const float g = exp2f(ml.x - at);
+            sum += ml.x == -INFINITY ? ml.y : ml.y * g;                    // a sum without a maximum is zero, or NaN and has to get through
+            const float4 u = *reinterpret_cast<const float4*>(ring_all + (size_t)w * C::NST * C::STAGE + (row * HD + d) * 4);
+            v.x += u.x * g;
+            v.y += u.y * g;
+            v.z += u.z * g;
+            v.w += u.w * g;
         }
-        __syncwarp();
+        if (done) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int R = unit.rb * C::ROWS + row;
+            bf16* dst = p.out + (long long)(c0 + R / p.G) * p.out_stride + (long long)(unit.h * p.G + R % p.G) * HD + d;
+            *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(v.x * inv, v.y * inv), pack_bf16(v.z * inv, v.w * inv));
+        } else {
+            *reinterpret_cast<float4*>(p.part_o + (slot * C::ROWS + row) * HD + d) = v;
+            if (d == 0) *reinterpret_cast<float2*>(p.part_ml + (slot * C::ROWS + row) * 2) = make_float2(top, sum);
+        }
     }
 }
 
-// Puts the parts of a unit together; WPR warps share a row.  Rows of sequences without rows or tokens, and (zero_tail) rows behind the
-// last sequence, become zero.
-template <int HD, int WPR>
-__global__ void __launch_bounds__(256)
-tree_merge_kernel(const TreeParams p, int ROWS, int TILE, int grid, int zero_tail) {
-    kb_dep_trigger();
-    kb_dep_wait();
-    constexpr int RPB = 8 / WPR, EPL = HD / 32;        // rows per block; dimensions per lane
-    __shared__ float so[WPR > 1 ? 8 : 1][HD], sml[8][2];
+// Puts the parts of a unit together; WPR warps share a row.  `per`: workers of a block; where all of a block's parts lie in the unit the
+// block has left one part for them.  Rows of sequences without rows or tokens, and (zero_tail) rows behind the last sequence, become zero.
+// ROW_MAJOR: parts are [rows][HD], else [HD / 4][rows][4].
+template <int HD, int WPR, bool ROW_MAJOR>
+__global__ void __launch_bounds__(WPR == 1 ? 256 : WPR * 32)
+tree_merge_kernel(const TreeParams p, int ROWS, int TILE, int workers, int per, int zero_tail) {
+    constexpr int RPB = WPR == 1 ? 8 : 1, EPL = HD / 32;       // rows per block; dimensions per lane
+    __shared__ float so[WPR > 1 ? WPR : 1][HD], sml[WPR][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
     const long long row = (long long)blockIdx.x * RPB + warp / WPR;
-    if (row >= (long long)p.N * p.H) return;           // (with WPR = 8 the whole block)
+    if (row >= (long long)p.N * p.H) return;           // (with several warps per row the whole block)
+    // What the sequences are was known before the kernel ahead began (it lets this one start after its own wait)
     const int n = (int)(row / p.H), head = (int)(row % p.H), h = head / p.G;
     int b = n;
-    if (p.cu) {
-        int a = 0, z = p.B;
-        while (z - a > 1) {
-            const int mid = (a + z) >> 1;
-            if (p.cu[mid] <= n) a = mid; else z = mid;
-        }
-        b = a;
+    if (p.cu) {                                        // sequences that end at or before row n
+        b = 0;
+        for (int i = lane; i < p.B; i += 32) b += p.cu[i + 1] <= n;
+        b = __reduce_add_sync(0xffffffffu, b);
     }
     const int c0 = b < p.B ? (p.cu ? p.cu[b] : b) : 0, c1 = b < p.B ? (p.cu ? p.cu[b + 1] : b + 1) : 0;
     const bool inside = b < p.B && n >= c0 && n < c1;
     bf16* dst = p.out + (long long)n * p.out_stride + (long long)head * HD + lane * EPL;
     const int2 sp = inside ? span_of(p, b, false) : make_int2(0, 0);
+    kb_dep_wait();
+    kb_dep_trigger();
     if (sp.x == 0) {
         if ((inside || zero_tail) && sub == 0)
 #pragma unroll
@@ -579,30 +514,41 @@ tree_merge_kernel(const TreeParams p, int ROWS, int TILE, int grid, int zero_tai
     }
     const int Rl = (n - c0) * p.G + head % p.G, rbs = (sp.x * p.G + ROWS - 1) / ROWS, T = (sp.y + TILE - 1) / TILE;
     const long long total = p.uoff[p.B], s0 = p.uoff[b] + (long long)(h * rbs + Rl / ROWS) * T;
-    const long long parts = min((long long)grid, total);
+    const long long parts = min((long long)workers, total);
     const int first = (int)(((s0 + 1) * parts - 1) / total), last = (int)(((s0 + T) * parts - 1) / total);
-    if (first == last) return;                         // finished by its CTA
+    // blocks of the first and last part, and whether a block has left one part
+    const int cA = first / per, cB = last / per;
+    auto whole = [&](int c) {
+        return (long long)(c + 1) * per <= parts && total * c * per / parts >= s0 && total * (c + 1) * per / parts <= s0 + T;
+    };
+    const bool wA = whole(cA), wB = whole(cB);
+    if (wA && cA == cB && s0 == total * cA * per / parts && s0 + T == total * (cA + 1) * per / parts) return;      // finished by its block
+    if (first == last && !wA) return;                  // finished by its worker
+    const int head_n = wA ? 1 : min(last, cA * per + per - 1) - first + 1, mid_n = cB > cA ? cB - cA - 1 : 0;
+    const int all = head_n + mid_n + (cB > cA ? (wB ? 1 : last - cB * per + 1) : 0);
     const int r = Rl % ROWS;
     float M = -INFINITY, L = 0.f, acc[EPL];
 #pragma unroll
     for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
     constexpr int U = 4;                               // parts in flight
-    for (int j0 = first + sub; j0 <= last; j0 += WPR * U) {
+    for (int k0 = sub; k0 < all; k0 += WPR * U) {
         float2 ml[U];
         float v[U][EPL];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int j = j0 + u * WPR;
+            const int k = k0 + u * WPR;
             ml[u] = make_float2(-INFINITY, 0.f);
 #pragma unroll
             for (int e = 0; e < EPL; ++e) v[u][e] = 0.f;
-            if (j <= last) {
-                const long long at = (2ll * j + (j == first)) * ROWS + r;
-                ml[u] = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+            if (k < all) {
+                const int j = k < head_n ? first + k : k < head_n + mid_n ? (cA + 1 + k - head_n) * per : cB * per + k - head_n - mid_n;
+                const long long slot = 2ll * j + (j == first);
+                ml[u] = *reinterpret_cast<const float2*>(p.part_ml + (slot * ROWS + r) * 2);
 #pragma unroll
                 for (int e = 0; e < EPL; e += 2) {
                     const int d = lane * EPL + e;
-                    *reinterpret_cast<float2*>(&v[u][e]) = *reinterpret_cast<const float2*>(p.part_o + (((2ll * j + (j == first)) * (HD / 4) + d / 4) * ROWS + r) * 4 + d % 4);
+                    const float* src = p.part_o + (ROW_MAJOR ? (slot * ROWS + r) * HD + d : ((slot * (HD / 4) + d / 4) * ROWS + r) * 4 + d % 4);
+                    *reinterpret_cast<float2*>(&v[u][e]) = *reinterpret_cast<const float2*>(src);
                 }
             }
         }
@@ -625,13 +571,13 @@ tree_merge_kernel(const TreeParams p, int ROWS, int TILE, int grid, int zero_tai
         __syncthreads();
         if (sub != 0) return;
         float top = M;
-#pragma unroll
+#pragma unroll 8
         for (int w = 1; w < WPR; ++w) top = fmaxf(top, sml[w][0]);
         const float at = top == -INFINITY ? 0.f : top;
         L = 0.f;
 #pragma unroll
         for (int e = 0; e < EPL; ++e) acc[e] = 0.f;
-#pragma unroll
+#pragma unroll 4
         for (int w = 0; w < WPR; ++w) {
             const float g = exp2f(sml[w][0] - at);
             L += sml[w][0] == -INFINITY ? sml[w][1] : sml[w][1] * g;
@@ -644,32 +590,7 @@ tree_merge_kernel(const TreeParams p, int ROWS, int TILE, int grid, int zero_tai
     for (int e = 0; e < EPL; e += 2) *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
 }
 
-typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeFn encoder() {
-    static EncodeFn enc = nullptr;
-    if (!enc) {
-        void* ptr = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
-        enc = reinterpret_cast<EncodeFn>(ptr);
-    }
-    return enc;
-}
 }  // namespace
-
-int tree::page_map(CUtensorMap* m, const void* base, long long rows, int hd, bool fp8, bool halves_apart) {
-    const EncodeFn enc = encoder();
-    if (!enc) return 100;
-    const int row_bytes = fp8 ? hd : 2 * hd, in = row_bytes > 128 ? 128 : row_bytes, esz = fp8 ? 1 : 2;
-    const cuuint64_t dims[3] = {(cuuint64_t)(in / esz), (cuuint64_t)rows, (cuuint64_t)(row_bytes / in)};
-    const cuuint64_t strides[2] = {(cuuint64_t)row_bytes, (cuuint64_t)in};
-    const cuuint32_t box[3] = {(cuuint32_t)(in / esz), PAGE, halves_apart ? 1u : (cuuint32_t)(row_bytes / in)}, one[3] = {1, 1, 1};
-    const CUresult r = enc(m, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box,
-                           one, CU_TENSOR_MAP_INTERLEAVE_NONE, in == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
-                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    return r == CUDA_SUCCESS ? 0 : 200 + (int)r;
-}
 
 int tree::sm_count() {
     static int count[64] = {};
@@ -679,63 +600,78 @@ int tree::sm_count() {
     return count[dev];
 }
 
-int tree::merge(const TreeParams& p, int hd, int rows, int tile, int grid, bool wide, int zero_tail, cudaStream_t st) {
-    const long long n = (long long)p.N * p.H;
-#define MERGE(HD_, W_)                                                                                                                  \
-    return kb_launch_dep(tree_merge_kernel<HD_, W_>, dim3((unsigned)((n + 8 / W_ - 1) / (8 / W_))), dim3(256), 0, st, p, rows, tile, grid, zero_tail)
-    if (hd == 128) {
-        if (wide) MERGE(128, 8);
-        MERGE(128, 1);
-    }
-    if (wide) MERGE(64, 8);
-    MERGE(64, 1);
-#undef MERGE
-}
-
 namespace {
 
 struct Plan {
-    int rows, tile, grid;
-    bool wide;
+    int rows, tile, grid, workers, per_cta, merge_warps;
 };
-// Which kernel, and how many CTAs: one per tile, at most what fits the GPU at once (one per SM for the 128-row kernel, two for the
-// others).
-Plan plan_for(int B, int N, int n_kv, int G, int max_q, int max_ctx, bool fp8) {
+// Which kernel, and how many CTAs: as many as there are tiles for, at most what fits the GPU at once.  More than 16 query rows per KV head
+// take the 128-row kernel: measured at 64 sequences over 2048 tokens with 32 rows, 8-bit / bf16 pages, 164 / 110 us against 200 / 215 us for
+// tiles of 32 rows here; with 16 rows 157 / 104 us against 75 / 84 us for the 16-row kernel.
+// The merge walks a unit's parts with one warp per row where there are about eight of them, else with 8 or 32.
+Plan plan_for(int B, int N, int n_kv, int G, int hd, int max_q, int max_ctx, bool fp8) {
     Plan pl;
     const int most_rows = max_q * G;
-    pl.rows = most_rows <= 16 ? 16 : most_rows <= 32 ? 32 : 128;
-    pl.tile = pl.rows == 128 ? 128 : WARPS * (fp8 ? 32 : 16);
+    pl.rows = most_rows <= 16 ? 16 : 128;
+    pl.tile = pl.rows == 128 ? 128 : fp8 || hd == 64 ? 32 : 16;
     const long long blocks = B + (long long)N * G / pl.rows;                            // units per KV head, at most
     const long long one = (most_rows + pl.rows - 1) / pl.rows;
     const long long units = n_kv * (blocks < B * one ? blocks : B * one), tiles = units * ((max_ctx + pl.tile - 1) / pl.tile);
-    const long long most = (pl.rows == 128 ? 1ll : 2ll) * sm_count();
-    pl.grid = (int)(tiles < most ? tiles : most);
-    pl.wide = pl.grid > 8 * units;                     // parts per unit: one warp per row walks up to about eight of them
+    pl.per_cta = pl.rows == 128 ? 1 : WARPS;
+    const long long want = (tiles + pl.per_cta - 1) / pl.per_cta, most = (long long)(pl.rows == 128 ? 1 : CTAS) * sm_count();
+    pl.grid = (int)(want < most ? want : most);
+    pl.workers = pl.grid * pl.per_cta;
+    pl.merge_warps = pl.grid <= 8 * units ? 1 : pl.grid <= 64 * units ? 8 : 32;
     return pl;
 }
 
-template <bool FP8, int HD, int MI>
-int launch_tree(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams& p, const Plan& pl, cudaStream_t st) {
+// The merge always starts while the kernel ahead of it runs: it waits for it on the device.
+template <int HD, int W, bool ROW_MAJOR>
+int launch_merge(const TreeParams& p, const Plan& pl, int zero_tail, cudaStream_t st) {
+    const long long n = (long long)p.N * p.H;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(W == 1 ? (n + 7) / 8 : n));
+    cfg.blockDim = dim3(W == 1 ? 256 : W * 32);
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaLaunchKernelEx(&cfg, tree_merge_kernel<HD, W, ROW_MAJOR>, p, pl.rows, pl.tile, pl.workers, pl.per_cta, zero_tail) == cudaSuccess) return 0;
+    cudaGetLastError();
+    return KB_LAUNCH_FAILED;
+}
+template <int HD, bool ROW_MAJOR>
+int merge(const TreeParams& p, const Plan& pl, int zero_tail, cudaStream_t st) {
+    return pl.merge_warps == 1   ? launch_merge<HD, 1, ROW_MAJOR>(p, pl, zero_tail, st)
+           : pl.merge_warps == 8 ? launch_merge<HD, 8, ROW_MAJOR>(p, pl, zero_tail, st)
+                                 : launch_merge<HD, 32, ROW_MAJOR>(p, pl, zero_tail, st);
+}
+
+template <bool FP8, int HD>
+int launch_tree(const TreeParams& p, const Plan& pl, cudaStream_t st) {
     static bool flags[64] = {};
     bool* set = kb_device_flag(flags);
     if (!set) return 7;
     if (!*set) {
-        if (cudaFuncSetAttribute(tree_attn_kernel<FP8, HD, MI>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<FP8, HD, MI>::SMEM) != cudaSuccess) return 7;
+        if (cudaFuncSetAttribute(tree_attn_kernel<FP8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<FP8, HD>::SMEM) != cudaSuccess) return 7;
         *set = true;
     }
-    return kb_launch_dep(tree_attn_kernel<FP8, HD, MI>, dim3(pl.grid), dim3(THREADS), Cfg<FP8, HD, MI>::SMEM, st, tmK, tmV, p);
+    return kb_launch_dep(tree_attn_kernel<FP8, HD>, dim3(pl.grid), dim3(THREADS), Cfg<FP8, HD>::SMEM, st, p);
 }
 
 }  // namespace
 
 // Floats of workspace that kb_tree_attn wants, 0 where the call is not one for it (the plain form takes it).
-KB_API long long kb_tree_attn_floats(int N, int B, int H, int n_kv, int hd, int max_q, int max_ctx, int num_pages, int fp8) {
+KB_API long long kb_tree_attn_floats(int N, int B, int H, int n_kv, int hd, int max_q, int max_ctx, int fp8) {
     if (N < 1 || B < 1 || B > MAX_B || n_kv < 1 || H < n_kv || H % n_kv || (hd != 64 && hd != 128) || max_q < 1 || max_q > 64 || max_ctx < 1 ||
-        (long long)num_pages * n_kv * PAGE > 0x7fffffffll || (long long)N * H > 0x7fffffffll ||
-        (long long)B * n_kv * ((max_q * (long long)(H / n_kv) + 15) / 16) * ((max_ctx + 63ll) / 64) > 0x7fffffffll / 1024)
+        (long long)N * H > 0x7fffffffll ||
+        (long long)B * n_kv * ((max_q * (long long)(H / n_kv) + 15) / 16) * ((max_ctx + 15ll) / 16) > 0x7fffffffll / 64)
         return 0;
-    const Plan pl = plan_for(B, N, n_kv, H / n_kv, max_q, max_ctx, fp8 != 0);
-    return 2ll * pl.grid * pl.rows * (hd + 2) + B + 4;
+    const Plan pl = plan_for(B, N, n_kv, H / n_kv, hd, max_q, max_ctx, fp8 != 0);
+    return 2ll * pl.workers * pl.rows * (hd + 2) + B + 4;
 }
 
 // As kb_tree_attn_plain for bf16 and heads of 64 and 128; query rows 16-byte, output rows 8-byte aligned; `work` has kb_tree_attn_floats
@@ -748,17 +684,14 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
     if ((ke == nullptr) != (ve == nullptr) || q_stride % 8 || out_stride % 4 || max_pages < 1 || num_pages < 1 || !status ||
         ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)work) % 16 || (uintptr_t)out % 8)
         return 5;
-    const long long need = kb_tree_attn_floats(N, B, H, n_kv, hd, max_q, max_ctx, num_pages, fp8);
+    const long long need = kb_tree_attn_floats(N, B, H, n_kv, hd, max_q, max_ctx, fp8);
     if (need == 0 || work_floats < need) return 5;
-    const Plan pl = plan_for(B, N, n_kv, H / n_kv, max_q, max_ctx, fp8);
-    CUtensorMap tmK, tmV;
-    const long long rows = (long long)num_pages * n_kv * PAGE;
-    int r = page_map(&tmK, k, rows, hd, fp8, pl.rows == 128);
-    if (!r) r = page_map(&tmV, v, rows, hd, fp8, pl.rows == 128);
-    if (r) return r;
+    const Plan pl = plan_for(B, N, n_kv, H / n_kv, hd, max_q, max_ctx, fp8);
     TreeParams p;
     p.q = (const bf16*)q;
     p.q_stride = q_stride;
+    p.k = (const uint8_t*)k;
+    p.v = (const uint8_t*)v;
     p.ke = (const uint8_t*)ke;
     p.ve = (const uint8_t*)ve;
     p.table = table;
@@ -768,8 +701,8 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
     p.out = (bf16*)out;
     p.out_stride = out_stride;
     p.part_o = work;
-    p.part_ml = work + 2ll * pl.grid * pl.rows * hd;
-    p.uoff = reinterpret_cast<int*>(p.part_ml + 2ll * pl.grid * pl.rows * 2);
+    p.part_ml = work + 2ll * pl.workers * pl.rows * hd;
+    p.uoff = reinterpret_cast<int*>(p.part_ml + 2ll * pl.workers * pl.rows * 2);
     p.max_pages = max_pages;
     p.num_pages = num_pages;
     p.B = B;
@@ -781,12 +714,12 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
     p.max_ctx = max_ctx;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.status = status;
-#define TREE(F, D) r = pl.rows == 16 ? launch_tree<F, D, 1>(tmK, tmV, p, pl, st) : launch_tree<F, D, 2>(tmK, tmV, p, pl, st)
-    if (pl.rows == 128) r = launch_tile(tmK, tmV, p, hd, fp8, pl.grid, st);
-    else if (fp8 && hd == 128) TREE(true, 128);
-    else if (fp8) TREE(true, 64);
-    else if (hd == 128) TREE(false, 128);
-    else TREE(false, 64);
-#undef TREE
-    return r ? r : merge(p, hd, pl.rows, pl.tile, pl.grid, pl.wide, zero_tail, st);
+    const int r = pl.rows == 128      ? launch_tile(p, hd, fp8, pl.grid, st)
+                  : fp8 && hd == 128 ? launch_tree<true, 128>(p, pl, st)
+                  : fp8              ? launch_tree<true, 64>(p, pl, st)
+                  : hd == 128        ? launch_tree<false, 128>(p, pl, st)
+                                     : launch_tree<false, 64>(p, pl, st);
+    if (r) return r;
+    if (pl.rows == 128) return hd == 128 ? merge<128, false>(p, pl, zero_tail, st) : merge<64, false>(p, pl, zero_tail, st);
+    return hd == 128 ? merge<128, true>(p, pl, zero_tail, st) : merge<64, true>(p, pl, zero_tail, st);
 }

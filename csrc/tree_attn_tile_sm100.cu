@@ -5,7 +5,7 @@
 //   warps 0-7    softmax: two groups of four, group g has the tiles of parity g; one thread per row
 //   warps 8-11   values: 8-bit pages -> f16 operand tile; places that hold no token -> zero.  Query rows -> shared memory, a unit ahead
 //   warp 12      MMA issue (the whole warp walks the loop, one elected lane issues)
-//   warps 13, 14 TMA of keys and values, a page per lane
+//   warps 13, 14 copies of keys and values, 16 bytes per lane
 //   warp 15      what of a tile exists; 8-bit pages: factors of the keys, unit of the values
 //
 //   S = Q K^T    both operands K-major in shared memory, one accumulator per group
@@ -13,7 +13,7 @@
 //                taken out, is the sum of two e4m3 numbers, hi + lo, which together hold bf16's eight bits (down to 2^-10 of the row's
 //                largest; below that the error is at most 2^-18 of the largest) - two products at twice the rate of one in 16 bits.
 //   softmax      in fp32, a row at a time in one pass: exponentials against the maximum so far, which is renewed only when a
-//                score exceeds it by more than 2^11 (2^40 where P is bf16); P back to tensor memory in 16 bits
+//                score exceeds it by more than 2^11 (2^20 where P is bf16); P back to tensor memory in 16 bits
 //   O += P V     A = P in tensor memory, B = value tile in shared memory (MN-major), one accumulator per group, so that the groups
 //                need nothing from one another before the end of a unit.  8-bit pages: P is f16 in units of 2^-4 (at most 2^15 with the
 //                2^11 of lazy maxima: eleven bits down to 2^-18, off by at most 2^-29 below); the values' f16 carry the token's power
@@ -124,7 +124,7 @@ struct TileMeta {
 
 template <bool FP8, int HD>
 __global__ void __launch_bounds__(THREADS, 1)
-tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeParams p) {
+tree_tile_kernel(const TreeParams p) {
     using L = Lay<FP8, HD>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -148,8 +148,8 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     volatile int* abort_flag = &abort_word;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::KST; ++i) { tc::mbar_init(&k_full[i], 1); tc::mbar_init(&k_empty[i], 1); }
-        for (int i = 0; i < L::RST; ++i) { tc::mbar_init(&r_full[i], 1); tc::mbar_init(&r_empty[i], 5); }
+        for (int i = 0; i < L::KST; ++i) { tc::mbar_init(&k_full[i], 33); tc::mbar_init(&k_empty[i], 1); }
+        for (int i = 0; i < L::RST; ++i) { tc::mbar_init(&r_full[i], 33); tc::mbar_init(&r_empty[i], 5); }
         for (int i = 0; i < L::VST; ++i) { tc::mbar_init(&v_ready[i], 4); tc::mbar_init(&pv_done[i], 1); }
         for (int i = 0; i < SLOTS; ++i) tc::mbar_init(&f_ready[i], 1);
         for (int i = 0; i < 2; ++i) {
@@ -161,20 +161,18 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
         tc::mbar_init(&xch, 8);
         abort_word = 0;
         tc::fence_barrier_init();
-        tc::prefetch_tmap(&tmK);
-        tc::prefetch_tmap(&tmV);
     }
     if (warp == W_MMA) {
         tc::tmem_alloc(&tmem_slot, 512);
         tc::tmem_relinquish();
     }
-    kb_dep_trigger();
     kb_dep_wait();
+    kb_dep_trigger();
     tc::tc_fence_before();
     count_tiles<TT, TT, THREADS>(p, uoff, wsum);       // (has the block's barriers)
     tc::tc_fence_after();
     const uint32_t tmem0 = tmem_slot, tmem_oacc = tmem0 + 256;             // S: two times 128 columns; O: two times HD
-    const int2 part = part_of_line(uoff[p.B]);
+    const int2 part = part_of_line(uoff[p.B], blockIdx.x, gridDim.x);
     const int lo = part.x, n_tiles = part.y - part.x;
     auto segment = [&](int j) { return segment_at<TT, TT>(p, uoff, lo + j, lo + n_tiles); };
     bool ok = true;
@@ -182,11 +180,11 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
     if (n_tiles == 0) {
         // more blocks than tiles
     } else if (warp == W_K || warp == W_V) {
-        // ------------------------------------------------------------ TMA: lane l < 8 brings page l of the tile
+        // ------------------------------------------------------------ copies of keys, of values: 16 bytes per lane
         const bool isv = warp == W_V;
         Segment sg = segment(0);
         int first = 0;                                 // tile at which sg begins
-        int next = -2;                                 // page of the next tile (-2: behind the context)
+        int next = -2;                                 // lane l < 8: page l of the next tile (-2: behind the context)
         auto fetch = [&](int j) {
             if (j >= n_tiles) return;
             if (j - first >= sg.t1 - sg.t0) {
@@ -201,7 +199,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             const int st = isv ? j % L::RST : j % L::KST, use = isv ? j / L::RST : j / L::KST;
             const bool good = next >= 0 && next < p.num_pages;
             if (next != -2 && !good && isv) atomicMax(p.status, (int)KB_BAD_INDEX);
-            const long long cell = (long long)next * p.n_kv + sg.h;
+            const long long mine = ((long long)next * p.n_kv + sg.h) * PAGE;       // first row of this lane's page
             const uint32_t have = __ballot_sync(0xffffffffu, good);
             fetch(j + 1);
             uint64_t* full = isv ? &r_full[st] : &k_full[st];
@@ -211,28 +209,35 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
                 ok = tc::mbar_wait(isv ? &r_empty[st] : &k_empty[st], (uint32_t)(use & 1) ^ 1u, abort_flag);
             }
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            const uint8_t* src = (isv ? p.v : p.k) + lane * 16;
+            const uint32_t dst = smem_u32((isv ? sR : sK) + st * L::KT);
+#pragma unroll 1
+            for (int pg = 0; pg < TT / PAGE; ++pg) {
+                const long long row = __shfl_sync(0xffffffffu, mine, pg);
+                if (!(have >> pg & 1u)) continue;
+                const uint8_t* from = src + row * L::ROW_BYTES;
+                const uint32_t to = dst + pg * PAGE * L::ROWB;
+#pragma unroll
+                for (int i = 0; i < PAGE * L::ROW_BYTES / 512; ++i) {
+                    const int q = i * 32 + lane;       // 16-byte piece of the page: its row, half and swizzled place
+                    const int t = q / (L::ROW_BYTES / 16), c = q % (L::ROW_BYTES / 16), h = c / (L::ROWB / 16), cc = c % (L::ROWB / 16);
+                    copy16(to + h * L::PIECE + t * L::ROWB + ((cc ^ (L::ROWB == 128 ? t & 7 : (t >> 1) & 3)) << 4), from + i * 512);
+                }
+            }
+            if (FP8 && isv && lane < 16) {             // exponents of the keys, then of the values
+                const long long row = __shfl_sync(0xffffu, mine, lane & 7);
+                if (have >> (lane & 7) & 1u)
+                    copy16(smem_u32(exps + st * 2 * TT + (lane >> 3) * TT + (lane & 7) * PAGE), (lane < 8 ? p.ke : p.ve) + row);
+            }
+            copy_arrive(full);
             if (lane == 0) {
                 if (isv) there[st] = have;
                 else there_k[j % SLOTS] = have;
-                tc::mbar_expect_tx(full, __popc(have) * (PAGE * L::ROW_BYTES + (FP8 && isv ? 2 * PAGE : 0)));
-            }
-            __syncwarp();
-            if (good) {
-                uint8_t* dst = (isv ? sR : sK) + st * L::KT + lane * PAGE * L::ROWB;
-#pragma unroll
-                for (int h = 0; h < L::HALVES; ++h) tc::tma_load_3d(dst + h * L::PIECE, isv ? &tmV : &tmK, full, 0, (int)(cell * PAGE), h);
-                if (FP8 && isv) {
-                    uint8_t* e = exps + st * 2 * TT + lane * PAGE;
-                    bulk_16(e, p.ke + cell * PAGE, full);
-                    bulk_16(e + TT, p.ve + cell * PAGE, full);
-                }
+                tc::mbar_arrive(full);
             }
         }
-        if (!ok && lane == 0) {
-            atomicMax(p.status, (int)KB_TIMEOUT_TMA);
-            const uint64_t t0 = global_timer_ns();     // copies in flight land before the block can exit
-            while (global_timer_ns() - t0 < 2000000ull) {}
-        }
+        copy_wait<0>();                                // copies in flight land before the block can exit
+        if (!ok && lane == 0) atomicMax(p.status, (int)KB_TIMEOUT_TMA);
     } else if (warp == W_MMA) {
         // ------------------------------------------------------------ products
         const uint32_t id_s = FP8 ? (1u << 4) | (uint32_t)(TT >> 3) << 17 | (uint32_t)(TT >> 4) << 24 : tc::instr_desc_f16(TT, TT, 1, 1, 0, 0);
@@ -256,6 +261,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             if (s_new && !wait(&q_ready[s_seg & 1], (uint32_t)(s_seg >> 1) & 1u)) return false;
             s_new = false;
             if (!wait(&k_full[st], (uint32_t)(j / L::KST) & 1u)) return false;
+            tc::fence_proxy_async();                   // the keys were copied through the generic proxy
             tc::tc_fence_after();
             const uint32_t b_lo = dk.lo + st * (L::KT >> 4), a_lo = dq.lo + (s_seg & 1) * (L::QT >> 4), d = tmem0 + (j & 1) * 128;
             if (tc::elect_one()) {
@@ -290,6 +296,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             const int vs = j % L::VST;
             ok = wait(&v_ready[vs], (uint32_t)(j / L::VST) & 1u) && wait(&p_ready[j & 1], (uint32_t)(j >> 1) & 1u);
             if (!ok) break;
+            if (!FP8) tc::fence_proxy_async();         // (8-bit pages: the warps that wrote the operand have fenced)
             tc::tc_fence_after();
             // a group's first tile overwrites its O, unless the softmax warps have begun it (values that are not finite)
             const TileMeta& mt = meta[j % SLOTS];
@@ -510,7 +517,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
             return good;
         };
         // log2 units: the maximum is renewed when a score exceeds it by more than GROW; P is in units of 2^-SHIFT.  f16 holds 2^(GROW + SHIFT)
-        constexpr float GROW = FP8 ? 11.f : 40.f, SHIFT = FP8 ? 4.f : 0.f;
+        constexpr float GROW = FP8 ? 11.f : 20.f, SHIFT = FP8 ? 4.f : 0.f;
         int j0 = 0;
         while (j0 < n_tiles && ok) {
             const Segment sg = segment(j0);
@@ -730,7 +737,7 @@ tree_tile_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant_
 }
 
 template <bool FP8, int HD>
-int run_tile(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams& p, int grid, cudaStream_t st) {
+int run_tile(const TreeParams& p, int grid, cudaStream_t st) {
     static bool flags[64] = {};
     bool* set = kb_device_flag(flags);
     if (!set) return 7;
@@ -738,12 +745,12 @@ int run_tile(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams& p
         if (cudaFuncSetAttribute(tree_tile_kernel<FP8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay<FP8, HD>::SMEM) != cudaSuccess) return 7;
         *set = true;
     }
-    return kb_launch_dep(tree_tile_kernel<FP8, HD>, dim3(grid), dim3(THREADS), Lay<FP8, HD>::SMEM, st, tmK, tmV, p);
+    return kb_launch_dep(tree_tile_kernel<FP8, HD>, dim3(grid), dim3(THREADS), Lay<FP8, HD>::SMEM, st, p);
 }
 
 }  // namespace
 
-int tree::launch_tile(const CUtensorMap& tmK, const CUtensorMap& tmV, const TreeParams& p, int hd, bool fp8, int grid, cudaStream_t st) {
-    if (fp8) return hd == 128 ? run_tile<true, 128>(tmK, tmV, p, grid, st) : run_tile<true, 64>(tmK, tmV, p, grid, st);
-    return hd == 128 ? run_tile<false, 128>(tmK, tmV, p, grid, st) : run_tile<false, 64>(tmK, tmV, p, grid, st);
+int tree::launch_tile(const TreeParams& p, int hd, bool fp8, int grid, cudaStream_t st) {
+    if (fp8) return hd == 128 ? run_tile<true, 128>(p, grid, st) : run_tile<true, 64>(p, grid, st);
+    return hd == 128 ? run_tile<false, 128>(p, grid, st) : run_tile<false, 64>(p, grid, st);
 }

@@ -443,11 +443,62 @@ INT4_CASES = [(1, 16, 64, 64, 0), (1, 1, 8, 128, 0), (3, 40, 200, 128, 8), (8, 9
               (33, 64, 64, 128, 0), (64, 48, 768, 64, 0), (65, 100, 1000, 128, 0), (130, 70, 136, 64, 8)]
 
 
-def tile_parts(total, grid):
-    """The line of ``total`` tiles as the tensor-core kernel cuts it (integer arithmetic of the kernel, for a check of its merge)."""
-    parts = min(grid, total)
-    return [(total * c // parts, total * (c + 1) // parts) for c in range(parts)]
+def tile_parts(total, workers):
+    """The line of ``total`` tiles as the tensor-core kernels cut it (integer arithmetic of the kernels)."""
+    parts = min(workers, total)
+    return [(total * c // parts, total * (c + 1) // parts) if c < parts else (0, 0) for c in range(workers)]
 
 
-def part_of(tile, total, grid):
-    return ((tile + 1) * min(grid, total) - 1) // total
+def written_parts(tiles, blocks, per):
+    """What the workers leave for each unit (``tiles``: tiles per unit): slots of partial results, or None where the unit is finished.  A block
+    whose ``per`` > 1 parts lie in one unit leaves one."""
+    total, workers = sum(tiles), blocks * per
+    parts = tile_parts(total, workers)
+    out, s0 = [], 0
+    for t in tiles:
+        slots, finished = [], False
+        for c in range(blocks):
+            mine = parts[c * per:(c + 1) * per]
+            lo, hi = mine[0][0], mine[-1][1]
+            if per > 1 and hi > 0 and lo >= s0 and hi <= s0 + t:
+                if (lo, hi) == (s0, s0 + t):
+                    finished = True
+                else:
+                    slots.append(2 * c * per + (lo == s0))
+                continue
+            for w, (a, b) in enumerate(mine):
+                a, b = max(a, s0), min(b, s0 + t)
+                if a < b:
+                    if (a, b) == (s0, s0 + t):
+                        finished = True
+                    else:
+                        slots.append(2 * (c * per + w) + (a == s0))
+        assert not (finished and slots)
+        out.append(None if finished else slots)
+        s0 += t
+    return out
+
+
+def merged_parts(tiles, blocks, per):
+    """What the merge kernel reads for each unit, in its arithmetic."""
+    total = sum(tiles)
+    parts = min(blocks * per, total)
+    out, s0 = [], 0
+    for t in tiles:
+        first, last = ((s0 + 1) * parts - 1) // total, ((s0 + t) * parts - 1) // total
+        ca, cb = first // per, last // per
+
+        def whole(c):
+            return (c + 1) * per <= parts and total * c * per // parts >= s0 and total * (c + 1) * per // parts <= s0 + t
+
+        wa, wb = whole(ca), whole(cb)
+        if (wa and ca == cb and s0 == total * ca * per // parts and s0 + t == total * (ca + 1) * per // parts) or (first == last and not wa):
+            out.append(None)
+        else:
+            head = 1 if wa else min(last, ca * per + per - 1) - first + 1
+            mid = cb - ca - 1 if cb > ca else 0
+            n = head + mid + ((1 if wb else last - cb * per + 1) if cb > ca else 0)
+            js = [first + k if k < head else (ca + 1 + k - head) * per if k < head + mid else cb * per + k - head - mid for k in range(n)]
+            out.append([2 * j + (j == first) for j in js])
+        s0 += t
+    return out

@@ -67,11 +67,15 @@ def test_operands_that_are_no_pages_or_weights():
             TORCH_OPS.quant_int4(torch.randn(*shape), group)
 
 
-def test_the_cut_of_the_tiles():
-    """Every part has a tile, and the merge finds the part of a tile: all parts between a unit's first and last hold some of it."""
-    for total in list(range(1, 40)) + [295, 296, 297, 1000, 8192]:
-        for grid in (1, 2, 7, 8, 148, 296):
-            parts = cases.tile_parts(total, grid)
-            assert parts[0][0] == 0 and parts[-1][1] == total and all(a < b for a, b in parts) and all(p[1] == q[0] for p, q in zip(parts, parts[1:]))
-            for c, (a, b) in enumerate(parts):
-                assert all(cases.part_of(t, total, grid) == c for t in (a, (a + b) // 2, b - 1))
+@pytest.mark.parametrize("per", [1, 4])
+def test_the_merge_reads_what_the_workers_leave(per):
+    """The line of tiles cut into parts, with units of all sizes against all numbers of blocks: every part has a tile, every unit is either
+    finished or its partial results are exactly the ones that the merge reads."""
+    import random
+    rng = random.Random(per)
+    for _ in range(4000):
+        tiles = [rng.randint(1, rng.choice([2, 9, 60])) for _ in range(rng.randint(1, 7))]
+        blocks = rng.randint(1, 25)
+        parts = [p for p in cases.tile_parts(sum(tiles), blocks * per) if p[1]]
+        assert parts[0][0] == 0 and parts[-1][1] == sum(tiles) and all(a < b for a, b in parts) and all(p[1] == q[0] for p, q in zip(parts, parts[1:]))
+        assert cases.written_parts(tiles, blocks, per) == cases.merged_parts(tiles, blocks, per)
