@@ -63,6 +63,12 @@ struct Cfg {
         if (ROW_BYTES == 128) return (i >> 3) * 128 + (((i & 7) ^ ((i >> 3) & 7)) << 4);
         return ((i >> 3) & 1) * 2048 + (i >> 4) * 128 + (((i & 7) ^ ((i >> 4) & 7)) << 4);
     }
+    // place(32 i + lane) from place(lane)
+    __device__ static __forceinline__ uint32_t place_next(uint32_t at, int i) {
+        if (ROW_BYTES == 64) return at + i * 512;
+        if (ROW_BYTES == 128) return (at ^ ((i & 1) << 6)) + i * 512;
+        return (at ^ ((i & 3) << 5)) + i * 256;
+    }
     static constexpr int RING = WARPS * NST * STAGE;
     static constexpr int EXPS = FP8 ? WARPS * NST * 2 * TILE : 0;      // exponents of a stage: keys, then values
     static constexpr int FACT = FP8 ? WARPS * 2 * TILE * 4 : 0;        // the step's factors as fp32
@@ -115,26 +121,33 @@ tree_attn_kernel(const TreeParams p) {
         if (lane < C::PAGES && tok < ps.ctx) next_page = p.table[(long long)ps.b * p.max_pages + tok / PAGE];
     };
     fetch_page();
+    const uint32_t my_place = C::place(lane);
+    auto copy_page = [&](uint32_t dst, int st, int pg) {
+        const uint32_t cell = (uint32_t)__shfl_sync(0xffffffffu, next_page, pg) * (uint32_t)p.n_kv + (uint32_t)ps.h;
+        const uint8_t *k = p.k + (unsigned long long)cell * C::PAGE_BYTES + lane * 16, *v = p.v + (unsigned long long)cell * C::PAGE_BYTES + lane * 16;
+#pragma unroll
+        for (int i = 0; i < C::PAGE_BYTES / 512; ++i) {
+            const uint32_t at = dst + pg * C::PAGE_BYTES + C::place_next(my_place, i);
+            copy16(at, k + i * 512);
+            copy16(at + C::PAGES * C::PAGE_BYTES, v + i * 512);
+        }
+        if (FP8 && lane < 2) copy16(smem_u32(exps + st * 2 * TILE + lane * TILE + pg * PAGE), (lane ? p.ve : p.ke) + (unsigned long long)cell * PAGE);
+    };
     auto issue = [&]() {                               // loads item px, then looks up the page numbers of the one after it
         if (px < hi) {
             const int st = (px - lo) % C::NST;
-            const bool good = next_page >= 0 && next_page < p.num_pages;
-            if (lane < C::PAGES && next_page != -2 && !good && p.status) atomicMax(p.status, (int)KB_BAD_INDEX);
+            const bool good = (uint32_t)next_page < (uint32_t)p.num_pages;
             const uint32_t have = __ballot_sync(0xffffffffu, lane < C::PAGES && good);
             if (lane == 0) there[warp][st] = have;
-            const uint32_t dst = smem_u32(ring + (size_t)st * C::STAGE);
+            const uint32_t dst = smem_u32(ring + st * C::STAGE);
+            if (have == (1u << C::PAGES) - 1u) {
 #pragma unroll
-            for (int pg = 0; pg < C::PAGES; ++pg) {
-                if (!(have >> pg & 1u)) continue;
-                const long long cell = (long long)__shfl_sync(0xffffffffu, next_page, pg) * p.n_kv + ps.h;
-                const uint8_t *k = p.k + cell * C::PAGE_BYTES + lane * 16, *v = p.v + cell * C::PAGE_BYTES + lane * 16;
-#pragma unroll
-                for (int i = 0; i < C::PAGE_BYTES / 512; ++i) {
-                    const uint32_t at = dst + pg * C::PAGE_BYTES + C::place(i * 32 + lane);
-                    copy16(at, k + i * 512);
-                    copy16(at + C::PAGES * C::PAGE_BYTES, v + i * 512);
-                }
-                if (FP8 && lane < 2) copy16(smem_u32(exps + st * 2 * TILE + lane * TILE + pg * PAGE), (lane ? p.ve : p.ke) + cell * PAGE);
+                for (int pg = 0; pg < C::PAGES; ++pg) copy_page(dst, st, pg);
+            } else {
+                if (lane < C::PAGES && next_page != -2 && !good && p.status) atomicMax(p.status, (int)KB_BAD_INDEX);
+#pragma unroll 1
+                for (int pg = 0; pg < C::PAGES; ++pg)
+                    if (have >> pg & 1u) copy_page(dst, st, pg);
             }
             ++px;
             fetch_page();
@@ -249,13 +262,12 @@ tree_attn_kernel(const TreeParams p) {
                         }
                 }
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    float2 f = make_float2(1.f, 1.f);
-                    if constexpr (FP8) f = *reinterpret_cast<const float2*>(fk + 8 * j + 2 * qd);
-                    s[j][0] *= f.x * rs[0];
-                    s[j][1] *= f.y * rs[0];
-                    s[j][2] *= f.x * rs[1];
-                    s[j][3] *= f.y * rs[1];
+                for (int j = 0; j < NT && FP8; ++j) {
+                    const float2 f = *reinterpret_cast<const float2*>(fk + 8 * j + 2 * qd);
+                    s[j][0] *= f.x;
+                    s[j][1] *= f.y;
+                    s[j][2] *= f.x;
+                    s[j][3] *= f.y;
                 }
                 // ---- what is not seen: places that hold no token, and drafted tokens the row's mask does not name
                 uint32_t odd = 0;                      // drafted tokens whose values are not finite: kept out of the product
@@ -295,6 +307,7 @@ tree_attn_kernel(const TreeParams p) {
                     mx[hf] = fmaxf(s[0][2 * hf], s[0][2 * hf + 1]);
 #pragma unroll
                     for (int j = 1; j < NT; ++j) mx[hf] = fmaxf(mx[hf], fmaxf(s[j][2 * hf], s[j][2 * hf + 1]));
+                    mx[hf] *= rs[hf];                  // (rs is positive)
                 }
                 if (__any_sync(0xffffffffu, mx[0] > m[0] + GROW || mx[1] > m[1] + GROW || (FP8 && grow != 1.f))) {
                     float f[2];
@@ -322,7 +335,7 @@ tree_attn_kernel(const TreeParams p) {
                     const float at = m[hf] == -INFINITY ? 0.f : m[hf];
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        float a = exp2f(s[j][2 * hf] - at), z = exp2f(s[j][2 * hf + 1] - at);
+                        float a = exp2f(fmaf(s[j][2 * hf], rs[hf], -at)), z = exp2f(fmaf(s[j][2 * hf + 1], rs[hf], -at));
                         l[hf] += a + z;
                         if constexpr (FP8) {
                             const float2 w = *reinterpret_cast<const float2*>(fk + TILE + 8 * j + 2 * qd);
@@ -338,19 +351,19 @@ tree_attn_kernel(const TreeParams p) {
                     // Values that must not enter the product: what the cache holds in places without a token, and drafted tokens that
                     // are not finite - those are added row by row (never in normal use)
                     uint8_t* pages = ring + (size_t)st * C::STAGE + C::PAGES * C::PAGE_BYTES;
+                    volatile float kept[NT][4];        // (indexed by the token: in local memory, here only)
+                    if (odd)
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) kept[j][e] = s[j][e];
 #pragma unroll 1
                     for (uint32_t left = odd; left; left &= left - 1u) {
                         const int tk = __ffs(left) - 1, src = (lane & ~3) | ((tk & 7) >> 1), tr = tk % PAGE;
                         const uint8_t* page = pages + (tk / PAGE) * C::PAGE_BYTES;
                         float pv[2];
 #pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            float mine = 0.f;
-#pragma unroll
-                            for (int j = 0; j < NT; ++j)
-                                if (j == tk >> 3) mine = tk & 1 ? s[j][2 * hf + 1] : s[j][2 * hf];
-                            pv[hf] = __shfl_sync(0xffffffffu, mine, src);
-                        }
+                        for (int hf = 0; hf < 2; ++hf) pv[hf] = __shfl_sync(0xffffffffu, kept[tk >> 3][2 * hf + (tk & 1)], src);
 #pragma unroll
                         for (int j = 0; j < HD / 8; ++j)
 #pragma unroll
@@ -681,7 +694,7 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
                         int H, int n_kv, int hd, int max_q, int max_ctx, float scale, int zero_tail, float* work, long long work_floats, int* status,
                         cudaStream_t st) {
     const bool fp8 = ke != nullptr;
-    if ((ke == nullptr) != (ve == nullptr) || q_stride % 8 || out_stride % 4 || max_pages < 1 || num_pages < 1 || !status ||
+    if ((ke == nullptr) != (ve == nullptr) || !(scale > 0.f) || (long long)num_pages * n_kv > 0x7fffffffll || q_stride % 8 || out_stride % 4 || max_pages < 1 || num_pages < 1 || !status ||
         ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)work) % 16 || (uintptr_t)out % 8)
         return 5;
     const long long need = kb_tree_attn_floats(N, B, H, n_kv, hd, max_q, max_ctx, fp8);

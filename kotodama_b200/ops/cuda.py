@@ -1052,7 +1052,7 @@ class CudaOps(TorchOps):
         if N == 0 or B == 0 or page_table.shape[1] == 0:
             return res if given else res.zero_()
         floats = 0
-        if q.dtype == torch.bfloat16 and q.stride(0) % 8 == 0 and res.stride(0) % 4 == 0 and q.data_ptr() % 16 == 0 and res.data_ptr() % 8 == 0:
+        if q.dtype == torch.bfloat16 and scale > 0 and q.stride(0) % 8 == 0 and res.stride(0) % 4 == 0 and q.data_ptr() % 16 == 0 and res.data_ptr() % 8 == 0:
             floats = self._tree_floats(N, B, H, kt.shape[1], hd, max_q, max_ctx, int(fp8))
         if floats:
             work = torch.empty(floats, device=dev, dtype=torch.float32)
