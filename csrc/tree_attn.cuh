@@ -35,6 +35,31 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
+__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) { return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3); }
+__device__ __forceinline__ uint32_t largest(uint32_t two_bf16) { return max(two_bf16 & 0x7fffu, (two_bf16 >> 16) & 0x7fffu); }
+// Four bf16 numbers times `inv` as the sum of two e4m3 numbers each: together they hold the eight bits of a bf16 number (numbers within 2^-10
+// of the type's upper end; below, they are off by at most 2^-10).
+__device__ __forceinline__ void split_e4m3(uint2 q, float inv, uint32_t& hi, uint32_t& lo) {
+    uint32_t h[2], l[2];
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+        const uint32_t w = z ? q.y : q.x;
+        const float a = __uint_as_float(w << 16) * inv, b = __uint_as_float(w & 0xffff0000u) * inv;
+        h[z] = e4m3x2(a, b);
+        const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h[z], __NV_E4M3)));
+        l[z] = e4m3x2(a - back.x, b - back.y);
+    }
+    hi = h[0] | h[1] << 16;
+    lo = l[0] | l[1] << 16;
+}
+// The power of two that brings a row's largest number to [2^7, 2^8), from the largest magnitude's bits, and its inverse; NaN where the row is not finite.
+__device__ __forceinline__ float q_down(uint32_t big) {
+    return big >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)min(254 - (int)(big >> 7) + 7, 254) << 23);
+}
+__device__ __forceinline__ float q_up(uint32_t big) {
+    const int b = 254 - min(254 - (int)(big >> 7) + 7, 254);
+    return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 0x00400000u);
+}
 // four e4m3 codes -> two f16 pairs
 __device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t& hi) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(c));

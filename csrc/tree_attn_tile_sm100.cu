@@ -32,6 +32,7 @@ using namespace tree;
 
 constexpr int TT = 128, THREADS = 512;
 constexpr int W_VAL = 8, W_MMA = 12, W_K = 13, W_V = 14, W_META = 15;
+constexpr int SEGS = 16;                               // segments that the key warp may be ahead (it is less than eight tiles ahead)
 constexpr int SLOTS = 8;                               // tiles that the notes on tiles reach ahead of the softmax, and more
 constexpr int HALF = TT * 128;                         // 128 tokens x 128 bytes: 16 KB
 
@@ -74,9 +75,6 @@ __device__ __forceinline__ bool passed(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
-    return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
@@ -84,7 +82,6 @@ __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ float2 f16x2_to_float(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
 
-__device__ __forceinline__ uint32_t largest(uint32_t two) { return max(two & 0x7fffu, (two >> 16) & 0x7fffu); }
 
 // Columns of tensor memory (a row per lane) times f: fp32 accumulators, packed probabilities.
 __device__ __noinline__ void scale_columns(uint32_t addr, int n, float f) {
@@ -144,6 +141,9 @@ tree_tile_kernel(const TreeParams p) {
     __shared__ TileMeta meta[SLOTS];                   // of tile j at j % SLOTS
     __shared__ uint32_t tmem_slot;
     __shared__ int unit_E[2];
+    __shared__ Segment segs[SEGS];
+    __shared__ float q_scale[FP8 ? 2 * TT : 1];        // the power of two taken out of a query row
+    __shared__ uint64_t seg_ready[SEGS];
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -158,6 +158,7 @@ tree_tile_kernel(const TreeParams p) {
             tc::mbar_init(&q_ready[i], 4);
             tc::mbar_init(&slow[i], 4);
         }
+        for (int i = 0; i < SEGS; ++i) tc::mbar_init(&seg_ready[i], 1);
         tc::mbar_init(&xch, 8);
         abort_word = 0;
         tc::fence_barrier_init();
@@ -174,22 +175,47 @@ tree_tile_kernel(const TreeParams p) {
     const uint32_t tmem0 = tmem_slot, tmem_oacc = tmem0 + 256;             // S: two times 128 columns; O: two times HD
     const int2 part = part_of_line(uoff[p.B], blockIdx.x, gridDim.x);
     const int lo = part.x, n_tiles = part.y - part.x;
-    auto segment = [&](int j) { return segment_at<TT, TT>(p, uoff, lo + j, lo + n_tiles); };
     bool ok = true;
+    // The s-th segment of this part: found by the key warp, which is ahead of all others and a segment ahead of itself.
+    auto segment = [&](int s) {
+        Segment g;
+        if (!tc::mbar_wait(&seg_ready[s % SEGS], (uint32_t)(s / SEGS) & 1u, abort_flag)) {
+            ok = false;
+            g.b = g.h = g.rb = g.t0 = 0;
+            g.n = g.ctx = g.T = g.t1 = 1;
+            return g;
+        }
+        return segs[s % SEGS];
+    };
 
     if (n_tiles == 0) {
         // more blocks than tiles
     } else if (warp == W_K || warp == W_V) {
         // ------------------------------------------------------------ copies of keys, of values: 16 bytes per lane
         const bool isv = warp == W_V;
+        // The key warp finds the segments, one ahead of the one that it works on (queries are fetched that early).
+        int pub = 0, pub_at = 0;                       // segments published; tile at which the next one begins
+        auto publish = [&]() {
+            if (pub_at >= n_tiles) return;
+            const Segment g = segment_at<TT, TT>(p, uoff, lo + pub_at, lo + n_tiles);
+            if (lane == 0) {
+                segs[pub % SEGS] = g;
+                tc::mbar_arrive(&seg_ready[pub % SEGS]);
+            }
+            pub_at += g.t1 - g.t0;
+            ++pub;
+        };
+        if (!isv) publish();
         Segment sg = segment(0);
-        int first = 0;                                 // tile at which sg begins
+        if (!isv) publish();
+        int first = 0, seg = 0;                        // tile at which sg begins, its number
         int next = -2;                                 // lane l < 8: page l of the next tile (-2: behind the context)
         auto fetch = [&](int j) {
             if (j >= n_tiles) return;
             if (j - first >= sg.t1 - sg.t0) {
-                sg = segment(j);
+                sg = segment(++seg);
                 first = j;
+                if (!isv) publish();
             }
             const int tok = (sg.t0 + j - first) * TT + lane * PAGE;
             next = lane < 8 && tok < sg.ctx ? p.table[(long long)sg.b * p.max_pages + tok / PAGE] : -2;
@@ -202,6 +228,7 @@ tree_tile_kernel(const TreeParams p) {
             const long long mine = ((long long)next * p.n_kv + sg.h) * PAGE;       // first row of this lane's page
             const uint32_t have = __ballot_sync(0xffffffffu, good);
             fetch(j + 1);
+            if (!ok) break;
             uint64_t* full = isv ? &r_full[st] : &k_full[st];
             if (isv && !FP8) {                         // the stage is the operand tile: free when its product has run
                 if (use > 0) ok = tc::mbar_wait(&pv_done[st], (uint32_t)(use - 1) & 1u, abort_flag);
@@ -246,14 +273,15 @@ tree_tile_kernel(const TreeParams p) {
         if (L::ROWB == 64) dq.hi = dk.hi = (dk.hi & ~(7u << 29)) | 4u << 29;       // rows of 64 bytes: 64-byte swizzle
         const tc::DescHalves dv = tc::smem_desc_halves(smem_u32(sV), HALF, 1024);
         Segment sg = segment(0);
-        int s_left = sg.t1 - sg.t0, s_seg = 0;         // tiles of the segment that S is at; its number
+        const int len0 = sg.t1 - sg.t0;
+        int s_left = len0, s_seg = 0;                  // tiles of the segment that S is at; its number
         bool s_new = true;                             // its queries have not been waited for
         auto wait = [&](uint64_t* bar, uint32_t parity) { return passed(bar, parity) || tc::mbar_wait(bar, parity, abort_flag); };
         auto scores = [&](int j) {                     // S(j): waits for its queries and keys
             if (s_left == 0) {
-                sg = segment(j);
+                sg = segment(++s_seg);
+                if (!ok) return false;
                 s_left = sg.t1 - sg.t0;
-                ++s_seg;
                 s_new = true;
             }
             --s_left;
@@ -284,12 +312,12 @@ tree_tile_kernel(const TreeParams p) {
             __syncwarp();
             return true;
         };
-        Segment og = sg;
-        int o_at = 0, o_len = og.t1 - og.t0;           // tile of the segment that O is at
-        ok = scores(0) && (n_tiles < 2 || scores(1));
+        int o_at = 0, o_len = len0, o_seg = 0;         // tile of the segment that O is at; its number
+        ok = ok && scores(0) && (n_tiles < 2 || scores(1));
         for (int j = 0; j < n_tiles && ok; ++j) {
             if (o_at == o_len) {
-                og = segment(j);
+                const Segment og = segment(++o_seg);
+                if (!ok) break;
                 o_len = og.t1 - og.t0;
                 o_at = 0;
             }
@@ -315,13 +343,14 @@ tree_tile_kernel(const TreeParams p) {
     } else if (warp == W_META) {
         // ------------------------------------------------------------ what of a tile exists, which drafted tokens are odd, factors
         Segment sg = segment(0);
-        int first = 0;                                 // tile at which sg begins
+        int first = 0, seg = 0;                        // tile at which sg begins, its number
         uint32_t E = 0;
         for (int j = 0; j < n_tiles; ++j) {
             if (j - first == sg.t1 - sg.t0) {
-                sg = segment(j);
+                sg = segment(++seg);
                 first = j;
             }
+            if (!ok) break;
             const int rst = j % L::RST;
             // (slot j % SLOTS is free: the load of tile j waited for the conversion, and with it the product, of tiles less than SLOTS back)
             ok = tc::mbar_wait(&r_full[rst], (uint32_t)(j / L::RST) & 1u, abort_flag);
@@ -390,31 +419,18 @@ tree_tile_kernel(const TreeParams p) {
                 uint32_t big = 0;
 #pragma unroll
                 for (int i = 0; i < HD / 8; ++i) big = max(big, max(max(largest(v[i].x), largest(v[i].y)), max(largest(v[i].z), largest(v[i].w))));
-                // the largest number comes to [2^7, 2^8); a row that is not finite becomes NaN
-                const float inv = big >= 0x7f80u ? __uint_as_float(0x7fc00000u) : pow2_biased(min(254 - (int)(big >> 7) + 7, 254));
+                const float inv = q_down(big);
 #pragma unroll
                 for (int c = 0; c < HD / 16; ++c) {    // sixteen numbers: a chunk of hi, a chunk of lo
-                    uint32_t hi4[4], lo4[4];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t w[4] = {v[2 * c + i].x, v[2 * c + i].y, v[2 * c + i].z, v[2 * c + i].w};
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            uint32_t h2[2], l2[2];
-#pragma unroll
-                            for (int z = 0; z < 2; ++z) {
-                                const float a = __uint_as_float(w[2 * e + z] << 16) * inv, b = __uint_as_float(w[2 * e + z] & 0xffff0000u) * inv;
-                                h2[z] = e4m3x2(a, b);
-                                const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h2[z], __NV_E4M3)));
-                                l2[z] = e4m3x2(a - back.x, b - back.y);
-                            }
-                            hi4[2 * i + e] = h2[0] | h2[1] << 16;
-                            lo4[2 * i + e] = l2[0] | l2[1] << 16;
-                        }
-                    }
-                    *reinterpret_cast<uint4*>(dst + ((c ^ sw) << 4)) = make_uint4(hi4[0], hi4[1], hi4[2], hi4[3]);
-                    *reinterpret_cast<uint4*>(dst + L::KT + ((c ^ sw) << 4)) = make_uint4(lo4[0], lo4[1], lo4[2], lo4[3]);
+                    uint4 h4, l4;
+                    split_e4m3(make_uint2(v[2 * c].x, v[2 * c].y), inv, h4.x, l4.x);
+                    split_e4m3(make_uint2(v[2 * c].z, v[2 * c].w), inv, h4.y, l4.y);
+                    split_e4m3(make_uint2(v[2 * c + 1].x, v[2 * c + 1].y), inv, h4.z, l4.z);
+                    split_e4m3(make_uint2(v[2 * c + 1].z, v[2 * c + 1].w), inv, h4.w, l4.w);
+                    *reinterpret_cast<uint4*>(dst + ((c ^ sw) << 4)) = h4;
+                    *reinterpret_cast<uint4*>(dst + L::KT + ((c ^ sw) << 4)) = l4;
                 }
+                q_scale[(seg & 1) * TT + t] = q_up(big);
             } else {
 #pragma unroll
                 for (int c = 0; c < HD / 8; ++c) *reinterpret_cast<uint4*>(dst + (c >> 3) * HALF + (((c & 7) ^ sw) << 4)) = v[c];
@@ -428,10 +444,10 @@ tree_tile_kernel(const TreeParams p) {
         for (int j = 0; j < n_tiles; ++j, ++at) {
             const int vs = j % L::VST, rst = j % L::RST;
             if (at == sg.t1 - sg.t0) {
-                sg = segment(j);
+                sg = segment(++seg);
                 at = 0;
-                ++seg;
             }
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             // queries of this unit, or of the next one once the products of the unit before this one (the buffer's last reader) have run
             const bool ahead = at == 1 && loaded == seg + 1 && j - at + (sg.t1 - sg.t0) < n_tiles;
             if (loaded <= seg || ahead) {
@@ -441,7 +457,7 @@ tree_tile_kernel(const TreeParams p) {
                     load_queries(sg, seg);
                     loaded = seg + 1;
                 } else {
-                    load_queries(segment(j - at + (sg.t1 - sg.t0)), seg + 1);
+                    load_queries(segment(seg + 1), seg + 1);
                     loaded = seg + 2;
                 }
             }
@@ -519,23 +535,16 @@ tree_tile_kernel(const TreeParams p) {
         // log2 units: the maximum is renewed when a score exceeds it by more than GROW; P is in units of 2^-SHIFT.  f16 holds 2^(GROW + SHIFT)
         constexpr float GROW = FP8 ? 11.f : 20.f, SHIFT = FP8 ? 4.f : 0.f;
         int j0 = 0;
-        while (j0 < n_tiles && ok) {
-            const Segment sg = segment(j0);
+        for (int seg = 0; j0 < n_tiles && ok; ++seg) {
+            const Segment sg = segment(seg);
+            if (!ok) break;
             const int len = sg.t1 - sg.t0, M = sg.n * p.G, R = sg.rb * TT + r, c0 = p.cu ? p.cu[sg.b] : sg.b, prefix = sg.ctx - sg.n;
             const bool live = sg.rb * TT + (warp & 3) * 32 < M;            // the warp has rows
             const int row_i = min(R, M - 1) / p.G, row_g = min(R, M - 1) % p.G;
             float scale = p.scale_log2;
-            if constexpr (FP8) {                       // the power of two that load_queries took out of this row
-                if (live) {
-                    const bf16* src = p.q + (long long)(c0 + row_i) * p.q_stride + (long long)(sg.h * p.G + row_g) * HD;
-                    uint32_t big = 0;
-#pragma unroll
-                    for (int i = 0; i < HD / 8; ++i) {
-                        const uint4 v = *reinterpret_cast<const uint4*>(src + i * 8);
-                        big = max(big, max(max(largest(v.x), largest(v.y)), max(largest(v.z), largest(v.w))));
-                    }
-                    scale *= pow2_biased(254 - min(254 - (int)(big >> 7) + 7, 254));       // 1 / inv of load_queries
-                }
+            if constexpr (FP8) {
+                if (!tc::mbar_wait(&q_ready[seg & 1], (uint32_t)(seg >> 1) & 1u, abort_flag)) { ok = false; break; }
+                scale *= q_scale[(seg & 1) * TT + r];
             }
             float m_used = -INFINITY, l = 0.f;
             int E = 0;
