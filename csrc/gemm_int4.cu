@@ -13,13 +13,13 @@
 // all SMs loading; a warp has four blocks of 512 bytes per row tile in flight while it works on the four before.
 #include <stddef.h>
 
-#include "common.cuh"
+#include "codes4.cuh"
 
 typedef __nv_bfloat16 bf16;
 
 namespace {
 
-constexpr int KB = 64;                                 // inputs of a block
+using namespace codes4;
 
 __device__ __forceinline__ void mma_bf16(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -31,20 +31,6 @@ __device__ __forceinline__ void mma_bf16_first(float* d, const uint32_t* a, uint
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
         : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
-}
-
-// One word (eight codes) -> the A fragment of one k step: pairs (row r, inputs 0 1), (r + 8, 0 1), (r, 2 3), (r + 8, 2 3).  Masked alone, a
-// nibble in the low byte of a half word is a subnormal bf16 number: code * 2^-133 (bits 0 - 3) or code * 2^-129 (bits 4 - 7, of which the top one
-// is the exponent's lowest: it counts the same).  Times 2^127 less 8 units that is (code - 8) / 64 for row r and (code - 8) / 4 for row r + 8, exactly.
-constexpr float UNIT0 = 64.f, UNIT1 = 4.f;
-__device__ __forceinline__ void expand(uint32_t w, uint32_t* a) {
-    const __nv_bfloat162 up = __float2bfloat162_rn(1.70141183460469231732e38f), o0 = __float2bfloat162_rn(-0.125f), o1 = __float2bfloat162_rn(-2.f);
-    const uint32_t z = w >> 8, v[4] = {w & 0x000f000fu, w & 0x00f000f0u, z & 0x000f000fu, z & 0x00f000f0u};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const __nv_bfloat162 d = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&v[i]), up, i & 1 ? o1 : o0);
-        a[i] = *reinterpret_cast<const uint32_t*>(&d);
-    }
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -61,11 +47,6 @@ __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_gr
 template <int N>
 __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-struct Int4Shape {
-    int M, N, K, nt, kb, ng;                           // row tiles, blocks of 64 inputs, groups
-    long long x_stride, y_stride, c_stride;
-};
-
 // TT tiles of eight tokens, RT tiles of 16 rows at once, PG blocks of 64 inputs per group, W warps, D stages of a warp's ring.
 template <int TT, int RT, int W, int D>
 struct Int4Smem {
@@ -81,7 +62,7 @@ struct Int4Smem {
 template <int TT, int RT, int PG, int W, int D>
 __global__ void __launch_bounds__(W * 32, 1)
 int4_kernel(const bf16* __restrict__ x, const uint4* __restrict__ packed, const uint32_t* __restrict__ scales, const bf16* c, bf16* y,
-            const Int4Shape s) {
+            const Shape s) {
     extern __shared__ __align__(16) unsigned char raw[];
     typedef Int4Smem<TT, RT, W, D> Smem;
     typedef typename Smem::Stage Stage;
@@ -255,7 +236,7 @@ int4_kernel(const bf16* __restrict__ x, const uint4* __restrict__ packed, const 
 }
 
 template <int TT, int RT, int PG, int W, int D>
-int run_int4(const bf16* x, const uint4* packed, const uint32_t* scales, const bf16* c, bf16* y, const Int4Shape& s, int ctas, cudaStream_t st) {
+int run_int4(const bf16* x, const uint4* packed, const uint32_t* scales, const bf16* c, bf16* y, const Shape& s, int ctas, cudaStream_t st) {
     const int chunks = (s.M + TT * 8 - 1) / (TT * 8);
     if (chunks > 65535) return 5;
     auto kernel = int4_kernel<TT, RT, PG, W, D>;
@@ -273,11 +254,11 @@ int run_int4(const bf16* x, const uint4* packed, const uint32_t* scales, const b
 
 // x: [M, K] bf16 in rows x_stride apart (16-byte aligned rows), packed / scales as Int4Weight lays them out, c (may be null, may be y): [M, N].
 KB_API int kb_gemm_int4(const void* x, long long x_stride, const void* packed, const void* scales, const void* c, long long c_stride, void* y,
-                        long long y_stride, int M, int N, int K, int group, cudaStream_t st) {
+                        long long y_stride, int M, int N, int K, int group, int* status, cudaStream_t st) {
     if (M < 1 || N < 1 || K < 8 || K % 8 || (group != 64 && group != 128) || x_stride % 8 || ((uintptr_t)x | (uintptr_t)packed) % 16 ||
         (uintptr_t)scales % 4)
         return 5;
-    const Int4Shape s{M, N, K, (N + 15) / 16, (K + KB - 1) / KB, (K + group - 1) / group, x_stride, y_stride, c_stride};
+    const Shape s{M, N, K, (N + 15) / 16, (K + KB - 1) / KB, (K + group - 1) / group, x_stride, y_stride, c_stride};
 #define INT4_RUN(TT, RT, W, D)                                                                                                                \
     return group == 64 ? run_int4<TT, RT, 1, W, D>((const bf16*)x, (const uint4*)packed, (const uint32_t*)scales, (const bf16*)c, (bf16*)y, s, sms, st) \
                        : run_int4<TT, RT, 2, W, D>((const bf16*)x, (const uint4*)packed, (const uint32_t*)scales, (const bf16*)c, (bf16*)y, s, sms, st)
@@ -291,11 +272,11 @@ KB_API int kb_gemm_int4(const void* x, long long x_stride, const void* packed, c
         if (per == 3 || per == 5 || per == 6) INT4_RUN(1, 3, 16, 3);
         INT4_RUN(1, 4, 16, 3);
     }
-    if (M <= 16) {
+    if (M <= 16 || x_stride < K) {                     // (the other kernel's copies take rows that do not overlap)
         if (per <= 2) INT4_RUN(2, 2, 16, 3);
         if (per == 3 || per == 5 || per == 6) INT4_RUN(2, 3, 12, 3);
         INT4_RUN(2, 4, 8, 3);
     }
-    INT4_RUN(4, 2, 8, 3);
 #undef INT4_RUN
+    return launch_tile((const bf16*)x, (const uint4*)packed, (const bf16*)scales, (const bf16*)c, (bf16*)y, s, group, sms, status, st);
 }

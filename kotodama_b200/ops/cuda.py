@@ -35,7 +35,7 @@ _ARGS = {
     "kb_kv_gather_fp8": "pppp" + "ii" + "piii" + "pppi" + "ppii" + "p",
     "kb_tree_attn_plain": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fii" + "p",
     "kb_tree_attn": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fi" + "pl" + "p",
-    "kb_gemm_int4": "pl" + "pp" + "pl" + "pl" + "iiii",
+    "kb_gemm_int4": "pl" + "pp" + "pl" + "pl" + "iiii" + "p",
 }
 
 
@@ -339,7 +339,7 @@ class CudaOps(TorchOps):
             with self._on(a):
                 self._launch("kb_gemm_int4", a.data_ptr(), a.stride(0), b.packed.data_ptr(), b.scales.data_ptr(),
                              c.data_ptr() if c is not None else None, c.stride(0) if c is not None and c.shape[0] > 1 else 0, out.data_ptr(),
-                             out.stride(0), M, N, K, b.group)
+                             out.stride(0), M, N, K, b.group, self.status(a.device).data_ptr())
         return out
 
     def gemm_nt(self, a, b, out=None, residual=None, accumulate=False):
