@@ -25,7 +25,7 @@ namespace {
 
 using namespace codes4;
 
-constexpr int ROWS = 128, TURNS = 4, SCALES = 8;       // rows of a CTA, turns of widened weights, groups of a flush thread's ring of scales
+constexpr int ROWS = 128, TURNS = 4, SCALES = 8;       // rows of a CTA, turns of operands (weights and tokens), groups of a flush thread's ring of scales
 constexpr int D = 4;                                   // turns of a widening warp's ring
 constexpr int PITCH = ROWS + 4;                        // floats of a token's sums
 
@@ -67,11 +67,10 @@ __device__ __forceinline__ void cluster_sync() {
 
 template <int TN, int PG>
 struct Roles {
-    static constexpr int AC = TN > 64 ? 64 : TN;       // columns of a flush thread
+    static constexpr int AC = TN > 64 ? 64 : 32;       // columns of a flush thread
     static constexpr int FLUSH = 4 * (TN / AC), WIDEN = 8, W_WIDEN = FLUSH, W_X = FLUSH + WIDEN, W_MMA = W_X + 1, THREADS = 32 * (W_MMA + 1);
     static constexpr int BLOCK = TN * 128;             // a block of 64 inputs of the tokens
-    static constexpr int SB = TN > 64 ? 4 : 6;         // turns of tokens
-    static constexpr int RING = SB * 2 * BLOCK, CODES = WIDEN * D * 2 * 512, SC = FLUSH * 32 * SCALES * 4;
+    static constexpr int RING = TURNS * 2 * BLOCK, CODES = WIDEN * D * 2 * 512, SC = FLUSH * 32 * SCALES * 4;
     static constexpr int SMEM = 1024 + RING + CODES + SC;
     static constexpr int SETS = 2, SET = TN * (2 / PG);                // accumulators: sets, columns of a set (the groups of a turn)
     static_assert(TN * PITCH * 4 <= RING, "the partial sums take the ring's place");
@@ -84,7 +83,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
     using R = Roles<TN, PG>;
     extern __shared__ uint8_t raw[];
     uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    __shared__ uint64_t a_full[TURNS], a_empty[TURNS], b_full[R::SB], b_empty[R::SB], acc_full[R::SETS], acc_empty[R::SETS];
+    __shared__ uint64_t full[TURNS], empty[TURNS], acc_full[R::SETS], acc_empty[R::SETS];
     __shared__ uint32_t tmem_slot;
     __shared__ int abort_word;
     volatile int* abort_flag = &abort_word;
@@ -95,12 +94,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
     const int b0 = 2 * t0, nb = min(2 * turns, s.kb - b0);
     if (threadIdx.x == 0) {
         for (int i = 0; i < TURNS; ++i) {
-            tc::mbar_init(&a_full[i], R::WIDEN);
-            tc::mbar_init(&a_empty[i], 1);
-        }
-        for (int i = 0; i < R::SB; ++i) {
-            tc::mbar_init(&b_full[i], 1);
-            tc::mbar_init(&b_empty[i], 1);
+            tc::mbar_init(&full[i], R::WIDEN + 1);     // (and the bytes of the tokens)
+            tc::mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < R::SETS; ++i) {
             tc::mbar_init(&acc_full[i], 1);
@@ -126,7 +121,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
         const bool live = tile < s.nt;
         const float unit = row & 8 ? UNIT1 : UNIT0;
         const uint32_t src = tmem_acc + ((uint32_t)((warp & 3) * 32) << 16) + col0;
-        constexpr int G = 2 / PG;                      // groups of a turn
+        constexpr int G = 2 / PG, PIECE = R::AC > 32 ? 16 : 32;        // groups of a turn; columns of a load
         const int n_groups = PG == 2 ? turns : nb;
         // scales: the word of rows r and r + 8, a ring of this thread's own
         const bf16* sc = scales + ((long long)tile * s.ng + (PG == 2 ? t0 : b0)) * 16 + (row & 7) * 2;
@@ -158,12 +153,13 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
                 const float f1 = __uint_as_float(row & 8 ? both & 0xffff0000u : both << 16) * unit;
                 const float2 f2 = make_float2(f1, f1);
 #pragma unroll
-                for (int e0 = 0; e0 < R::AC; e0 += 16) {
-                    uint32_t v[16];
-                    tc::tmem_ld16(src + set * R::SET + h * TN + e0, v);
+                for (int e0 = 0; e0 < R::AC; e0 += PIECE) {
+                    uint32_t v[PIECE];
+                    if constexpr (PIECE == 32) tc::tmem_ld32(src + set * R::SET + h * TN + e0, v);
+                    else tc::tmem_ld16(src + set * R::SET + h * TN + e0, v);
                     tc::tmem_ld_wait();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
+                    for (int e = 0; e < PIECE / 2; ++e)
                         acc[e0 / 2 + e] = __ffma2_rn(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), f2, acc[e0 / 2 + e]);
                 }
             }
@@ -229,7 +225,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
                     a[u][4 * k + 2] = e[1];
                     a[u][4 * k + 3] = e[3];
                 }
-            ok = tc::mbar_wait(&a_empty[st], ((uint32_t)(i / TURNS) & 1u) ^ 1u, abort_flag);
+            ok = tc::mbar_wait(&empty[st], ((uint32_t)(i / TURNS) & 1u) ^ 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::tc_fence_after();
             const uint32_t dst = tmem_a + st * 64 + ((uint32_t)(first * 16) << 16);
@@ -238,7 +234,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
             tc::tmem_st_wait();
             tc::tc_fence_before();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&a_full[st]);
+            if (lane == 0) tc::mbar_arrive(&full[st]);
         }
         copy_wait<0>();
         if (!ok && lane == 0) atomicMax(status, (int)KB_TIMEOUT_TMA);
@@ -247,21 +243,19 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
         kb_dep_wait();
         kb_dep_trigger();
         const bool lead = tc::elect_one();
-        int st = 0;
-        uint32_t phase = 1;
 #pragma unroll 1
         for (int i = 0; i < turns; ++i) {
-            ok = tc::mbar_wait(&b_empty[st], phase, abort_flag);
+            const int st = i % TURNS;
+            ok = tc::mbar_wait(&empty[st], ((uint32_t)(i / TURNS) & 1u) ^ 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             if (lead) {
                 const bool two = 2 * i + 1 < nb;
                 const int k = (b0 + 2 * i) * KB;
-                tc::mbar_expect_tx(&b_full[st], two ? 2 * R::BLOCK : R::BLOCK);
-                tc::tma_load_3d(ring + st * 2 * R::BLOCK, &x, &b_full[st], k, m0, 0);
-                if (two) tc::tma_load_3d(ring + (st * 2 + 1) * R::BLOCK, &x, &b_full[st], k + KB, m0, 0);
+                tc::mbar_expect_tx(&full[st], two ? 2 * R::BLOCK : R::BLOCK);
+                tc::tma_load_3d(ring + st * 2 * R::BLOCK, &x, &full[st], k, m0, 0);
+                if (two) tc::tma_load_3d(ring + (st * 2 + 1) * R::BLOCK, &x, &full[st], k + KB, m0, 0);
             }
             __syncwarp();
-            if (++st == R::SB) st = 0, phase ^= 1;
         }
         if (!ok && lane == 0) atomicMax(status, (int)KB_TIMEOUT_TMA);
     } else {
@@ -271,18 +265,15 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
         const uint32_t idesc = tc::instr_desc_f16(ROWS, TN, 1, 1, 0, 0);
         const tc::DescHalves d = tc::smem_desc_halves(smem_u32(ring), 16, 1024);
         const bool lead = tc::elect_one();
-        int sb = 0;
-        uint32_t phase = 0;
 #pragma unroll 1
         for (int i = 0; i < turns; ++i) {
-            const int sa = i % TURNS, set = i % R::SETS;
+            const int st = i % TURNS, set = i % R::SETS;
             ok = tc::mbar_wait(&acc_empty[set], ((uint32_t)(i / R::SETS) & 1u) ^ 1u, abort_flag);
-            ok = ok && tc::mbar_wait(&b_full[sb], phase, abort_flag);
-            ok = ok && tc::mbar_wait(&a_full[sa], (uint32_t)(i / TURNS) & 1u, abort_flag);
+            ok = ok && tc::mbar_wait(&full[st], (uint32_t)(i / TURNS) & 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::tc_fence_after();
             if (lead) {
-                const uint32_t acc = tmem_acc + set * R::SET, a = tmem_a + sa * 64, b = d.lo + ((sb * 2 * R::BLOCK) >> 4);
+                const uint32_t acc = tmem_acc + set * R::SET, a = tmem_a + st * 64, b = d.lo + ((st * 2 * R::BLOCK) >> 4);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) tc::mma_f16_ts_h(acc, a + 8 * k, b + 2 * k, d.hi, idesc, k != 0);
                 if (2 * i + 1 < nb) {
@@ -290,12 +281,10 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
                     for (int k = 0; k < 4; ++k)
                         tc::mma_f16_ts_h(acc + (PG == 1 ? TN : 0), a + 32 + 8 * k, b + (R::BLOCK >> 4) + 2 * k, d.hi, idesc, PG == 2 || k != 0);
                 }
-                tc::tc_commit(&a_empty[sa]);
-                tc::tc_commit(&b_empty[sb]);
+                tc::tc_commit(&empty[st]);
                 tc::tc_commit(&acc_full[set]);
             }
             __syncwarp();
-            if (++sb == R::SB) sb = 0, phase ^= 1;
         }
         if (!ok && lane == 0) atomicMax(status, (int)KB_TIMEOUT_MMA);
     }
