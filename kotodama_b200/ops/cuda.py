@@ -31,11 +31,11 @@ _OUT = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 # arguments of the launchers that are called through CudaOps._launch: p address, i int, l long long, f float; the stream follows
 _CTYPE = {"p": _VP, "i": _I, "l": _LL, "f": _F}
 _ARGS = {
-    "kb_kv_append_fp8": "ppllppppp" + "iiil" + "ip",
-    "kb_kv_gather_fp8": "pppp" + "ii" + "piii" + "pppi" + "ppii" + "p",
-    "kb_tree_attn_plain": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fii" + "p",
-    "kb_tree_attn": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fi" + "pl" + "p",
-    "kb_gemm_int4": "pl" + "pp" + "pl" + "pl" + "iiii" + "p",
+    "kb_kv_append_fp8": "ppllppppp" + "iiil" + "i",
+    "kb_kv_gather_fp8": "pppp" + "ii" + "piii" + "pppi" + "ppii",
+    "kb_tree_attn_plain": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fii",
+    "kb_tree_attn": "pl" + "pppp" + "pii" + "ppip" + "pl" + "iiiiii" + "fi" + "pl",
+    "kb_gemm_int4": "pl" + "pp" + "pl" + "pl" + "iiii",
 }
 
 
@@ -63,6 +63,7 @@ class CudaOps(TorchOps):
         self.launches = 0              # launches of kernels from this library
         self._status: dict[int, torch.Tensor] = {}
         self._fns: dict = {}
+        self._status_at: dict[int, int] = {}       # addresses of the status words
         self.gemm_max_ctas = 0
         self.split_k_small_m = True
         self._splitk_ws: dict = {}
@@ -100,22 +101,26 @@ class CudaOps(TorchOps):
     def _call(self, fn: str, *args) -> None:
         self._rc(getattr(self.lib, fn)(*args), fn)
 
-    def _launch(self, fn: str, *args) -> None:
-        """A launcher called with plain numbers and addresses (its argument types are declared in ``_ARGS``); the stream is the current
-        one.  Cheaper on the host than wrapping every argument: the smallest operators are bound by it."""
+    def _launch(self, fn: str, t: torch.Tensor, *args) -> None:
+        """A launcher called with plain numbers and addresses (its argument types are declared in ``_ARGS``; the status word and the
+        stream follow), on the current stream of ``t``'s device.  Cheaper on the host than wrapping every argument: the smallest
+        operators are bound by it."""
         f = self._fns.get(fn)
         if f is None:
             f = self._fns[fn] = getattr(self.lib, fn)
-            f.argtypes = [_CTYPE[c] for c in _ARGS[fn]] + [_VP]
+            f.argtypes = [_CTYPE[c] for c in _ARGS[fn]] + [_VP, _VP]
+        dev = t.get_device()
+        word = self._status_at.get(dev)
+        if word is None:
+            word = self._status_at[dev] = self.status(t.device).data_ptr()
         self.launches += 1
-        rc = f(*args, torch.cuda.current_stream().cuda_stream)
+        if dev == torch.cuda.current_device():
+            rc = f(*args, word, torch._C._cuda_getCurrentRawStream(dev))
+        else:
+            with torch.cuda.device(dev):
+                rc = f(*args, word, torch._C._cuda_getCurrentRawStream(dev))
         if rc != 0:
             raise KernelError(f"{fn}: launcher returned {rc}")
-
-    @staticmethod
-    def _on(t: torch.Tensor):
-        """The tensor's device made current, where it is not already (launches go to its stream)."""
-        return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
     def status(self, device: torch.device) -> torch.Tensor:
         idx = device.index if device.index is not None else torch.cuda.current_device()
@@ -324,22 +329,29 @@ class CudaOps(TorchOps):
 
     def _gemm_int4(self, a, b, out, residual, accumulate):
         M, K = a.shape
-        N = b.shape[0]
+        N, inputs = b.shape
+        dtype, dev, packed = a.dtype, a.device, b.packed
         if out is None:
-            out = torch.empty(M, N, device=a.device, dtype=a.dtype)
-        if accumulate and residual is not None:
-            raise KernelError("a product with 4-bit weights has one addend")
-        c = residual if residual is not None else (out if accumulate else None)
-        if (K != b.shape[1] or a.dtype != torch.bfloat16 or a.stride(1) != 1 or a.stride(0) % 8 or a.data_ptr() % 16 or out.shape != (M, N)
-                or any(t.dtype != a.dtype or t.stride(-1) != 1 or t.device != a.device for t in (out, c) if t is not None)
-                or b.packed.device != a.device or (c is not None and c.shape not in ((M, N), (1, N)))):
-            raise KernelError(f"4-bit product: bf16 rows of {b.shape[1]} numbers, 16-byte aligned, got {tuple(a.shape)} {a.dtype} {a.stride()}; "
+            out = torch.empty(M, N, device=dev, dtype=dtype)
+            good = True
+        else:
+            good = out.shape == (M, N) and out.dtype == dtype and out.stride(1) == 1 and out.device == dev
+        c, c_stride = residual, 0
+        if accumulate:
+            if residual is not None:
+                raise KernelError("a product with 4-bit weights has one addend")
+            c = out
+        if c is not None:
+            good = good and c.shape in ((M, N), (1, N)) and c.dtype == dtype and c.stride(1) == 1 and c.device == dev
+            c_stride = c.stride(0) if c.shape[0] > 1 else 0
+        stride, inner = a.stride()
+        if (not good or K != inputs or dtype != torch.bfloat16 or inner != 1 or stride % 8 or a.data_ptr() % 16 or packed.device != dev
+                or packed.data_ptr() % 16):
+            raise KernelError(f"4-bit product: bf16 rows of {inputs} numbers, 16-byte aligned, got {tuple(a.shape)} {dtype} {a.stride()}; "
                               f"output and addend bf16 [{M}, {N}]")
         if M:
-            with self._on(a):
-                self._launch("kb_gemm_int4", a.data_ptr(), a.stride(0), b.packed.data_ptr(), b.scales.data_ptr(),
-                             c.data_ptr() if c is not None else None, c.stride(0) if c is not None and c.shape[0] > 1 else 0, out.data_ptr(),
-                             out.stride(0), M, N, K, b.group, self.status(a.device).data_ptr())
+            self._launch("kb_gemm_int4", a, a.data_ptr(), stride, packed.data_ptr(), b.scales.data_ptr(), None if c is None else c.data_ptr(), c_stride,
+                         out.data_ptr(), out.stride(0), M, N, K, b.group)
         return out
 
     def gemm_nt(self, a, b, out=None, residual=None, accumulate=False):
@@ -729,25 +741,29 @@ class CudaOps(TorchOps):
 
     def _kv_append_fp8(self, k, v, k_pages, v_pages, slots):
         pages, n_kv, _, hd = k_pages.shape
-        N = self._fp8_pages(k_pages, v_pages, k, slots)
-        if (k.shape != (N, n_kv * hd) or v.shape != k.shape or slots.shape != (N,) or k.dtype not in _TYPE or v.dtype != k.dtype
-                or k.stride(1) != 1 or v.stride(1) != 1 or slots.dtype != torch.int64 or not slots.is_contiguous() or v.device != k.device):
+        kc, ke, vc, ve = self._fp8_pages(k_pages, v_pages, k.device)
+        N = k.shape[0]
+        dtype = k.dtype
+        (k_stride, k1), (v_stride, v1) = k.stride(), v.stride()
+        if (k.shape != (N, n_kv * hd) or v.shape != (N, n_kv * hd) or slots.shape != (N,) or dtype not in _TYPE or v.dtype != dtype
+                or k1 != 1 or v1 != 1 or slots.dtype != torch.int64 or not slots.is_contiguous() or v.device != k.device or slots.device != k.device):
             raise KernelError(f"8-bit cache append: rows {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}, slots {tuple(slots.shape)} "
                               f"{slots.dtype} for pages {tuple(k_pages.shape)}")
         if N:
-            with self._on(k):
-                self._launch("kb_kv_append_fp8", k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), k_pages.codes.data_ptr(),
-                             k_pages.exps.data_ptr(), v_pages.codes.data_ptr(), v_pages.exps.data_ptr(), slots.data_ptr(), N, n_kv, hd, pages * 16,
-                             _TYPE[k.dtype], self.status(k.device).data_ptr())
+            self._launch("kb_kv_append_fp8", k, k.data_ptr(), v.data_ptr(), k_stride, v_stride, kc, ke, vc, ve, slots.data_ptr(), N, n_kv, hd,
+                         pages * 16, _TYPE[dtype])
 
     @staticmethod
-    def _fp8_pages(k_pages, v_pages, rows, *others) -> int:
-        """Checks that 8-bit pages belong together and lie where ``rows`` do; returns the number of rows."""
-        same = isinstance(v_pages, Fp8Pages) and k_pages.shape == v_pages.shape
-        if not same or k_pages.shape[2] != 16 or not all(t.is_contiguous() and t.device == rows.device for p in (k_pages, v_pages)
-                                                         for t in (p.codes, p.exps)) or any(t.device != rows.device for t in others):
-            raise KernelError("8-bit keys and values are dense pages of one shape, on the device of the rows")
-        return rows.shape[0]
+    def _fp8_pages(k_pages, v_pages, device) -> tuple[int, int, int, int]:
+        """Checks that 8-bit pages belong together and lie on ``device``; returns their addresses."""
+        if isinstance(v_pages, Fp8Pages) and k_pages.shape == v_pages.shape and k_pages.shape[2] == 16:
+            own = (k_pages.codes, k_pages.exps, v_pages.codes, v_pages.exps)
+            for t in own:
+                if not t.is_contiguous() or t.device != device:
+                    break
+            else:
+                return tuple(t.data_ptr() for t in own)
+        raise KernelError("8-bit keys and values are dense pages of one shape, on the device of the rows")
 
     def paged_decode_attention(self, q, k_pages, v_pages, page_table, ctx_lens, max_ctx, n_q, n_kv, hd, split=512):
         """``q[B, n_q*hd]`` (one new token per request) against the paged cache; returns ``[B, n_q*hd]``."""
@@ -978,20 +994,20 @@ class CudaOps(TorchOps):
 
     def _kv_gather_fp8(self, k_pages, v_pages, page_table, seg_seq, seg_first, cu, total, dtype):
         pages, G, _, hd = k_pages.shape
-        segs = seg_seq.numel()
-        self._fp8_pages(k_pages, v_pages, page_table, seg_seq, seg_first, cu)
-        if (dtype not in _TYPE or page_table.ndim != 2 or seg_first.numel() != segs or cu.numel() != segs + 1 or (total and not segs)
-                or any(t.dtype != torch.int32 or not t.is_contiguous() for t in (page_table, seg_seq, seg_first, cu))):
-            raise KernelError(f"8-bit cache rows are read as bf16 or fp32, by dense int32 tables: {dtype}, {segs} segments, "
+        segs, dev = seg_seq.numel(), page_table.device
+        kc, ke, vc, ve = self._fp8_pages(k_pages, v_pages, dev)
+        good = dtype in _TYPE and page_table.ndim == 2 and seg_first.numel() == segs and cu.numel() == segs + 1 and (not total or segs)
+        for t in (page_table, seg_seq, seg_first, cu):
+            good = good and t.dtype == torch.int32 and t.is_contiguous() and t.device == dev
+        if not good:
+            raise KernelError(f"8-bit cache rows are read as bf16 or fp32, by dense int32 tables on the pages' device: {dtype}, {segs} segments, "
                               f"{seg_first.numel()} first positions, {cu.numel()} boundaries")
-        k = torch.empty(total, G, hd, device=page_table.device, dtype=dtype)
+        k = torch.empty(total, G, hd, device=dev, dtype=dtype)
         v = torch.empty_like(k)
         if total:
-            with self._on(page_table):
-                self._launch("kb_kv_gather_fp8", k_pages.codes.data_ptr(), k_pages.exps.data_ptr(), v_pages.codes.data_ptr(),
-                             v_pages.exps.data_ptr(), G, hd, page_table.data_ptr(), page_table.shape[0], page_table.shape[1], pages,
-                             seg_seq.data_ptr(), seg_first.data_ptr(), cu.data_ptr(), segs, k.data_ptr(), v.data_ptr(), total, _TYPE[dtype],
-                             self.status(page_table.device).data_ptr())
+            seqs, width = page_table.shape
+            self._launch("kb_kv_gather_fp8", page_table, kc, ke, vc, ve, G, hd, page_table.data_ptr(), seqs, width, pages, seg_seq.data_ptr(),
+                         seg_first.data_ptr(), cu.data_ptr(), segs, k.data_ptr(), v.data_ptr(), total, _TYPE[dtype])
         return k, v
 
     def paged_attention(self, q, k_pages, v_pages, page_table, ctx_lens, cu_seqlens, max_ctx, scale, softcap, chunk, gate, vdim, cols):
@@ -1026,49 +1042,58 @@ class CudaOps(TorchOps):
         """bf16 queries with heads of 64 or 128 take the tensor-core kernel (``csrc/tree_attn_sm100.cu``); the 32-bit mode, other head
         sizes and query rows that are not 16-byte aligned the plain one (``csrc/tree_attn.cu``)."""
         N, H, hd = q.shape
-        dev = q.device
-        fp8 = isinstance(k_pages, Fp8Pages)
+        dev, dtype = q.device, q.dtype
         B = ctx_lens.numel()
         given = out is not None
-        res = out if given else torch.empty(N, H * hd, device=dev, dtype=q.dtype)
+        fp8 = isinstance(k_pages, Fp8Pages)
         if fp8:
-            self._fp8_pages(k_pages, v_pages, q, page_table, ctx_lens)
-            kt, vt, ke, ve = k_pages.codes, v_pages.codes, k_pages.exps.data_ptr(), v_pages.exps.data_ptr()
+            kp, ke, vp, ve = self._fp8_pages(k_pages, v_pages, dev)
         else:
-            kt, vt, ke, ve = k_pages, v_pages, None, None
-            if (isinstance(v_pages, Fp8Pages) or kt.shape != vt.shape or kt.dtype != q.dtype or vt.dtype != q.dtype or not kt.is_contiguous()
-                    or not vt.is_contiguous() or kt.device != dev or vt.device != dev):
+            if (isinstance(v_pages, Fp8Pages) or k_pages.shape != v_pages.shape or k_pages.dtype != dtype or v_pages.dtype != dtype
+                    or not k_pages.is_contiguous() or not v_pages.is_contiguous() or k_pages.device != dev or v_pages.device != dev
+                    or k_pages.ndim != 4):
                 raise KernelError("keys and values are dense pages of one shape, of the queries' type and device")
-        if (q.dtype not in _TYPE or q.stride(2) != 1 or q.stride(1) != hd or kt.ndim != 4 or kt.shape[2] != 16 or kt.shape[3] != hd
-                or H % kt.shape[1] or res.shape != (N, H * hd) or res.dtype != q.dtype or res.stride(1) != 1 or res.device != dev):
-            raise KernelError(f"tree attention: queries {tuple(q.shape)} {q.dtype} {q.stride()} for pages {tuple(kt.shape)}, output "
-                              f"{tuple(res.shape)} {res.dtype}")
-        if (page_table.ndim != 2 or page_table.shape[0] != B or (cu_seqlens.numel() != B + 1 if cu_seqlens is not None else B > N)
-                or (masks is not None and (masks.shape != (N,) or masks.dtype != torch.int64 or not masks.is_contiguous() or masks.device != dev))
-                or any(t.dtype != torch.int32 or not t.is_contiguous() or t.device != dev
-                       for t in (page_table, ctx_lens, cu_seqlens) if t is not None)):
+            kp, ke, vp, ve = k_pages.data_ptr(), None, v_pages.data_ptr(), None
+        pages, n_kv, size, d = k_pages.shape
+        row, head, inner = q.stride()
+        if given:
+            good = out.shape == (N, H * hd) and out.dtype == dtype and out.stride(1) == 1 and out.device == dev
+        else:
+            out = torch.empty(N, H * hd, device=dev, dtype=dtype)
+            good = True
+        if not good or dtype not in _TYPE or inner != 1 or head != hd or size != 16 or d != hd or H % n_kv:
+            raise KernelError(f"tree attention: queries {tuple(q.shape)} {dtype} {q.stride()} for pages {tuple(k_pages.shape)}, output "
+                              f"{tuple(out.shape)} {out.dtype}")
+        good = page_table.ndim == 2 and page_table.shape[0] == B
+        cu = tree = None
+        if cu_seqlens is None:
+            good = good and B <= N
+        else:
+            good = good and cu_seqlens.numel() == B + 1 and cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.device == dev
+            cu = cu_seqlens.data_ptr()
+        if masks is not None:
+            good = good and masks.shape == (N,) and masks.dtype == torch.int64 and masks.is_contiguous() and masks.device == dev
+            tree = masks.data_ptr()
+        for t in (page_table, ctx_lens):
+            good = good and t.dtype == torch.int32 and t.is_contiguous() and t.device == dev
+        if not good:
             raise KernelError(f"tree attention: {B} lengths, page lists {tuple(page_table.shape)}, boundaries "
                               f"{None if cu_seqlens is None else tuple(cu_seqlens.shape)}, {N} rows; tables are dense int32, masks int64 per row")
-        if N == 0 or B == 0 or page_table.shape[1] == 0:
-            return res if given else res.zero_()
-        floats = 0
-        if q.dtype == torch.bfloat16 and scale > 0 and q.stride(0) % 8 == 0 and res.stride(0) % 4 == 0 and q.data_ptr() % 16 == 0 and res.data_ptr() % 8 == 0:
-            floats = self._tree_floats(N, B, H, kt.shape[1], hd, max_q, max_ctx, int(fp8))
+        width = page_table.shape[1]
+        if N == 0 or B == 0 or width == 0:
+            return out if given else out.zero_()
+        q_at, out_at, out_row, floats = q.data_ptr(), out.data_ptr(), out.stride(0), 0
+        if dtype == torch.bfloat16 and scale > 0 and row % 8 == 0 and out_row % 4 == 0 and q_at % 16 == 0 and out_at % 8 == 0:
+            floats = self._tree_floats(N, B, H, n_kv, hd, max_q, max_ctx, int(fp8))
+        where = (q_at, row, kp, ke, vp, ve, page_table.data_ptr(), width, pages, ctx_lens.data_ptr(), cu, B, tree, out_at, out_row, N, H, n_kv, hd,
+                 max_q, max_ctx, scale, int(not given))
         if floats:
             work = torch.empty(floats, device=dev, dtype=torch.float32)
-            with self._on(q):
-                self._launch("kb_tree_attn", q.data_ptr(), q.stride(0), kt.data_ptr(), ke, vt.data_ptr(), ve, page_table.data_ptr(),
-                             page_table.shape[1], kt.shape[0], ctx_lens.data_ptr(), cu_seqlens.data_ptr() if cu_seqlens is not None else None, B,
-                             masks.data_ptr() if masks is not None else None, res.data_ptr(), res.stride(0), N, H, kt.shape[1], hd, max_q, max_ctx,
-                             scale, int(not given), work.data_ptr(), floats, self.status(dev).data_ptr())
+            self._launch("kb_tree_attn", q, *where, work.data_ptr(), floats)
             self.launches += 1
-            return res
-        with self._on(q):
-            self._launch("kb_tree_attn_plain", q.data_ptr(), q.stride(0), kt.data_ptr(), ke, vt.data_ptr(), ve, page_table.data_ptr(),
-                         page_table.shape[1], kt.shape[0], ctx_lens.data_ptr(), cu_seqlens.data_ptr() if cu_seqlens is not None else None, B,
-                         masks.data_ptr() if masks is not None else None, res.data_ptr(), res.stride(0), N, H, kt.shape[1], hd, max_q, max_ctx,
-                         scale, int(not given), _TYPE[q.dtype], self.status(dev).data_ptr())
-        return res
+        else:
+            self._launch("kb_tree_attn_plain", q, *where, _TYPE[dtype])
+        return out
 
     delta_short = 16        # most tokens of a sequence in one pass for which the recurrence is walked token by token
 
