@@ -42,29 +42,30 @@ append_kernel(const T* __restrict__ k, const T* __restrict__ v, const AppendShap
     kb_dep_wait();
     constexpr int GROUPS = THREADS / LANES;
     const int sub = threadIdx.x % LANES;
-    const long long rows = 2ll * s.N * s.n_kv;
-    const long long base = (long long)blockIdx.x * (GROUPS * U) + threadIdx.x / LANES;
+    const uint32_t rows = 2u * s.N * s.n_kv, per = 2u * s.n_kv;
+    const uint32_t base = blockIdx.x * (GROUPS * U) + threadIdx.x / LANES;
     const bool mine = sub * 8 < s.hd;
     float x[U][8];
     long long at[U];
     bool isv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const long long r = base + (long long)u * GROUPS;
+        const uint32_t r = base + u * GROUPS;
         at[u] = -1;
         isv[u] = false;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
         if (r < rows) {
-            const int per = 2 * s.n_kv, n = (int)(r / per), c = (int)(r % per);
-            isv[u] = c >= s.n_kv;
-            const int head = isv[u] ? c - s.n_kv : c;
+            const uint32_t n = r / per, c = r % per;
+            isv[u] = c >= (uint32_t)s.n_kv;
+            const uint32_t head = isv[u] ? c - s.n_kv : c;
+            // (the row is fetched beside its slot, not behind it)
+            if (mine) load8((isv[u] ? v + n * s.v_stride : k + n * s.k_stride) + (long long)head * s.hd + sub * 8, x[u]);
             const long long slot = slots[n];
             if (slot >= s.num_slots) {
                 if (c == 0 && sub == 0 && status) atomicMax(status, (int)KB_BAD_INDEX);
             } else if (slot >= 0) {
                 at[u] = ((slot / PAGE) * s.n_kv + head) * PAGE + slot % PAGE;
-                if (mine) load8((isv[u] ? v + n * s.v_stride : k + n * s.k_stride) + (long long)head * s.hd + sub * 8, x[u]);
             }
         }
     }
@@ -97,6 +98,26 @@ __device__ __forceinline__ void unpack16(const uint4 c, float f, float* x) {
         x[2 * i] = p.x * f;
         x[2 * i + 1] = p.y * f;
     }
+}
+
+// Sixteen numbers as whole 32-byte sectors (16-byte stores 32 bytes apart would write each sector in two halves).
+__device__ __forceinline__ void store32(void* dst, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]),
+                 "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+__device__ __forceinline__ void store16(bf16* dst, const float* x) {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+    }
+    store32(dst, w);
+}
+__device__ __forceinline__ void store16(float* dst, const float* x) {
+    store32(dst, reinterpret_cast<const uint32_t*>(x));
+    store32(dst + 8, reinterpret_cast<const uint32_t*>(x) + 8);
 }
 
 struct GatherShape {
@@ -149,8 +170,7 @@ gather_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ ke, co
                 float x[16];
                 unpack16(w[u], pow2(e[u]), x);
                 T* dst = (isv ? v : k) + row * s.G * s.hd + (long long)(isv ? c - pieces : c) * 16;
-                store8(dst, x);
-                store8(dst + 8, x + 8);
+                store16(dst, x);
             }
         }
     }
@@ -160,10 +180,10 @@ template <typename T, int LANES>
 int launch_append(const void* k, const void* v, const AppendShape& s, void* kc, void* ke, void* vc, void* ve, const long long* slots,
                   int* status, cudaStream_t st) {
     const long long rows = 2ll * s.N * s.n_kv, groups = THREADS / LANES;
+    if (rows > 0x7fffffffll - 4 * groups) return 5;
     // four rows per lane group once that still fills the GPU with warps
     if (rows >= 148ll * 8 * groups * 4) {
         const long long blocks = (rows + groups * 4 - 1) / (groups * 4);
-        if (blocks > 0x7fffffffll) return 5;
         return kb_launch_dep(append_kernel<T, LANES, 4>, dim3((unsigned)blocks), dim3(THREADS), 0, st, (const T*)k, (const T*)v, s, (uint8_t*)kc,
                              (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, slots, status);
     }
@@ -200,7 +220,7 @@ KB_API int kb_kv_gather_fp8(const void* kc, const void* ke, const void* vc, cons
                             int num_pages, const int* seq, const int* first, const int* cu, int segs, void* k, void* v, int total, int type,
                             int* status, cudaStream_t st) {
     if (G < 1 || hd < 16 || hd > 256 || hd % 16 || B < 1 || segs < 1 || total < 1 || type < 0 || type > 1 ||
-        ((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) % 16)
+        ((uintptr_t)k | (uintptr_t)v) % 32 || ((uintptr_t)kc | (uintptr_t)vc) % 16)
         return 5;
     const GatherShape s{G, hd, B, max_pages, num_pages, segs, total};
     const unsigned blocks = (unsigned)((total + THREADS / 32 - 1) / (THREADS / 32));

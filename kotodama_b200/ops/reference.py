@@ -69,16 +69,12 @@ class Fp8Pages:
         if codes.dtype != torch.float8_e4m3fn or exps.dtype != torch.uint8 or codes.ndim != 4 or codes.shape[:3] != exps.shape:
             raise ValueError(f"8-bit pages are e4m3 codes [pages, n_kv, 16, hd] and uint8 exponents [pages, n_kv, 16], got "
                              f"{codes.dtype} {tuple(codes.shape)}, {exps.dtype} {tuple(exps.shape)}")
-        self.codes, self.exps = codes, exps
+        self.codes, self.exps, self.shape = codes, exps, codes.shape
 
     @classmethod
     def zeros(cls, pages: int, n_kv: int, hd: int, device: torch.device | str) -> "Fp8Pages":
         return cls(torch.zeros(pages, n_kv, 16, hd, device=device, dtype=torch.float8_e4m3fn),
                    torch.full((pages, n_kv, 16), 127, device=device, dtype=torch.uint8))
-
-    @property
-    def shape(self):
-        return self.codes.shape
 
     @property
     def device(self):
