@@ -17,12 +17,6 @@ namespace {
 constexpr int PAGE = 16;
 constexpr int THREADS = 256;
 
-__device__ __forceinline__ uint32_t pack4(const float* v, float inv) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(v[2] * inv, v[3] * inv), __NV_SATFINITE, __NV_E4M3);
-    return lo | (hi << 16);
-}
-
 __device__ __forceinline__ float pow2(uint32_t biased) {         // 2^(biased - 127); 255 gives infinity
     return __uint_as_float(biased ? biased << 23 : 0x00400000u);
 }
@@ -32,8 +26,69 @@ struct AppendShape {
     long long k_stride, v_stride, num_slots;
 };
 
-// LANES (a power of two, at least hd / 8) lanes share a row, eight elements each; a row is one (token, key or value, kv head).
-// U rows per lane group are loaded before the first is used.
+// Eight elements of a row as they lie in memory.
+template <typename T>
+struct Piece {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void load(const T* src) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(src) + i * 16);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)(2 * sizeof(T)); ++i) w[i] = 0;
+    }
+    __device__ __forceinline__ uint2 codes(float inv) const {
+        uint32_t h[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float lo = __uint_as_float(sizeof(T) == 2 ? w[i] << 16 : w[2 * i % (2 * sizeof(T))]);
+            const float hi = __uint_as_float(sizeof(T) == 2 ? w[i] & 0xffff0000u : w[(2 * i + 1) % (2 * sizeof(T))]);
+            h[i] = __nv_cvt_float2_to_fp8x2(make_float2(lo * inv, hi * inv), __NV_SATFINITE, __NV_E4M3);
+        }
+        return make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+    }
+};
+
+// Largest magnitudes of a row of keys and a row of values over LANES lanes, as bits of fp32 (infinities and NaNs are largest).  Two bf16
+// magnitudes share a word on the way: half the shuffles.
+template <int LANES>
+__device__ __forceinline__ uint2 largest(const Piece<bf16>& k, const Piece<bf16>& v) {
+    uint32_t a = k.w[0] & 0x7fff7fffu, b = v.w[0] & 0x7fff7fffu;
+#pragma unroll
+    for (int i = 1; i < 4; ++i) {
+        a = __vmaxu2(a, k.w[i] & 0x7fff7fffu);
+        b = __vmaxu2(b, v.w[i] & 0x7fff7fffu);
+    }
+    uint32_t m = __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = __vmaxu2(m, __shfl_xor_sync(0xffffffffu, m, o));
+    return make_uint2(m << 16, m & 0xffff0000u);
+}
+template <int LANES>
+__device__ __forceinline__ uint2 largest(const Piece<float>& k, const Piece<float>& v) {
+    uint32_t a = 0, b = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        a = max(a, k.w[i] & 0x7fffffffu);
+        b = max(b, v.w[i] & 0x7fffffffu);
+    }
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) {
+        a = max(a, __shfl_xor_sync(0xffffffffu, a, o));
+        b = max(b, __shfl_xor_sync(0xffffffffu, b, o));
+    }
+    return make_uint2(a, b);
+}
+
+// LANES (a power of two, at least hd / 8) lanes share a (token, kv head): its row of keys and its row of values, eight elements of each per
+// lane.  U of them per lane group are loaded before the first is used.
 template <typename T, int LANES, int U>
 __global__ void __launch_bounds__(THREADS)
 append_kernel(const T* __restrict__ k, const T* __restrict__ v, const AppendShape s, uint8_t* __restrict__ kc, uint8_t* __restrict__ ke,
@@ -42,50 +97,49 @@ append_kernel(const T* __restrict__ k, const T* __restrict__ v, const AppendShap
     kb_dep_wait();
     constexpr int GROUPS = THREADS / LANES;
     const int sub = threadIdx.x % LANES;
-    const uint32_t rows = 2u * s.N * s.n_kv, per = 2u * s.n_kv;
-    const uint32_t base = blockIdx.x * (GROUPS * U) + threadIdx.x / LANES;
+    const uint32_t rows = (uint32_t)s.N * s.n_kv, base = blockIdx.x * (GROUPS * U) + threadIdx.x / LANES;
     const bool mine = sub * 8 < s.hd;
-    float x[U][8];
+    Piece<T> x[U], y[U];
     long long at[U];
-    bool isv[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const uint32_t r = base + u * GROUPS;
         at[u] = -1;
-        isv[u] = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[u][i] = 0.f;
+        x[u].zero();
+        y[u].zero();
         if (r < rows) {
-            const uint32_t n = r / per, c = r % per;
-            isv[u] = c >= (uint32_t)s.n_kv;
-            const uint32_t head = isv[u] ? c - s.n_kv : c;
-            // (the row is fetched beside its slot, not behind it)
-            if (mine) load8((isv[u] ? v + n * s.v_stride : k + n * s.k_stride) + (long long)head * s.hd + sub * 8, x[u]);
+            const uint32_t n = r / s.n_kv, head = r - n * s.n_kv;
             const long long slot = slots[n];
+            if (mine) {                                // (the rows are fetched beside their slot, not behind it)
+                const uint32_t col = head * s.hd + sub * 8;
+                x[u].load(k + n * s.k_stride + col);
+                y[u].load(v + n * s.v_stride + col);
+            }
             if (slot >= s.num_slots) {
-                if (c == 0 && sub == 0 && status) atomicMax(status, (int)KB_BAD_INDEX);
+                if (head == 0 && sub == 0 && status) atomicMax(status, (int)KB_BAD_INDEX);
             } else if (slot >= 0) {
-                at[u] = ((slot / PAGE) * s.n_kv + head) * PAGE + slot % PAGE;
+                at[u] = (((unsigned long long)slot / PAGE) * s.n_kv + head) * PAGE + (slot & (PAGE - 1));
             }
         }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        uint32_t m = 0;                                  // largest magnitude, as bits: infinities and NaNs are largest
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(x[u][i]) & 0x7fffffffu);
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+        const uint2 m = largest<LANES>(x[u], y[u]);
         if (at[u] < 0) continue;
         // 448 = 1.75 * 2^8: the exponent is that of the magnitude less 8, one more where its mantissa is above 1.75
-        const int e = min(max((int)(m >> 23) - 8 + ((m & 0x7fffffu) > 0x600000u), 1), 254);
-        const bool bad = m >= 0x7f800000u;
-        const float inv = pow2(254 - e);
+        const int e = min(max((int)(m.x >> 23) - 8 + ((m.x & 0x7fffffu) > 0x600000u), 1), 254);
+        const int f = min(max((int)(m.y >> 23) - 8 + ((m.y & 0x7fffffu) > 0x600000u), 1), 254);
+        const bool bad = m.x >= 0x7f800000u, worse = m.y >= 0x7f800000u;
         if (mine) {
-            const uint2 c = bad ? make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu) : make_uint2(pack4(x[u], inv), pack4(x[u] + 4, inv));
-            *reinterpret_cast<uint2*>((isv[u] ? vc : kc) + at[u] * s.hd + sub * 8) = c;
+            const uint2 c = x[u].codes(pow2(254 - e)), d = y[u].codes(pow2(254 - f)), nan = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+            const long long to = at[u] * s.hd + sub * 8;
+            *reinterpret_cast<uint2*>(kc + to) = bad ? nan : c;
+            *reinterpret_cast<uint2*>(vc + to) = worse ? nan : d;
         }
-        if (sub == 0) (isv[u] ? ve : ke)[at[u]] = (uint8_t)(bad ? 255 : e);
+        if (sub == 0) {
+            ke[at[u]] = (uint8_t)(bad ? 255 : e);
+            ve[at[u]] = (uint8_t)(worse ? 255 : f);
+        }
     }
 }
 
@@ -179,14 +233,12 @@ gather_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ ke, co
 template <typename T, int LANES>
 int launch_append(const void* k, const void* v, const AppendShape& s, void* kc, void* ke, void* vc, void* ve, const long long* slots,
                   int* status, cudaStream_t st) {
-    const long long rows = 2ll * s.N * s.n_kv, groups = THREADS / LANES;
-    if (rows > 0x7fffffffll - 4 * groups) return 5;
-    // four rows per lane group once that still fills the GPU with warps
-    if (rows >= 148ll * 8 * groups * 4) {
-        const long long blocks = (rows + groups * 4 - 1) / (groups * 4);
-        return kb_launch_dep(append_kernel<T, LANES, 4>, dim3((unsigned)blocks), dim3(THREADS), 0, st, (const T*)k, (const T*)v, s, (uint8_t*)kc,
-                             (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, slots, status);
-    }
+    const long long rows = (long long)s.N * s.n_kv, groups = THREADS / LANES;
+    if (rows > 0x7fffffffll - 2 * groups) return 5;
+    // two per lane group once that still fills the GPU with warps
+    if (rows >= 148ll * 8 * groups * 2)
+        return kb_launch_dep(append_kernel<T, LANES, 2>, dim3((unsigned)((rows + groups * 2 - 1) / (groups * 2))), dim3(THREADS), 0, st, (const T*)k,
+                             (const T*)v, s, (uint8_t*)kc, (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, slots, status);
     return kb_launch_dep(append_kernel<T, LANES, 1>, dim3((unsigned)((rows + groups - 1) / groups)), dim3(THREADS), 0, st, (const T*)k,
                          (const T*)v, s, (uint8_t*)kc, (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, slots, status);
 }
