@@ -6,6 +6,8 @@ from typing import Any, Optional, Sequence
 
 import torch
 
+from ..ops import Fp8Pages
+
 PAGE = 16                          # tokens per page
 
 
@@ -49,13 +51,17 @@ class PagePool:
 
 
 class PagedKVCache(PagePool):
-    """Keys and values per KV head."""
+    """Keys and values per KV head, in 8 bits (:class:`~kotodama_b200.ops.Fp8Pages` per layer) where ``fp8`` asks for it."""
 
     def __init__(self, cfg: Any, num_pages: int, device: torch.device, dtype: torch.dtype,
-                 n_kv_local: Optional[int] = None) -> None:
+                 n_kv_local: Optional[int] = None, fp8: bool = False) -> None:
         super().__init__(num_pages)
         self.n_kv = n_kv_local or cfg.num_kv_heads
         self.hd = cfg.head_dim
+        if fp8:
+            make = lambda: [Fp8Pages.zeros(num_pages, self.n_kv, self.hd, device) for _ in range(cfg.num_layers)]
+            self.k, self.v = make(), make()
+            return
         shape = (cfg.num_layers, num_pages, self.n_kv, PAGE, self.hd)      # 16 rows of one (page, head) are contiguous
         self.k = torch.zeros(shape, device=device, dtype=dtype)
         self.v = torch.zeros(shape, device=device, dtype=dtype)

@@ -32,7 +32,7 @@ import torch
 
 from ..ops import get_ops
 from .cache import PAGE, PagedKVCache, PagePool  # noqa: F401  (the engine module re-exports its cache)
-from .runners import Batch, make_runner
+from .runners import Batch, make_runner, runner_class
 
 
 @dataclass
@@ -93,7 +93,9 @@ class ServingEngine:
     def __init__(self, model: Any, *, device: torch.device | str = "cpu",
                  dtype: torch.dtype = torch.float32, max_batch: int = 64, num_pages: Optional[int] = None,
                  max_ctx: Optional[int] = None, ops: Any = None, tp: Any = None,
-                 prefill_batch_tokens: int = 8192, prefill_portion: int = 0) -> None:
+                 prefill_batch_tokens: int = 8192, prefill_portion: int = 0, kv_dtype: Optional[str] = None, weight_bits: int = 16) -> None:
+        """``kv_dtype`` "fp8": keys and values of the cache in 8 bits (one power of two per token and head); ``weight_bits`` 4: the layers'
+        projections in 4 bits (one scale per 128 inputs), in bf16 passes on CUDA.  Llama family, one GPU."""
         self.device = torch.device(device)
         self.dtype = dtype
         self.model = model.eval()
@@ -102,6 +104,16 @@ class ServingEngine:
         self.tp = tp                                  # tensor-parallel helper (``serve.tp``) or None
         self.max_batch = max_batch
         self.max_ctx = max_ctx or self.cfg.max_position_embeddings
+        if kv_dtype not in (None, "fp8") or weight_bits not in (4, 16):
+            raise ValueError(f"kv_dtype is None or 'fp8', weight_bits 4 or 16; got {kv_dtype!r}, {weight_bits!r}")
+        self.kv_dtype, self.weight_bits = kv_dtype, weight_bits
+        if kv_dtype is not None or weight_bits != 16:
+            if not getattr(runner_class(self.model), "low_bits", False) or tp is not None:
+                raise ValueError("an 8-bit cache and 4-bit weights are for the Llama family, on one GPU")
+            if weight_bits == 4 and self.device.type == "cuda" and dtype != torch.bfloat16:
+                raise ValueError(f"4-bit weights on CUDA are for bf16 passes, not {dtype}")
+            if kv_dtype == "fp8" and (self.cfg.head_dim % 16 or self.cfg.head_dim > 256):
+                raise ValueError(f"an 8-bit cache has heads of a multiple of 16, at most 256; not {self.cfg.head_dim}")
         self.runner = make_runner(self)
         self.arena = getattr(self.runner, "arena", None)
         self.H, self.KV = getattr(self.runner, "H", None), getattr(self.runner, "KV", None)     # local heads, where one number describes all layers

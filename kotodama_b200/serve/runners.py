@@ -41,17 +41,23 @@ class Batch:
     spans: Optional[list[tuple[int, int]]] = None  # per sequence (tokens in the cache before, new tokens); not for decode
 
 
+def runner_class(model: Any) -> type:
+    return globals()[family_of(model).runner]
+
+
 def make_runner(engine: Any) -> Any:
-    return globals()[family_of(engine.model).runner](engine)
+    return runner_class(engine.model)(engine)
 
 
 class LlamaRunner:
     """Llama-family decoder with block attention residuals (``models/llama.py``): the executor's forward schedule
-    on the same ops backend, keys and values in the paged cache."""
+    on the same ops backend, keys and values in the paged cache.  The cache may be kept in 8 bits and the layers' projections in 4
+    (``ServingEngine``'s ``kv_dtype`` and ``weight_bits``); the embedding and the head stay as they are."""
 
     continues = False
     needs_prev = False
     context_buckets = True
+    low_bits = True
 
     def __init__(self, eng: Any) -> None:
         self.ops, self.cfg, self.tp, self.model = eng.ops, eng.model.config, eng.tp, eng.model
@@ -67,7 +73,8 @@ class LlamaRunner:
         for i in range(cfg.num_layers):
             p = f"layers.{i}."
             g = lambda n: ar.view(p + n) if (p + n) in ar.by_name else None
-            dw = self.ops.decode_weight          # on CUDA: adds the tile-major copy that decode-size products stream
+            # decode_weight, on CUDA: adds the tile-major copy that decode-size products stream
+            dw = self.ops.quant_int4 if eng.weight_bits == 4 else self.ops.decode_weight
             self.layers.append(dict(
                 wqkv=dw(ar.fused(p + "attn.q_proj.weight", p + "attn.v_proj.weight")), wo=dw(ar.view(p + "attn.o_proj.weight")),
                 wgu=dw(ar.fused(p + "ffn.gate_proj.weight", p + "ffn.up_proj.weight")), wd=dw(ar.view(p + "ffn.down_proj.weight")),
@@ -75,10 +82,11 @@ class LlamaRunner:
                 kn=g("attn.k_norm.weight"), aq=g("attn_res_query"), an=g("attn_res_norm.weight"),
                 mq=g("mlp_res_query"), mn=g("mlp_res_norm.weight")))
         self.boundaries = frozenset(cfg.boundaries()) if cfg.attn_res else frozenset()
+        self.fp8_cache = eng.kv_dtype == "fp8"
         self.cache: Any = None
 
     def make_cache(self, pages: int) -> PagedKVCache:
-        self.cache = PagedKVCache(self.cfg, pages, self.device, self.dtype, n_kv_local=self.KV)
+        self.cache = PagedKVCache(self.cfg, pages, self.device, self.dtype, n_kv_local=self.KV, fp8=self.fp8_cache)
         return self.cache
 
     @torch.no_grad()
@@ -109,6 +117,9 @@ class LlamaRunner:
                                          v_rows.view(1, N, KV, hd), need_grad=False, cu_seqlens=b.cu_seqlens,
                                          max_seqlen=b.max_seqlen)
                 attn = o.reshape(N, H * hd)
+            elif self.fp8_cache:
+                attn = ops.paged_tree_attention(qk[:, : H * hd].view(N, H, hd), self.cache.k[i], self.cache.v[i], b.page_table, b.ctx_lens,
+                                                None, 1, b.max_ctx, hd ** -0.5)
             else:
                 attn = ops.paged_decode_attention(qk[:, : H * hd], self.cache.k[i], self.cache.v[i],
                                                   b.page_table, b.ctx_lens, b.max_ctx, H, KV, hd)

@@ -83,6 +83,9 @@ def main() -> None:
                     help="default: bfloat16 on CUDA, float32 on CPU; float32 on CUDA for families with 32-bit kernels")
     ap.add_argument("--prefill_portion", type=int, default=0,
                     help="most prompt tokens of one request per step (0: whole prompts); families that continue a cached context")
+    ap.add_argument("--kv_cache", default=None, choices=["fp8"], help="keys and values of the cache in 8 bits (Llama family, one GPU)")
+    ap.add_argument("--weight_bits", type=int, default=16, choices=[4, 16],
+                    help="4: the layers' projections in 4 bits (Llama family, one GPU; bfloat16 on CUDA)")
     args = ap.parse_args()
     logging.basicConfig(level=logging.INFO, format="%(asctime)s %(levelname)s %(name)s: %(message)s")
     device = "cuda" if args.device == "cuda" and torch.cuda.is_available() else "cpu"
@@ -112,7 +115,8 @@ def main() -> None:
         name = f"kotodama-{args.model_size}"
     dtype = getattr(torch, args.dtype) if args.dtype else torch.bfloat16 if device.startswith("cuda") else torch.float32
     engine = ServingEngine(model, device=device, dtype=dtype, max_batch=args.max_batch, max_ctx=args.max_ctx, tp=tp,
-                           prefill_batch_tokens=args.prefill_batch_tokens, prefill_portion=args.prefill_portion)
+                           prefill_batch_tokens=args.prefill_batch_tokens, prefill_portion=args.prefill_portion, kv_dtype=args.kv_cache,
+                           weight_bits=args.weight_bits)
     if tp is not None and rank > 0:
         run_follower(engine, tp)
         return
