@@ -36,6 +36,8 @@ def main() -> None:
     ap.add_argument("--seed", type=int, default=0)
     ap.add_argument("--prefill-batch-tokens", type=int, default=8192,
                     help="rows of one padded prefill pass shared by several prompts (0: one prompt per pass)")
+    ap.add_argument("--kv-cache", default=None, choices=["fp8"], help="keys and values of the cache in 8 bits")
+    ap.add_argument("--weight-bits", type=int, default=16, choices=[4, 16], help="4: the layers' projections in 4 bits")
     ap.add_argument("--device", default="cuda")
     ap.add_argument("--passes", type=int, default=2, help="2: report the second (warm) pass, the first one separately")
     ap.add_argument("--profile-decode-step", type=int, default=-1,
@@ -75,8 +77,10 @@ def run(a, rank: int, world: int, local: int) -> dict:
         model = KotodamaModel(cfg)
     eng = ServingEngine(model, device=a.device, dtype=torch.bfloat16 if cuda else torch.float32,
                         max_batch=a.requests, max_ctx=a.max_prompt + a.new_tokens + 16, tp=tp,
-                        prefill_batch_tokens=a.prefill_batch_tokens)
+                        prefill_batch_tokens=a.prefill_batch_tokens, kv_dtype=getattr(a, "kv_cache", None), weight_bits=getattr(a, "weight_bits", 16))
     eng.arena.init_weights(cfg.num_layers, a.seed)
+    if eng.weight_bits == 4:
+        eng.runner.layers = eng.runner.load_layers()
     g = torch.Generator().manual_seed(a.seed)
     lens = torch.randint(a.min_prompt, a.max_prompt + 1, (a.requests,), generator=g).tolist()
     prompts = [torch.randint(0, cfg.vocab_size, (n,), generator=g).tolist() for n in lens]

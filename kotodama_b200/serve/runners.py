@@ -64,26 +64,32 @@ class LlamaRunner:
         self.device, self.dtype = eng.device, eng.dtype
         if self.tp is not None:
             self.tp.prepare_model(self.model)
-        ar = self.arena = ParamArena(self.model, self.device, self.dtype, with_grads=False)
+        self.arena = ParamArena(self.model, self.device, self.dtype, with_grads=False)
         cfg = self.cfg
         tpn = self.tp.size if self.tp is not None else 1
         self.H, self.KV = cfg.num_attention_heads // tpn, cfg.num_kv_heads // tpn
         self.hd = cfg.head_dim
-        self.layers = []
-        for i in range(cfg.num_layers):
+        self.weight_bits = eng.weight_bits
+        self.layers = self.load_layers()
+        self.boundaries = frozenset(cfg.boundaries()) if cfg.attn_res else frozenset()
+        self.fp8_cache = eng.kv_dtype == "fp8"
+        self.cache: Any = None
+
+    def load_layers(self) -> list[dict]:
+        """The layers' weights as their products take them, from the arena's values (again where those have changed)."""
+        ar, layers = self.arena, []
+        for i in range(self.cfg.num_layers):
             p = f"layers.{i}."
             g = lambda n: ar.view(p + n) if (p + n) in ar.by_name else None
             # decode_weight, on CUDA: adds the tile-major copy that decode-size products stream
-            dw = self.ops.quant_int4 if eng.weight_bits == 4 else self.ops.decode_weight
-            self.layers.append(dict(
+            dw = self.ops.quant_int4 if self.weight_bits == 4 else self.ops.decode_weight
+            layers.append(dict(
                 wqkv=dw(ar.fused(p + "attn.q_proj.weight", p + "attn.v_proj.weight")), wo=dw(ar.view(p + "attn.o_proj.weight")),
                 wgu=dw(ar.fused(p + "ffn.gate_proj.weight", p + "ffn.up_proj.weight")), wd=dw(ar.view(p + "ffn.down_proj.weight")),
                 attn_norm=g("attn_norm.weight"), ffn_norm=g("ffn_norm.weight"), qn=g("attn.q_norm.weight"),
                 kn=g("attn.k_norm.weight"), aq=g("attn_res_query"), an=g("attn_res_norm.weight"),
                 mq=g("mlp_res_query"), mn=g("mlp_res_norm.weight")))
-        self.boundaries = frozenset(cfg.boundaries()) if cfg.attn_res else frozenset()
-        self.fp8_cache = eng.kv_dtype == "fp8"
-        self.cache: Any = None
+        return layers
 
     def make_cache(self, pages: int) -> PagedKVCache:
         self.cache = PagedKVCache(self.cfg, pages, self.device, self.dtype, n_kv_local=self.KV, fp8=self.fp8_cache)
