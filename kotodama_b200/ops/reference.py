@@ -207,7 +207,7 @@ class TorchOps:
     # ------------------------------------------------------------------ 4-bit weights
     def quant_int4(self, w: torch.Tensor, group: int = 128) -> Int4Weight:
         """``w[N, K]`` (K a multiple of 8) in 4 bits: scale ``amax / 7`` per row and group, rounded to bf16 first so that the codes
-        fit the stored scale; ties to even."""
+        fit the stored scale; ties to even.  A group that holds an infinity or a NaN has a scale that is not finite."""
         N, K = w.shape
         if K % 8 or group not in (64, 128):
             raise ValueError(f"4-bit weights take groups of 64 or 128 and inputs in eights, got {tuple(w.shape)}, group {group}")
@@ -217,7 +217,7 @@ class TorchOps:
         x = x.view(nt * 16, ng, group)
         scale = (x.abs().amax(-1) / 7.0).to(torch.bfloat16)
         div = torch.where(scale == 0, torch.ones_like(scale), scale).float()
-        codes = torch.round(x / div[..., None]).clamp(-8, 7).to(torch.int64) + 8
+        codes = torch.nan_to_num(torch.round(x / div[..., None])).clamp(-8, 7).to(torch.int64) + 8
         c = codes.view(nt * 16, ng * group)[:, : kb * 64].reshape(nt, 2, 8, kb, 4, 4, 4).permute(0, 3, 2, 4, 5, 1, 6)
         words = (c << torch.tensor(_INT4_SHIFT, device=w.device)).sum((-1, -2))                # nt, kb, r, c, j
         packed = (words - ((words >> 31) << 32)).to(torch.int32).reshape(nt, kb, 32, 4).contiguous()

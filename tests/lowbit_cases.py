@@ -442,6 +442,48 @@ def check_int4(ops, device, dtype, M, N, K, group, seed=0, stride=0):
 INT4_CASES = [(1, 16, 64, 64, 0), (1, 1, 8, 128, 0), (3, 40, 200, 128, 8), (8, 96, 512, 128, 0), (9, 33, 520, 64, 0), (17, 130, 1032, 128, 16),
               (33, 64, 64, 128, 0), (64, 48, 768, 64, 0), (65, 100, 1000, 128, 0), (130, 70, 136, 64, 8)]
 
+# every form of the two product kernels: row tiles per block of threads (1 to 4 at a time, steps of unequal size), rings that turn over,
+# inputs shared by clusters and not, one block left over, several portions of tokens
+INT4_LARGE_CASES = [(4, 2501, 136, 64, 0), (8, 5001, 200, 128, 0), (1, 9500, 72, 64, 8), (7, 16500, 192, 128, 0), (2, 40, 8200, 128, 0), (5, 64, 4160, 64, 0),
+                    (16, 2500, 648, 128, 0), (12, 5000, 136, 64, 0), (9, 12001, 264, 128, 0), (11, 48, 8232, 128, 0), (10, 96, 5000, 64, 8),
+                    (40, 9990, 1032, 128, 0), (20, 130, 8200, 128, 0), (64, 200, 8264, 64, 0), (100, 128, 2056, 128, 0), (300, 100, 1352, 128, 8),
+                    (130, 1000, 968, 64, 0), (1000, 272, 456, 128, 0), (17, 13, 24, 64, 0), (33, 1, 8, 128, 0)]
+
+
+def check_int4_overlapping_rows(ops, device):
+    """Rows of x that are one row, and rows that overlap."""
+    x, w = int4_case(24, 40, 136, 64, 5)
+    dense, _ = plain_int4(w)
+    wd = Int4Weight(w.packed.to(device), w.scales.to(device), w.shape, w.group)
+    flat = x.to(device).reshape(-1)
+    for rows in (x[:1].to(device).expand(24, 136), flat.as_strided((24, 136), (8, 1))):
+        want = rows.cpu().to(F64) @ dense.t()
+        held = 143 * 1.1 * rows.cpu().to(F64).abs().sum(1, keepdim=True)
+        err = (ops.gemm_nt(rows, wd).cpu().to(F64) - want).abs()
+        assert bool((err <= 2.0 ** -8 * want.abs() + 8 * 2.0 ** -22 * held).all())
+
+
+def check_quant_int4_not_finite(ops, device):
+    """A group that holds an infinity or a NaN has a scale that is not finite; all others are as without it."""
+    w = torch.randn(33, 256, generator=torch.Generator().manual_seed(4))
+    clean = plain_int4(ops.quant_int4(w.to(device), 64))[0]
+    for what in (math.nan, math.inf, -math.inf):
+        d = w.clone()
+        d[9, 70] = what
+        q = ops.quant_int4(d.to(device), 64)
+        got = plain_int4(q)[0]
+        bad = torch.zeros(33, 256, dtype=torch.bool)
+        bad[9, 64:128] = True
+        assert torch.equal(got[~bad], clean[~bad]) and not bool(torch.isfinite(q.scales.cpu()).all())
+
+
+def ragged(n, most, rows, seed):
+    """Lengths and rows of ``n`` sequences: empty ones, single tokens, long ones, in no order."""
+    g = torch.Generator().manual_seed(seed)
+    sizes = torch.randint(0, rows + 1, (n,), generator=g).tolist()
+    lens = [s + (int(torch.randint(0, most, (1,), generator=g)) if i % 3 else 0) for i, s in enumerate(sizes)]
+    return sizes, [max(a, 1) for a in lens]
+
 
 def tile_parts(total, workers):
     """The line of ``total`` tiles as the tensor-core kernels cut it (integer arithmetic of the kernels)."""

@@ -79,3 +79,54 @@ def test_the_merge_reads_what_the_workers_leave(per):
         parts = [p for p in cases.tile_parts(sum(tiles), blocks * per) if p[1]]
         assert parts[0][0] == 0 and parts[-1][1] == sum(tiles) and all(a < b for a, b in parts) and all(p[1] == q[0] for p, q in zip(parts, parts[1:]))
         assert cases.written_parts(tiles, blocks, per) == cases.merged_parts(tiles, blocks, per)
+
+
+def test_products_of_overlapping_rows():
+    cases.check_int4_overlapping_rows(TORCH_OPS, "cpu")
+
+
+def test_quantise_weights_that_are_not_finite():
+    cases.check_quant_int4_not_finite(TORCH_OPS, "cpu")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    try:
+        from kotodama_b200.ops import _build
+        return _build.load()
+    except Exception as e:                                   # no compiler and no built library
+        pytest.skip(f"native library unavailable: {e}")
+
+
+def test_launchers_refuse_bad_arguments(lib):
+    """Refused on the host, before any pointer is looked at."""
+    import ctypes
+    from kotodama_b200.ops.cuda import _ARGS, _CTYPE
+    P = 4096
+
+    def call(name, good, **bad):
+        names = list(good)
+        assert len(names) == len(_ARGS[name])
+        f = getattr(lib, name)
+        f.argtypes = [_CTYPE[c] for c in _ARGS[name]] + [ctypes.c_void_p, ctypes.c_void_p]
+        status = bad.pop("status", P)
+        return f(*[{**good, **bad}[n] for n in names], status, None)
+
+    app = dict(k=P, v=P, ks=128, vs=128, kc=P, ke=P, vc=P, ve=P, slots=P, N=4, n_kv=2, hd=64, slots_n=64, type=0)
+    for bad in (dict(N=0), dict(n_kv=0), dict(hd=24), dict(hd=272), dict(hd=0), dict(ks=4), dict(vs=129), dict(slots_n=-1), dict(type=2), dict(type=-1),
+                dict(k=P + 8), dict(v=P + 2), dict(kc=P + 8), dict(vc=P + 1), dict(N=2 ** 30, n_kv=4)):
+        assert call("kb_kv_append_fp8", app, **bad) == 5, bad
+    gat = dict(kc=P, ke=P, vc=P, ve=P, G=2, hd=64, table=P, B=1, width=4, pages=8, seq=P, first=P, cu=P, segs=1, k=P, v=P, total=4, type=0)
+    for bad in (dict(G=0), dict(hd=8), dict(hd=264), dict(B=0), dict(segs=0), dict(total=0), dict(type=3), dict(kc=P + 4), dict(k=P + 16), dict(v=P + 2)):
+        assert call("kb_kv_gather_fp8", gat, **bad) == 5, bad
+    tree = dict(q=P, qs=256, k=P, ke=None, v=P, ve=None, table=P, width=4, pages=8, lens=P, cu=None, B=2, masks=None, out=P, outs=256, N=2, H=4, n_kv=2, hd=64,
+                max_q=1, max_ctx=64, scale=0.125, zero=0)
+    for bad in (dict(ke=P), dict(ve=P), dict(hd=40), dict(hd=272), dict(H=3), dict(B=0), dict(N=0), dict(width=0), dict(pages=0), dict(type=2)):
+        assert call("kb_tree_attn_plain", dict(tree, type=0), **bad) == 5, bad
+    for bad in (dict(ke=P), dict(ve=P), dict(hd=80), dict(hd=32), dict(H=3), dict(B=0), dict(N=0), dict(width=0), dict(pages=0), dict(scale=0.0), dict(scale=-1.0),
+                dict(scale=float("nan")), dict(qs=252), dict(outs=254), dict(q=P + 8), dict(k=P + 8), dict(out=P + 4), dict(work=P + 8), dict(floats=0),
+                dict(max_q=0), dict(max_ctx=0), dict(pages=2 ** 31 - 1), dict(status=None)):
+        assert call("kb_tree_attn", dict(tree, work=P, floats=2 ** 40), **bad) != 0, bad
+    prod = dict(x=P, xs=128, packed=P, scales=P, c=None, cs=0, y=P, ys=64, M=4, N=64, K=128, group=128)
+    for bad in (dict(M=0), dict(N=0), dict(K=0), dict(K=12), dict(group=32), dict(group=256), dict(xs=4), dict(x=P + 8), dict(packed=P + 4), dict(scales=P + 2)):
+        assert call("kb_gemm_int4", prod, **bad) == 5, bad

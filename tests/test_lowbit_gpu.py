@@ -85,6 +85,41 @@ def test_tree_attention(case, fp8, dtype):
     get_ops("cuda").check_status()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("H,G,hd,n,most,rows", [(16, 4, 128, 45, 700, 3), (8, 2, 64, 200, 90, 1), (8, 1, 128, 30, 500, 20), (24, 2, 64, 21, 300, 64),
+                                                (12, 1, 128, 1, 9000, 64)])
+def test_ragged_batches(H, G, hd, n, most, rows, fp8):
+    """Many sequences per block of threads and many blocks per sequence, empty ones among them, on both tensor-core kernels."""
+    sizes, lens = cases.ragged(n, most, rows, 7 * n + rows) if n > 1 else ([rows], [most])
+    guarded(lambda ops: cases.check_tree(ops, "cuda", H, G, hd, sizes, lens, fp8, torch.bfloat16, rows > 1))
+    get_ops("cuda").check_status()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_calls_that_take_the_plain_kernel(fp8):
+    """More sequences than the tensor-core kernels' lists hold, scales that are not positive, query and output rows that are not aligned."""
+    ops = get_ops("cuda")
+    guarded(lambda ops: cases.check_tree(ops, "cuda", 2, 1, 64, [1] * 1100, [1 + i % 37 for i in range(1100)], fp8, torch.bfloat16, False))
+    c = cases.tree_case(4, 2, 64, [3, 2], [40, 9], fp8, torch.bfloat16, 3)
+    dense = [cases._dense(c[n]) for n in ("k", "v")]
+    for scale in (0.0, -0.25):
+        want, mass = cases.plain_tree(c["q"], *dense, c["table"].tolist(), c["lens"], c["cu"], scale, None)
+        err = (cases.run_tree(ops, "cuda", c, None, scale).cpu().double().view(5, 4, 64) - want).abs()
+        assert bool((err <= cases.tree_tolerance(c, want, mass, abs(scale))).all())
+    good = cases.run_tree(ops, "cuda", c, None, 0.125)
+    want, mass = cases.plain_tree(c["q"], *dense, c["table"].tolist(), c["lens"], c["cu"], 0.125, None)
+    room = torch.zeros(5, 4 * 64 + 1, device="cuda", dtype=torch.bfloat16)
+    room[:, 1:] = c["q"].view(5, -1).cuda()
+    odd = torch.zeros(5, 4 * 64 + 1, device="cuda", dtype=torch.bfloat16)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    args = (cases._put(c["k"], "cuda"), cases._put(c["v"], "cuda"), c["table"].cuda(), t(c["lens"]), t(c["cu"]), 3, 40, 0.125)
+    a = ops.paged_tree_attention(room[:, 1:].view(5, 4, 64), *args)
+    ops.paged_tree_attention(c["q"].cuda(), *args, None, odd[:, 1:])
+    for got in (good, a, odd[:, 1:]):
+        assert bool(((got.cpu().double().view(5, 4, 64) - want).abs() <= cases.tree_tolerance(c, want, mass, 0.125)).all())
+    ops.check_status()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("hd", [64, 128])
@@ -114,6 +149,31 @@ def test_products_with_4_bit_weights(case):
     M, N, K, group, stride = case
     guarded(lambda ops: cases.check_int4(ops, "cuda", torch.bfloat16, M, N, K, group, stride=stride))
     get_ops("cuda").check_status()
+
+
+@pytest.mark.parametrize("case", cases.INT4_LARGE_CASES, ids=str)
+def test_products_in_every_form(case):
+    M, N, K, group, stride = case
+    guarded(lambda ops: cases.check_int4(ops, "cuda", torch.bfloat16, M, N, K, group, stride=stride))
+    get_ops("cuda").check_status()
+
+
+def test_products_of_overlapping_rows():
+    guarded(lambda ops: cases.check_int4_overlapping_rows(ops, "cuda"))
+
+
+def test_quantise_weights_that_are_not_finite():
+    cases.check_quant_int4_not_finite(get_ops("cuda"), "cuda")
+
+
+def test_one_token_repeats_bit_by_bit():
+    """A token's result does not depend on the tokens beside it within a form, nor on the run."""
+    ops = get_ops("cuda")
+    x, w = cases.int4_case(64, 272, 4160, 64, 2)
+    x, w = x.cuda(), Int4Weight(w.packed.cuda(), w.scales.cuda(), w.shape, w.group)
+    for rows in ((8, 1), (16, 9), (32, 17), (64, 33)):
+        full = ops.gemm_nt(x[: rows[0]], w)
+        assert torch.equal(ops.gemm_nt(x[: rows[0]], w), full) and torch.equal(ops.gemm_nt(x[: rows[1]], w), full[: rows[1]])
 
 
 # ------------------------------------------------------------------ refusals
