@@ -87,18 +87,17 @@ def plain_int4(weight: Int4Weight):
     w = torch.zeros(-(-N // 16) * 16, -(-K // 64) * 64, dtype=F64)
     c = torch.zeros_like(w)
     nibble = {(0, 0): 0, (0, 1): 4, (0, 2): 2, (0, 3): 6, (1, 0): 1, (1, 1): 5, (1, 2): 3, (1, 3): 7}
-    for tile in range(words.shape[0]):
-        for half in range(2):
-            for r in range(8):
-                for lane in range(4):
-                    for j in range(4):
-                        for i in range(4):
-                            k = torch.arange(words.shape[1]) * 64 + 16 * lane + 4 * j + i
-                            code = (words[tile, :, 4 * r + lane, j] >> (4 * nibble[half, i])) & 15
-                            n = tile * 16 + half * 8 + r
-                            g = (k // weight.group).clamp_max(scales.shape[1] - 1)
-                            c[n, k] = code.to(F64)
-                            w[n, k] = (code.to(F64) - 8) * scales[tile, g, r, half]
+    n = torch.arange(words.shape[0])[:, None] * 16                     # all row tiles at once
+    for half in range(2):
+        for r in range(8):
+            for lane in range(4):
+                for j in range(4):
+                    for i in range(4):
+                        k = torch.arange(words.shape[1]) * 64 + 16 * lane + 4 * j + i
+                        code = (words[:, :, 4 * r + lane, j] >> (4 * nibble[half, i])) & 15
+                        g = (k // weight.group).clamp_max(scales.shape[1] - 1)
+                        c[n + half * 8 + r, k] = code.to(F64)
+                        w[n + half * 8 + r, k] = (code.to(F64) - 8) * scales[:, g, r, half]
     return w[:N, :K], c
 
 
