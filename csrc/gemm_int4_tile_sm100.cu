@@ -70,7 +70,7 @@ struct Roles {
     static constexpr int AC = TN > 64 ? 64 : 32;       // columns of a flush thread
     static constexpr int FLUSH = 4 * (TN / AC), WIDEN = 8, W_WIDEN = FLUSH, W_X = FLUSH + WIDEN, W_MMA = W_X + 1, THREADS = 32 * (W_MMA + 1);
     static constexpr int BLOCK = TN * 128;             // a block of 64 inputs of the tokens
-    static constexpr int RING = TURNS * 2 * BLOCK, CODES = WIDEN * D * 2 * 512, SC = FLUSH * 32 * SCALES * 4;
+    static constexpr int RING = TURNS * 2 * BLOCK, CODES = 8 * D * 2 * 512, SC = FLUSH * 32 * SCALES * 4;
     static constexpr int SMEM = 1024 + RING + CODES + SC;
     static constexpr int SETS = 2, SET = TN * (2 / PG);                // accumulators: sets, columns of a set (the groups of a turn)
     static_assert(TN * PITCH * 4 <= RING, "the partial sums take the ring's place");
@@ -140,32 +140,38 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
 #pragma unroll 1
         for (int i = 0; i < turns; ++i) {
             const int set = i % R::SETS;
-            ok = tc::mbar_wait(&acc_full[set], (uint32_t)(i / R::SETS) & 1u, abort_flag);
-            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-            tc::tc_fence_after();
+            float2 f[G];
 #pragma unroll
             for (int h = 0; h < G; ++h) {
-                if (h && i * G + h >= n_groups) break;
                 const int g = i * G + h;
                 copy_wait<SCALES - 2>();
                 const uint32_t both = ld_shared(slots + (g % SCALES) * (R::FLUSH * 128));              // (rows that do not exist: anything)
                 fetch(g + SCALES - 1);
-                const float f1 = __uint_as_float(row & 8 ? both & 0xffff0000u : both << 16) * unit;
-                const float2 f2 = make_float2(f1, f1);
+                f[h].x = f[h].y = __uint_as_float(row & 8 ? both & 0xffff0000u : both << 16) * unit;
+            }
+            ok = tc::mbar_wait(&acc_full[set], (uint32_t)(i / R::SETS) & 1u, abort_flag);
+            if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            tc::tc_fence_after();
+            const bool both = G == 1 || i * G + 1 < n_groups;          // the last turn may have one group
+#pragma unroll
+            for (int h = 0; h < G; ++h) {
+                if (h && !both) break;
 #pragma unroll
                 for (int e0 = 0; e0 < R::AC; e0 += PIECE) {
                     uint32_t v[PIECE];
                     if constexpr (PIECE == 32) tc::tmem_ld32(src + set * R::SET + h * TN + e0, v);
                     else tc::tmem_ld16(src + set * R::SET + h * TN + e0, v);
                     tc::tmem_ld_wait();
+                    if (e0 + PIECE == R::AC && (h == G - 1 || !both)) {
+                        tc::tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) tc::mbar_arrive(&acc_empty[set]);
+                    }
 #pragma unroll
                     for (int e = 0; e < PIECE / 2; ++e)
-                        acc[e0 / 2 + e] = __ffma2_rn(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), f2, acc[e0 / 2 + e]);
+                        acc[e0 / 2 + e] = __ffma2_rn(make_float2(__uint_as_float(v[2 * e]), __uint_as_float(v[2 * e + 1])), f[h], acc[e0 / 2 + e]);
                 }
             }
-            tc::tc_fence_before();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&acc_empty[set]);
         }
         copy_wait<0>();
         if (!ok && lane == 0) atomicMax(status, (int)KB_TIMEOUT_EPI);
@@ -185,17 +191,17 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
         }
     } else if (warp < R::W_X) {
         // ------------------------------------------------------------ codes -> operand
+        constexpr int U = 2;                           // blocks of a turn
         const int w = warp - R::W_WIDEN, first = (w & 3) * 2 + (w >> 2);               // the tile's place among eight; a warp reaches lanes 32 (w % 4) ..
         const int r = lane >> 2, q = lane & 3, ex = r >> 1;
-        constexpr int TURN = 2 * 512;                  // bytes of a turn: [block][32 lanes of 16]
+        constexpr int TURN = U * 512;                  // bytes of a turn: [block][32 lanes of 16]
         const uint32_t codes = smem_u32(ring + R::RING) + w * (D * TURN);
         const uint32_t put = codes + (lane ^ ex) * 16, get = codes + (4 * r + ex) * 16 + q * 4;        // ex: two bits, of the place in the row
         const uint4* src = packed + ((long long)min(n0 / 16 + first, s.nt - 1) * s.kb + b0) * 32 + lane;       // (rows behind the last: not stored)
         auto fetch = [&](int i) {
-            if (i < turns) {
-                copy16(put + (i % D) * TURN, src + (long long)i * 64);
-                if (2 * i + 1 < nb) copy16(put + (i % D) * TURN + 512, src + (long long)i * 64 + 32);
-            }
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (i < turns && 2 * i + u < nb) copy16(put + (i % D) * TURN + u * 512, src + (long long)i * 64 + u * 32);
             copy_commit();
         };
 #pragma unroll
@@ -209,13 +215,13 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
             __syncwarp();                              // the words are other lanes' copies; and all have read the turn that is filled next
             fetch(i + D - 1);
             const uint32_t at = get + (i % D) * TURN;
-            uint32_t v[2][4], a[2][16];                // two blocks at once (of one behind the last: what its place held, read by no product)
+            uint32_t v[U][4], a[U][16];                // (of a block behind the last: what its place held, read by no product)
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) v[u][k] = ld_shared((at ^ (k * 16)) + u * 512);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     uint32_t e[4];
@@ -229,8 +235,8 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
             tc::tc_fence_after();
             const uint32_t dst = tmem_a + st * 64 + ((uint32_t)(first * 16) << 16);
-            st_16x256_x4(dst, a[0]);
-            st_16x256_x4(dst + 32, a[1]);
+#pragma unroll
+            for (int u = 0; u < U; ++u) st_16x256_x4(dst + u * 32, a[u]);
             tc::tmem_st_wait();
             tc::tc_fence_before();
             __syncwarp();
