@@ -58,6 +58,11 @@ struct Int4Smem {
     float part[2][W][RT * 16][TT * 8 + 1];
 };
 
+template <int N>
+struct Tiles {
+    static constexpr int value = N;
+};
+
 // A block of threads owns an even share of the row tiles, taken up to RT at a time; its warps share the groups of inputs.
 template <int TT, int RT, int PG, int W, int D>
 __global__ void __launch_bounds__(W * 32, 1)
@@ -157,58 +162,65 @@ int4_kernel(const bf16* __restrict__ x, const uint4* __restrict__ packed, const 
             for (int j = 0; j < TT; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[t][j][i] = 0.f;
+        // T tiles of the step, without a branch among them
+        auto walk = [&](auto tiles) {
+            constexpr int T = decltype(tiles)::value;
 #pragma unroll 1
-        for (int b = b0; b < b1; b += PG) {
-            float d[RT][TT][4];
+            for (int b = b0; b < b1; b += PG) {
+                float d[T][TT][4];
 #pragma unroll
-            for (int i = 0; i < PG; ++i) {
-                if (i && b + i >= b1) break;           // (then the last group has one block: b1 is the end of the row)
-                copy_wait<D - 2>();
-                __syncwarp();                          // the copies are all lanes'; and all have read the slot that is filled next
-                if (ahead.tile < t1) {
-                    copy_w(ahead);
-                    copy_x(ahead);
-                    next(ahead);
-                }
-                copy_commit();
-                const Stage& st = *reinterpret_cast<const Stage*>(reinterpret_cast<const unsigned char*>(&sm.ring[warp][0]) + slot);
-                uint4 xb[TT][2];
-#pragma unroll
-                for (int j = 0; j < TT; ++j)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) xb[j][h] = st.x[(j * 8 + r) * 8 + ((2 * qd + h) ^ r)];
-                const bool last = i == PG - 1 || b + i + 1 == b1;
-#pragma unroll
-                for (int t = 0; t < RT; ++t) {         // (up to three: all of them, whatever their stage held before)
-                    if (RT > 3 && t && t >= cnt) break;
-                    const uint4 v = st.w[t * 32 + lane];
-                    uint32_t a[4];
-                    expand(v.x, a);
+                for (int i = 0; i < PG; ++i) {
+                    if (i && b + i >= b1) break;           // (then the last group has one block: b1 is the end of the row)
+                    copy_wait<D - 2>();
+                    __syncwarp();                          // the copies are all lanes'; and all have read the slot that is filled next
+                    if (ahead.tile < t1) {
+                        copy_w(ahead);
+                        copy_x(ahead);
+                        next(ahead);
+                    }
+                    copy_commit();
+                    const Stage& st = *reinterpret_cast<const Stage*>(reinterpret_cast<const unsigned char*>(&sm.ring[warp][0]) + slot);
+                    uint4 xb[TT][2];
 #pragma unroll
                     for (int j = 0; j < TT; ++j)
-                        if (i) mma_bf16(d[t][j], a, xb[j][0].x, xb[j][0].y);
-                        else mma_bf16_first(d[t][j], a, xb[j][0].x, xb[j][0].y);
-                    expand(v.y, a);
 #pragma unroll
-                    for (int j = 0; j < TT; ++j) mma_bf16(d[t][j], a, xb[j][0].z, xb[j][0].w);
-                    expand(v.z, a);
+                        for (int h = 0; h < 2; ++h) xb[j][h] = st.x[(j * 8 + r) * 8 + ((2 * qd + h) ^ r)];
+                    const bool last = i == PG - 1 || b + i + 1 == b1;
 #pragma unroll
-                    for (int j = 0; j < TT; ++j) mma_bf16(d[t][j], a, xb[j][1].x, xb[j][1].y);
-                    expand(v.w, a);
-#pragma unroll
-                    for (int j = 0; j < TT; ++j) mma_bf16(d[t][j], a, xb[j][1].z, xb[j][1].w);
-                    if (last) {
-                        const uint32_t sc = st.sc[t * 8 + r];
-                        const float s0 = __uint_as_float(sc << 16), s1 = __uint_as_float(sc & 0xffff0000u);
+                    for (int t = 0; t < T; ++t) {
+                        const uint4 v = st.w[t * 32 + lane];
+                        uint32_t a[4];
+                        expand(v.x, a);
 #pragma unroll
                         for (int j = 0; j < TT; ++j)
+                            if (i) mma_bf16(d[t][j], a, xb[j][0].x, xb[j][0].y);
+                            else mma_bf16_first(d[t][j], a, xb[j][0].x, xb[j][0].y);
+                        expand(v.y, a);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) acc[t][j][e] = fmaf(e < 2 ? s0 : s1, d[t][j][e], acc[t][j][e]);
+                        for (int j = 0; j < TT; ++j) mma_bf16(d[t][j], a, xb[j][0].z, xb[j][0].w);
+                        expand(v.z, a);
+#pragma unroll
+                        for (int j = 0; j < TT; ++j) mma_bf16(d[t][j], a, xb[j][1].x, xb[j][1].y);
+                        expand(v.w, a);
+#pragma unroll
+                        for (int j = 0; j < TT; ++j) mma_bf16(d[t][j], a, xb[j][1].z, xb[j][1].w);
+                        if (last) {
+                            const uint32_t sc = st.sc[t * 8 + r];
+                            const float s0 = __uint_as_float(sc << 16), s1 = __uint_as_float(sc & 0xffff0000u);
+#pragma unroll
+                            for (int j = 0; j < TT; ++j)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) acc[t][j][e] = fmaf(e < 2 ? s0 : s1, d[t][j][e], acc[t][j][e]);
+                        }
                     }
+                    slot = slot == (D - 1) * sizeof(Stage) ? 0 : slot + (uint32_t)sizeof(Stage);
                 }
-                slot = slot == (D - 1) * sizeof(Stage) ? 0 : slot + (uint32_t)sizeof(Stage);
             }
-        }
+        };
+        // a last step of fewer tiles than three: so many; else all, whatever the stage of one that is not there held before
+        if (RT > 2 && cnt == 1) walk(Tiles<1>());
+        else if (RT > 3 && cnt == 2) walk(Tiles<(RT > 2 ? 2 : 1)>());
+        else walk(Tiles<RT>());
 #pragma unroll
         for (int t = 0; t < RT; ++t) {
 #pragma unroll
