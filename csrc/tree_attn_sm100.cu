@@ -618,14 +618,16 @@ namespace {
 struct Plan {
     int rows, tile, grid, workers, per_cta, merge_warps;
 };
-// Which kernel, and how many CTAs: as many as there are tiles for, at most what fits the GPU at once.  More than 16 query rows per KV head
-// take the 128-row kernel: measured at 64 sequences over 2048 tokens with 32 rows, 8-bit / bf16 pages, 164 / 110 us against 200 / 215 us for
-// tiles of 32 rows here; with 16 rows 157 / 104 us against 75 / 84 us for the 16-row kernel.
-// The merge walks a unit's parts with one warp per row where there are about eight of them, else with 8 or 32.
+// Which kernel, and how many CTAs: as many as there are tiles for, at most what fits the GPU at once.  The 128-row kernel pays for 128 rows
+// whatever there are, this one for units of 16 rows, of which each reads the keys and values again.  Measured (us, this kernel / the 128-row one), 64
+// sequences over 2048 tokens, four query heads per KV head, rows per KV head 16 / 32 / 48 / 64: 8-bit pages 64 / 158, 98 / 165, 141 / 172, 178 / 179;
+// bf16 pages 89 / 114, 139 / 120, -, 237 / 136.  So: up to 48 rows on 8-bit pages, up to 16 on bf16 pages.
+// The merge walks a unit's parts with one warp per row where there are about eight of them, else with 8 or 32: (us, 1 / 8 / 32 warps) one token of 64
+// sequences over 2048 tokens 52 / 59 / 98, one of one sequence over 4000 tokens 20 / 13 / 14, of four over 8000 35 / 30 / 30.
 Plan plan_for(int B, int N, int n_kv, int G, int hd, int max_q, int max_ctx, bool fp8) {
     Plan pl;
     const int most_rows = max_q * G;
-    pl.rows = most_rows <= 16 ? 16 : 128;
+    pl.rows = most_rows <= (fp8 ? 48 : 16) ? 16 : 128;
     pl.tile = pl.rows == 128 ? 128 : fp8 || hd == 64 ? 32 : 16;
     const long long blocks = B + (long long)N * G / pl.rows;                            // units per KV head, at most
     const long long one = (most_rows + pl.rows - 1) / pl.rows;

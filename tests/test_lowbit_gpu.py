@@ -86,7 +86,7 @@ def test_tree_attention(case, fp8, dtype):
 
 
 @pytest.mark.parametrize("fp8", [False, True])
-@pytest.mark.parametrize("H,G,hd,n,most,rows", [(16, 4, 128, 45, 700, 3), (8, 2, 64, 200, 90, 1), (8, 1, 128, 30, 500, 20), (24, 2, 64, 21, 300, 64),
+@pytest.mark.parametrize("H,G,hd,n,most,rows", [(16, 4, 128, 45, 700, 3), (8, 2, 64, 200, 90, 1), (8, 1, 128, 30, 500, 20), (24, 2, 64, 21, 300, 64), (12, 4, 128, 25, 600, 13),
                                                 (12, 1, 128, 1, 9000, 64)])
 def test_ragged_batches(H, G, hd, n, most, rows, fp8):
     """Many sequences per block of threads and many blocks per sequence, empty ones among them, on both tensor-core kernels."""
