@@ -8,6 +8,11 @@
 // directions exact up to the one rounding of the code: scaling by it rounds nothing, and code * 2^e has four significant bits,
 // which bf16 holds.  A row that holds an infinity or a NaN is stored as exponent 255 with NaN codes; it reads back as NaN.
 // Compiled without fast-math (denormal results are kept).
+//
+// Append is bound by instructions (about 100 per warp and two rows of 128 each of keys and values; 8191 tokens x 8 heads x 128: 10.7 us, 4.7 TB/s; the 50 MB would take 7.8), since a
+// row's largest magnitude is needed before its first code; two bf16 magnitudes share a word on the way (one at a time: 22 us).  The rows are
+// fetched beside their slot: the two loads' latencies do not add up.  Reading back is bound by the memory: 16 x 4096 tokens x 8 heads x 128 in
+// 50.7 us, 6.1 TB/s (66 us with 16-byte stores).
 #include <cuda_fp8.h>
 
 #include "vec.cuh"
@@ -88,8 +93,8 @@ __device__ __forceinline__ uint2 largest(const Piece<float>& k, const Piece<floa
 }
 
 // LANES (a power of two, at least hd / 8) lanes share a (token, kv head): its row of keys and its row of values, eight elements of each per
-// lane.  U of them per lane group are loaded before the first is used.
-template <typename T, int LANES, int U>
+// lane.  (Two of them per lane group: 12.2 us against 10.7 for 8191 tokens, 2.6 against 1.8 for 64.)
+template <typename T, int LANES>
 __global__ void __launch_bounds__(THREADS)
 append_kernel(const T* __restrict__ k, const T* __restrict__ v, const AppendShape s, uint8_t* __restrict__ kc, uint8_t* __restrict__ ke,
               uint8_t* __restrict__ vc, uint8_t* __restrict__ ve, const long long* __restrict__ slots, int* __restrict__ status) {
@@ -97,49 +102,41 @@ append_kernel(const T* __restrict__ k, const T* __restrict__ v, const AppendShap
     kb_dep_wait();
     constexpr int GROUPS = THREADS / LANES;
     const int sub = threadIdx.x % LANES;
-    const uint32_t rows = (uint32_t)s.N * s.n_kv, base = blockIdx.x * (GROUPS * U) + threadIdx.x / LANES;
+    const uint32_t r = blockIdx.x * GROUPS + threadIdx.x / LANES;
     const bool mine = sub * 8 < s.hd;
-    Piece<T> x[U], y[U];
-    long long at[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint32_t r = base + u * GROUPS;
-        at[u] = -1;
-        x[u].zero();
-        y[u].zero();
-        if (r < rows) {
-            const uint32_t n = r / s.n_kv, head = r - n * s.n_kv;
-            const long long slot = slots[n];
-            if (mine) {                                // (the rows are fetched beside their slot, not behind it)
-                const uint32_t col = head * s.hd + sub * 8;
-                x[u].load(k + n * s.k_stride + col);
-                y[u].load(v + n * s.v_stride + col);
-            }
-            if (slot >= s.num_slots) {
-                if (head == 0 && sub == 0 && status) atomicMax(status, (int)KB_BAD_INDEX);
-            } else if (slot >= 0) {
-                at[u] = (((unsigned long long)slot / PAGE) * s.n_kv + head) * PAGE + (slot & (PAGE - 1));
-            }
+    Piece<T> x, y;
+    x.zero();
+    y.zero();
+    long long at = -1;
+    if (r < (uint32_t)s.N * s.n_kv) {
+        const uint32_t n = r / s.n_kv, head = r - n * s.n_kv;
+        const long long slot = slots[n];
+        if (mine) {                                    // (the rows are fetched beside their slot, not behind it)
+            const uint32_t col = head * s.hd + sub * 8;
+            x.load(k + n * s.k_stride + col);
+            y.load(v + n * s.v_stride + col);
+        }
+        if (slot >= s.num_slots) {
+            if (head == 0 && sub == 0 && status) atomicMax(status, (int)KB_BAD_INDEX);
+        } else if (slot >= 0) {
+            at = (((unsigned long long)slot / PAGE) * s.n_kv + head) * PAGE + (slot & (PAGE - 1));
         }
     }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-        const uint2 m = largest<LANES>(x[u], y[u]);
-        if (at[u] < 0) continue;
-        // 448 = 1.75 * 2^8: the exponent is that of the magnitude less 8, one more where its mantissa is above 1.75
-        const int e = min(max((int)(m.x >> 23) - 8 + ((m.x & 0x7fffffu) > 0x600000u), 1), 254);
-        const int f = min(max((int)(m.y >> 23) - 8 + ((m.y & 0x7fffffu) > 0x600000u), 1), 254);
-        const bool bad = m.x >= 0x7f800000u, worse = m.y >= 0x7f800000u;
-        if (mine) {
-            const uint2 c = x[u].codes(pow2(254 - e)), d = y[u].codes(pow2(254 - f)), nan = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-            const long long to = at[u] * s.hd + sub * 8;
-            *reinterpret_cast<uint2*>(kc + to) = bad ? nan : c;
-            *reinterpret_cast<uint2*>(vc + to) = worse ? nan : d;
-        }
-        if (sub == 0) {
-            ke[at[u]] = (uint8_t)(bad ? 255 : e);
-            ve[at[u]] = (uint8_t)(worse ? 255 : f);
-        }
+    const uint2 m = largest<LANES>(x, y);
+    if (at < 0) return;
+    // 448 = 1.75 * 2^8: the exponent is that of the magnitude less 8, one more where its mantissa is above 1.75
+    const int e = min(max((int)(m.x >> 23) - 8 + ((m.x & 0x7fffffu) > 0x600000u), 1), 254);
+    const int f = min(max((int)(m.y >> 23) - 8 + ((m.y & 0x7fffffu) > 0x600000u), 1), 254);
+    const bool bad = m.x >= 0x7f800000u, worse = m.y >= 0x7f800000u;
+    if (mine) {
+        const uint2 c = x.codes(pow2(254 - e)), d = y.codes(pow2(254 - f)), nan = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+        const long long to = at * s.hd + sub * 8;
+        *reinterpret_cast<uint2*>(kc + to) = bad ? nan : c;
+        *reinterpret_cast<uint2*>(vc + to) = worse ? nan : d;
+    }
+    if (sub == 0) {
+        ke[at] = (uint8_t)(bad ? 255 : e);
+        ve[at] = (uint8_t)(worse ? 255 : f);
     }
 }
 
@@ -234,13 +231,9 @@ template <typename T, int LANES>
 int launch_append(const void* k, const void* v, const AppendShape& s, void* kc, void* ke, void* vc, void* ve, const long long* slots,
                   int* status, cudaStream_t st) {
     const long long rows = (long long)s.N * s.n_kv, groups = THREADS / LANES;
-    if (rows > 0x7fffffffll - 2 * groups) return 5;
-    // two per lane group once that still fills the GPU with warps
-    if (rows >= 148ll * 8 * groups * 2)
-        return kb_launch_dep(append_kernel<T, LANES, 2>, dim3((unsigned)((rows + groups * 2 - 1) / (groups * 2))), dim3(THREADS), 0, st, (const T*)k,
-                             (const T*)v, s, (uint8_t*)kc, (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, slots, status);
-    return kb_launch_dep(append_kernel<T, LANES, 1>, dim3((unsigned)((rows + groups - 1) / groups)), dim3(THREADS), 0, st, (const T*)k,
-                         (const T*)v, s, (uint8_t*)kc, (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, slots, status);
+    if (rows > 0x7fffffffll - groups) return 5;
+    return kb_launch_dep(append_kernel<T, LANES>, dim3((unsigned)((rows + groups - 1) / groups)), dim3(THREADS), 0, st, (const T*)k, (const T*)v, s,
+                         (uint8_t*)kc, (uint8_t*)ke, (uint8_t*)vc, (uint8_t*)ve, slots, status);
 }
 
 template <typename T>

@@ -1,16 +1,21 @@
 // Products with 4-bit weights: y[M, N] = x[M, K] . w[N, K]^T (+ c), w[n, k] = scale[n, k / group] * (code[n, k] - 8), group 64 or 128.
 //
-// Mathematics.  Codes become bf16 numbers c - 8 (exact): 128 + c is one mask and one or of the packed word (0x4300 | nibble), minus 136.
-// The products of a group are summed in fp32 by the tensor cores, then times the group's scale in fp32 added to the result, so nothing is
-// rounded but the result.
+// Mathematics.  Codes become bf16 numbers (code - 8) times a power of two, exactly (codes4.cuh).  The products of a group are summed in fp32 by
+// the tensor cores, then times the group's scale in fp32 added to the result, so nothing is rounded but the result.
 //
 // Layout.  `mma.m16n8k16` with the weights as the 16-row operand and up to eight tokens as columns.  512 contiguous bytes are 16 rows x
 // 64 inputs in the order of the fragments: a lane's 16 bytes hold, for the rows lane / 4 and lane / 4 + 8, the inputs 16 (lane % 4) .. + 15 of the
-// block, four per word and k step - so the activations of a lane's fragments are 16 consecutive numbers of a row of x, two
-// 16-byte loads (the order of inputs inside a product is free as long as both operands have it).
+// block, four per word and k step - so the activations of a lane's fragments are 16 consecutive numbers of a row of x (the order of inputs
+// inside a product is free as long as both operands have it).
 //
-// What bounds it: the weights' bytes.  A block owns RT * 16 rows; its eight warps share the K range, so that even a narrow weight keeps
-// all SMs loading; a warp has four blocks of 512 bytes per row tile in flight while it works on the four before.
+// This file: up to 16 tokens (more: gemm_int4_tile_sm100.cu).  One block of threads per SM owns an even share of the row tiles; its warps share the
+// groups of inputs and meet in shared memory once per step of up to four tiles.  Every warp streams its blocks - a block of each tile, the tokens' inputs
+// for them, the scales - through a ring of its own by 16-byte asynchronous copies, across the steps, so that no load waits for arithmetic.
+//
+// What bounds it: instructions.  Of about 80 per 512 bytes 36 widen the codes, 4 multiply; the rest is copies, addresses, sums.  At 8 x 28672 x 4096
+// the schedulers issue in 56 % of the cycles and the ALU is half busy (18 us, 3.4 TB/s); the 64 MB alone would take 9.5 us.  Tried: registers instead
+// of the ring (23 us: fewer loads in flight), x straight from the L1 cache (27 us: it does not fit beside the rings), more and smaller
+// blocks of threads (20 to 25 us), 8 warps (20 us).
 #include <stddef.h>
 
 #include "codes4.cuh"
@@ -274,7 +279,10 @@ KB_API int kb_gemm_int4(const void* x, long long x_stride, const void* packed, c
 #define INT4_RUN(TT, RT, W, D)                                                                                                                \
     return group == 64 ? run_int4<TT, RT, 1, W, D>((const bf16*)x, (const uint4*)packed, (const uint32_t*)scales, (const bf16*)c, (bf16*)y, s, sms, st) \
                        : run_int4<TT, RT, 2, W, D>((const bf16*)x, (const uint4*)packed, (const uint32_t*)scales, (const bf16*)c, (bf16*)y, s, sms, st)
-    // as many row tiles at once as a block owns, up to four
+    // As many row tiles at once as a block owns, up to four: they share the tokens' copies, and a step ends in a barrier and sums over the warps.  us at
+    // 8 tokens, K 4096, with 1 / 2 / 3 / 4 at once: N 4096 (two tiles a block) 5.8 / 4.9 / - / 4.9, N 6144 (three) 7.5 / 7.1 / 5.9 / 6.4, N 28672 (thirteen)
+    // 25.3 / 20.2 / 18.6 / 18.0.  16 tokens: the second half of the columns doubles the copies; 12 and 8 warps leave room for three and four tiles.
+    // More than 16 go to tcgen05: 16 tokens take 7.1 us here and 9.9 there at N 6144, 25 and 28 at N 28672; 32 tokens 13.3 and 10.2, 47 and 29.
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 7;
     const int per = (s.nt + sms - 1) / sms;

@@ -12,10 +12,16 @@
 // into just that.  For step k lane q takes word q of the packed lane k of its row, so that the operand has the inputs in x's order.  The words are
 // read from shared memory one by one; the copies' places there are exchanged (by the row's bits 1 and 2) so that no two meet in a bank.
 //
-// What bounds it is the issue of instructions (36 of a tile's block are the widening itself, 40 clocks of the ALU per scheduler).
+// What bounds it: the length of a turn's way from codes to sums, and instructions.  A turn of 64 tokens takes about 900 clocks, of which the products
+// need 256: each role works 500 to 600 and waits for another the rest of the time, with the schedulers issuing in 54 % of the cycles (64 x 4096 x 14336:
+// 18.2 us, of which the bytes would take 5.2).  At 1024 x 6144 x 4096 it reaches 910 TFLOP/s, 0.54 of the library's bf16 product, because
+// every group's sums go through registers once.  Tried: x by 8-byte copies in the order that the store gives (30 us: issuing them), 16 widening warps
+// (22 us), a barrier per operand (36 us at 64 x 28672 x 4096, 32 with one for both).  Weights widened into shared memory would move 48 KB through it
+// per block, 384 clocks.
+// Token tiles: up to 32, 64 or 128.  128 tokens x 6144 x 4096 take 14.5 us as one tile, 16.9 as two; 32 take 10.2 as a tile of 32, 11.6 of 64.
 //
-// Few row tiles: a cluster of up to eight CTAs shares the groups of a row tile and adds up through distributed shared memory, in
-// the order of the ranks.  All waits are bounded (status word on timeout).
+// Few row tiles: a cluster of up to eight CTAs shares the turns of a row tile and adds up through distributed shared memory, in
+// the order of the ranks (64 x 4096 x 14336: 46 us without).  All waits are bounded (status word on timeout).
 #include "attn_common.cuh"
 #include "codes4.cuh"
 

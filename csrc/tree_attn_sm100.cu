@@ -4,8 +4,8 @@
 // What bounds it.  A cached row is used by the (drafted token, query head) rows of its KV head only - 1 to a few hundred - so the
 // cache's bytes bound the call, and above ~100 rows the tensor cores do.  Each (sequence, KV head) has its n * G query rows as the
 // M side of `mma.sync.m16n8k16` tiles (16 of them per unit of work), cached tokens are the N side of the score product and the K side of
-// the output product; probabilities go from accumulators to operands in registers.  Calls with more than 16 rows per KV head take
-// tree_attn_tile_sm100.cu.
+// the output product; probabilities go from accumulators to operands in registers.  Calls with more rows per KV head
+// (`plan_for` below) take tree_attn_tile_sm100.cu.
 //
 // Work.  A unit is (sequence, KV head, block of rows); its tiles are TILE tokens of the context.  All units' tiles form one line
 // that is cut into equal parts, one per worker, so that ragged contexts and one long context load the GPU alike.  Here a worker is a
