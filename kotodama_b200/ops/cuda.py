@@ -110,6 +110,8 @@ class CudaOps(TorchOps):
             f = self._fns[fn] = getattr(self.lib, fn)
             f.argtypes = [_CTYPE[c] for c in _ARGS[fn]] + [_VP, _VP]
         dev = t.get_device()
+        if dev < 0:
+            raise KernelError(f"{fn}: the operands are not on a GPU")
         word = self._status_at.get(dev)
         if word is None:
             word = self._status_at[dev] = self.status(t.device).data_ptr()
@@ -730,7 +732,7 @@ class CudaOps(TorchOps):
     # ------------------------------------------------------------------ serving
     def kv_append(self, k, v, k_pages, v_pages, slots):
         """Copy rows ``k[n], v[n]`` (``[N, n_kv*hd]`` views) into cache slot ``slots[n]`` (page*16 + offset); with :class:`Fp8Pages`
-        quantised on the way (bf16 or fp32 rows)."""
+        quantised on the way (bf16 or fp32 rows).  Slots are distinct, negative ones are skipped."""
         if isinstance(k_pages, Fp8Pages):
             return self._kv_append_fp8(k, v, k_pages, v_pages, slots)
         N, row = k.shape

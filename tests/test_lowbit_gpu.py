@@ -252,6 +252,68 @@ def verification_step(ops, seed=0):
     return run, plain, [rand(12, D).bfloat16() for _ in range(3)]
 
 
+def test_operands_on_the_host_are_refused():
+    """They agree on their device, and it is not a GPU."""
+    ops = get_ops("cuda")
+    x, w = cases.int4_case(3, 32, 64, 64, 0)
+    with pytest.raises(KernelError, match="GPU"):
+        ops.gemm_nt(x, w)
+    c = cases.tree_case(2, 1, 64, [1], [3], True, torch.bfloat16, 0)
+    with pytest.raises(KernelError, match="GPU"):
+        cases.run_tree(ops, "cpu", c, None, 0.125)
+    with pytest.raises(KernelError, match="GPU"):
+        ops.kv_append(x, x, Fp8Pages.zeros(1, 1, 64, "cpu"), Fp8Pages.zeros(1, 1, 64, "cpu"), torch.arange(3))
+    i32 = lambda *a: torch.tensor(a, dtype=torch.int32)
+    with pytest.raises(KernelError, match="GPU"):
+        ops.kv_gather(c["k"], c["v"], i32(0)[None], i32(0), i32(0), i32(0, 2), 2)
+
+
+# ------------------------------------------------------------------ offsets beyond 32 bits
+@pytest.mark.parametrize("fp8", [False, True])
+def test_caches_of_more_than_4_gigabytes(fp8):
+    """The last pages of a large cache give what the pages of a small one give, bit by bit."""
+    ops = get_ops("cuda")
+    n_kv, hd, few, many = 8, 128, 6, 280_000 if fp8 else 140_000
+    assert many * n_kv * 16 * hd * (1 if fp8 else 2) > 1 << 32
+    g = torch.Generator(device="cuda").manual_seed(6)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=g).bfloat16()
+    k, v, slots = rand(90, n_kv * hd), rand(90, n_kv * hd), torch.randperm(few * 16, device="cuda", generator=g)[:90]
+    table = torch.tensor([[3, 0, 5], [1, 4, 2]], dtype=torch.int32, device="cuda")
+    t = lambda *a: torch.tensor(a, dtype=torch.int32, device="cuda")
+    got = []
+    for pages in (few, many):
+        at = pages - few
+        new = (lambda: Fp8Pages.zeros(pages, n_kv, hd, "cuda")) if fp8 else (lambda: torch.zeros(pages, n_kv, 16, hd, device="cuda", dtype=torch.bfloat16))
+        kp, vp = new(), new()
+        ops.kv_append(k, v, kp, vp, slots + at * 16)
+        out = list(ops.kv_gather(kp, vp, table + at, t(0, 1), t(2, 0), t(0, 44, 92), 92))
+        for H in (16, 64):                            # 6, 24, 24 and 96 rows per KV head
+            for rows in (3, 12):
+                q = torch.randn(2 * rows, H, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(H + rows)).bfloat16()
+                out.append(ops.paged_tree_attention(q, kp, vp, table + at, t(46, 33), t(0, rows, 2 * rows), rows, 48, 0.09))
+        got.append(out)
+        del kp, vp
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and bool((got[0][0] != 0).any())
+    ops.check_status()
+
+
+def test_weights_of_more_than_4_gigabytes():
+    """The last rows of a large weight give what they give alone."""
+    ops = get_ops("cuda")
+    N, K = 140_000, 65_536
+    g = torch.Generator(device="cuda").manual_seed(8)
+    packed = torch.randint(-2 ** 31, 2 ** 31 - 1, (N // 16, K // 64, 32, 4), device="cuda", dtype=torch.int32, generator=g)
+    scales = (torch.rand(N // 16, K // 128, 8, 2, device="cuda", generator=g) + 0.5).bfloat16()
+    assert packed.numel() * 4 > 1 << 32
+    whole, end = Int4Weight(packed, scales, (N, K), 128), Int4Weight(packed[-8:].clone(), scales[-8:].clone(), (128, K), 128)
+    for M in (4, 40):
+        x = torch.randn(M, K, device="cuda", generator=g).bfloat16()
+        a, b = ops.gemm_nt(x, whole)[:, -128:].double(), ops.gemm_nt(x, end).double()
+        # both round sums over 65536 inputs (fp32, in differing order) to bf16: half a step each
+        assert float((a - b).norm() / b.norm()) < 2 * 2.0 ** -8
+    ops.check_status()
+
+
 def test_verification_step():
     ops = get_ops("cuda")
     run, plain, xs = verification_step(ops)
