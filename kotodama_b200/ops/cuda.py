@@ -347,6 +347,8 @@ class CudaOps(TorchOps):
             good = good and c.shape in ((M, N), (1, N)) and c.dtype == dtype and c.stride(1) == 1 and c.device == dev
             c_stride = c.stride(0) if c.shape[0] > 1 else 0
         stride, inner = a.stride()
+        if M == 1:
+            stride = K
         if (not good or K != inputs or dtype != torch.bfloat16 or inner != 1 or stride % 8 or a.data_ptr() % 16 or packed.device != dev
                 or packed.data_ptr() % 16):
             raise KernelError(f"4-bit product: bf16 rows of {inputs} numbers, 16-byte aligned, got {tuple(a.shape)} {dtype} {a.stride()}; "
@@ -747,6 +749,8 @@ class CudaOps(TorchOps):
         N = k.shape[0]
         dtype = k.dtype
         (k_stride, k1), (v_stride, v1) = k.stride(), v.stride()
+        if N == 1:
+            k_stride = v_stride = n_kv * hd
         if (k.shape != (N, n_kv * hd) or v.shape != (N, n_kv * hd) or slots.shape != (N,) or dtype not in _TYPE or v.dtype != dtype
                 or k1 != 1 or v1 != 1 or slots.dtype != torch.int64 or not slots.is_contiguous() or v.device != k.device or slots.device != k.device):
             raise KernelError(f"8-bit cache append: rows {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}, slots {tuple(slots.shape)} "

@@ -162,6 +162,20 @@ def test_products_of_overlapping_rows():
     guarded(lambda ops: cases.check_int4_overlapping_rows(ops, "cuda"))
 
 
+def test_a_single_row_has_any_stride():
+    ops = get_ops("cuda")
+    x, w = cases.int4_case(1, 40, 136, 64, 3)
+    w = Int4Weight(w.packed.cuda(), w.scales.cuda(), w.shape, w.group)
+    row = x.cuda().as_strided((1, 136), (1001, 1))
+    assert torch.equal(ops.gemm_nt(row, w), ops.gemm_nt(x.cuda(), w))
+    got = []
+    for k in (x[:, :128].cuda(), row[:, :128]):
+        kp, vp = Fp8Pages.zeros(1, 2, 64, "cuda"), Fp8Pages.zeros(1, 2, 64, "cuda")
+        ops.kv_append(k, k, kp, vp, torch.tensor([7], device="cuda"))
+        got.append((kp.codes.view(torch.uint8), kp.exps, vp.codes.view(torch.uint8), vp.exps))
+    assert all(torch.equal(a, b) for a, b in zip(*got)) and bool(got[0][0][0, :, 7].any())
+
+
 def test_quantise_weights_that_are_not_finite():
     cases.check_quant_int4_not_finite(get_ops("cuda"), "cuda")
 
