@@ -101,22 +101,21 @@ class CudaOps(TorchOps):
     def _call(self, fn: str, *args) -> None:
         self._rc(getattr(self.lib, fn)(*args), fn)
 
-    def _launch(self, fn: str, t: torch.Tensor, *args) -> None:
+    def _launch(self, fn: str, dev: int, *args) -> None:
         """A launcher called with plain numbers and addresses (its argument types are declared in ``_ARGS``; the status word and the
-        stream follow), on the current stream of ``t``'s device.  Cheaper on the host than wrapping every argument: the smallest
+        stream follow), on the current stream of device ``dev``.  Cheaper on the host than wrapping every argument: the smallest
         operators are bound by it."""
         f = self._fns.get(fn)
         if f is None:
             f = self._fns[fn] = getattr(self.lib, fn)
             f.argtypes = [_CTYPE[c] for c in _ARGS[fn]] + [_VP, _VP]
-        dev = t.get_device()
-        if dev < 0:
-            raise KernelError(f"{fn}: the operands are not on a GPU")
         word = self._status_at.get(dev)
         if word is None:
-            word = self._status_at[dev] = self.status(t.device).data_ptr()
+            if dev < 0:
+                raise KernelError(f"{fn}: the operands are not on a GPU")
+            word = self._status_at[dev] = self.status(torch.device("cuda", dev)).data_ptr()
         self.launches += 1
-        if dev == torch.cuda.current_device():
+        if dev == torch._C._cuda_getDevice():
             rc = f(*args, word, torch._C._cuda_getCurrentRawStream(dev))
         else:
             with torch.cuda.device(dev):
@@ -332,29 +331,29 @@ class CudaOps(TorchOps):
     def _gemm_int4(self, a, b, out, residual, accumulate):
         M, K = a.shape
         N, inputs = b.shape
-        dtype, dev, packed = a.dtype, a.device, b.packed
+        dtype, dev, packed = a.dtype, a.get_device(), b.packed
         if out is None:
-            out = torch.empty(M, N, device=dev, dtype=dtype)
+            out = torch.empty(M, N, device=a.device, dtype=dtype)
             good = True
         else:
-            good = out.shape == (M, N) and out.dtype == dtype and out.stride(1) == 1 and out.device == dev
+            good = out.shape == (M, N) and out.dtype == dtype and out.stride(1) == 1 and out.get_device() == dev
         c, c_stride = residual, 0
         if accumulate:
             if residual is not None:
                 raise KernelError("a product with 4-bit weights has one addend")
             c = out
         if c is not None:
-            good = good and c.shape in ((M, N), (1, N)) and c.dtype == dtype and c.stride(1) == 1 and c.device == dev
+            good = good and c.shape in ((M, N), (1, N)) and c.dtype == dtype and c.stride(1) == 1 and c.get_device() == dev
             c_stride = c.stride(0) if c.shape[0] > 1 else 0
         stride, inner = a.stride()
         if M == 1:
             stride = K
-        if (not good or K != inputs or dtype != torch.bfloat16 or inner != 1 or stride % 8 or a.data_ptr() % 16 or packed.device != dev
+        if (not good or K != inputs or dtype != torch.bfloat16 or inner != 1 or stride % 8 or a.data_ptr() % 16 or packed.get_device() != dev
                 or packed.data_ptr() % 16):
             raise KernelError(f"4-bit product: bf16 rows of {inputs} numbers, 16-byte aligned, got {tuple(a.shape)} {dtype} {a.stride()}; "
                               f"output and addend bf16 [{M}, {N}]")
         if M:
-            self._launch("kb_gemm_int4", a, a.data_ptr(), stride, packed.data_ptr(), b.scales.data_ptr(), None if c is None else c.data_ptr(), c_stride,
+            self._launch("kb_gemm_int4", dev, a.data_ptr(), stride, packed.data_ptr(), b.scales.data_ptr(), None if c is None else c.data_ptr(), c_stride,
                          out.data_ptr(), out.stride(0), M, N, K, b.group)
         return out
 
@@ -745,30 +744,29 @@ class CudaOps(TorchOps):
 
     def _kv_append_fp8(self, k, v, k_pages, v_pages, slots):
         pages, n_kv, _, hd = k_pages.shape
-        kc, ke, vc, ve = self._fp8_pages(k_pages, v_pages, k.device)
+        dev = k.get_device()
+        kc, ke, vc, ve = self._fp8_pages(k_pages, v_pages, dev)
         N = k.shape[0]
         dtype = k.dtype
         (k_stride, k1), (v_stride, v1) = k.stride(), v.stride()
         if N == 1:
             k_stride = v_stride = n_kv * hd
         if (k.shape != (N, n_kv * hd) or v.shape != (N, n_kv * hd) or slots.shape != (N,) or dtype not in _TYPE or v.dtype != dtype
-                or k1 != 1 or v1 != 1 or slots.dtype != torch.int64 or not slots.is_contiguous() or v.device != k.device or slots.device != k.device):
+                or k1 != 1 or v1 != 1 or slots.dtype != torch.int64 or not slots.is_contiguous() or v.get_device() != dev or slots.get_device() != dev):
             raise KernelError(f"8-bit cache append: rows {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}, slots {tuple(slots.shape)} "
                               f"{slots.dtype} for pages {tuple(k_pages.shape)}")
         if N:
-            self._launch("kb_kv_append_fp8", k, k.data_ptr(), v.data_ptr(), k_stride, v_stride, kc, ke, vc, ve, slots.data_ptr(), N, n_kv, hd,
+            self._launch("kb_kv_append_fp8", dev, k.data_ptr(), v.data_ptr(), k_stride, v_stride, kc, ke, vc, ve, slots.data_ptr(), N, n_kv, hd,
                          pages * 16, _TYPE[dtype])
 
     @staticmethod
-    def _fp8_pages(k_pages, v_pages, device) -> tuple[int, int, int, int]:
-        """Checks that 8-bit pages belong together and lie on ``device``; returns their addresses."""
+    def _fp8_pages(k_pages, v_pages, dev: int) -> tuple[int, int, int, int]:
+        """Checks that 8-bit pages belong together and lie on device ``dev``; returns their addresses."""
         if isinstance(v_pages, Fp8Pages) and k_pages.shape == v_pages.shape and k_pages.shape[2] == 16:
-            own = (k_pages.codes, k_pages.exps, v_pages.codes, v_pages.exps)
-            for t in own:
-                if not t.is_contiguous() or t.device != device:
-                    break
-            else:
-                return tuple(t.data_ptr() for t in own)
+            kc, ke, vc, ve = k_pages.codes, k_pages.exps, v_pages.codes, v_pages.exps
+            if (kc.is_contiguous() and ke.is_contiguous() and vc.is_contiguous() and ve.is_contiguous()
+                    and kc.get_device() == ke.get_device() == vc.get_device() == ve.get_device() == dev):
+                return kc.data_ptr(), ke.data_ptr(), vc.data_ptr(), ve.data_ptr()
         raise KernelError("8-bit keys and values are dense pages of one shape, on the device of the rows")
 
     def paged_decode_attention(self, q, k_pages, v_pages, page_table, ctx_lens, max_ctx, n_q, n_kv, hd, split=512):
@@ -1000,19 +998,19 @@ class CudaOps(TorchOps):
 
     def _kv_gather_fp8(self, k_pages, v_pages, page_table, seg_seq, seg_first, cu, total, dtype):
         pages, G, _, hd = k_pages.shape
-        segs, dev = seg_seq.numel(), page_table.device
+        segs, dev = seg_seq.numel(), page_table.get_device()
         kc, ke, vc, ve = self._fp8_pages(k_pages, v_pages, dev)
         good = dtype in _TYPE and page_table.ndim == 2 and seg_first.numel() == segs and cu.numel() == segs + 1 and (not total or segs)
         for t in (page_table, seg_seq, seg_first, cu):
-            good = good and t.dtype == torch.int32 and t.is_contiguous() and t.device == dev
+            good = good and t.dtype == torch.int32 and t.is_contiguous() and t.get_device() == dev
         if not good:
             raise KernelError(f"8-bit cache rows are read as bf16 or fp32, by dense int32 tables on the pages' device: {dtype}, {segs} segments, "
                               f"{seg_first.numel()} first positions, {cu.numel()} boundaries")
-        k = torch.empty(total, G, hd, device=dev, dtype=dtype)
+        k = torch.empty(total, G, hd, device=page_table.device, dtype=dtype)
         v = torch.empty_like(k)
         if total:
             seqs, width = page_table.shape
-            self._launch("kb_kv_gather_fp8", page_table, kc, ke, vc, ve, G, hd, page_table.data_ptr(), seqs, width, pages, seg_seq.data_ptr(),
+            self._launch("kb_kv_gather_fp8", dev, kc, ke, vc, ve, G, hd, page_table.data_ptr(), seqs, width, pages, seg_seq.data_ptr(),
                          seg_first.data_ptr(), cu.data_ptr(), segs, k.data_ptr(), v.data_ptr(), total, _TYPE[dtype])
         return k, v
 
@@ -1048,7 +1046,7 @@ class CudaOps(TorchOps):
         """bf16 queries with heads of 64 or 128 take the tensor-core kernel (``csrc/tree_attn_sm100.cu``); the 32-bit mode, other head
         sizes and query rows that are not 16-byte aligned the plain one (``csrc/tree_attn.cu``)."""
         N, H, hd = q.shape
-        dev, dtype = q.device, q.dtype
+        dev, dtype = q.get_device(), q.dtype
         B = ctx_lens.numel()
         given = out is not None
         fp8 = isinstance(k_pages, Fp8Pages)
@@ -1056,16 +1054,16 @@ class CudaOps(TorchOps):
             kp, ke, vp, ve = self._fp8_pages(k_pages, v_pages, dev)
         else:
             if (isinstance(v_pages, Fp8Pages) or k_pages.shape != v_pages.shape or k_pages.dtype != dtype or v_pages.dtype != dtype
-                    or not k_pages.is_contiguous() or not v_pages.is_contiguous() or k_pages.device != dev or v_pages.device != dev
+                    or not k_pages.is_contiguous() or not v_pages.is_contiguous() or k_pages.get_device() != dev or v_pages.get_device() != dev
                     or k_pages.ndim != 4):
                 raise KernelError("keys and values are dense pages of one shape, of the queries' type and device")
             kp, ke, vp, ve = k_pages.data_ptr(), None, v_pages.data_ptr(), None
         pages, n_kv, size, d = k_pages.shape
         row, head, inner = q.stride()
         if given:
-            good = out.shape == (N, H * hd) and out.dtype == dtype and out.stride(1) == 1 and out.device == dev
+            good = out.shape == (N, H * hd) and out.dtype == dtype and out.stride(1) == 1 and out.get_device() == dev
         else:
-            out = torch.empty(N, H * hd, device=dev, dtype=dtype)
+            out = torch.empty(N, H * hd, device=q.device, dtype=dtype)
             good = True
         if not good or dtype not in _TYPE or inner != 1 or head != hd or size != 16 or d != hd or H % n_kv:
             raise KernelError(f"tree attention: queries {tuple(q.shape)} {dtype} {q.stride()} for pages {tuple(k_pages.shape)}, output "
@@ -1075,13 +1073,13 @@ class CudaOps(TorchOps):
         if cu_seqlens is None:
             good = good and B <= N
         else:
-            good = good and cu_seqlens.numel() == B + 1 and cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.device == dev
+            good = good and cu_seqlens.numel() == B + 1 and cu_seqlens.dtype == torch.int32 and cu_seqlens.is_contiguous() and cu_seqlens.get_device() == dev
             cu = cu_seqlens.data_ptr()
         if masks is not None:
-            good = good and masks.shape == (N,) and masks.dtype == torch.int64 and masks.is_contiguous() and masks.device == dev
+            good = good and masks.shape == (N,) and masks.dtype == torch.int64 and masks.is_contiguous() and masks.get_device() == dev
             tree = masks.data_ptr()
         for t in (page_table, ctx_lens):
-            good = good and t.dtype == torch.int32 and t.is_contiguous() and t.device == dev
+            good = good and t.dtype == torch.int32 and t.is_contiguous() and t.get_device() == dev
         if not good:
             raise KernelError(f"tree attention: {B} lengths, page lists {tuple(page_table.shape)}, boundaries "
                               f"{None if cu_seqlens is None else tuple(cu_seqlens.shape)}, {N} rows; tables are dense int32, masks int64 per row")
@@ -1094,11 +1092,11 @@ class CudaOps(TorchOps):
         where = (q_at, row, kp, ke, vp, ve, page_table.data_ptr(), width, pages, ctx_lens.data_ptr(), cu, B, tree, out_at, out_row, N, H, n_kv, hd,
                  max_q, max_ctx, scale, int(not given))
         if floats:
-            work = torch.empty(floats, device=dev, dtype=torch.float32)
-            self._launch("kb_tree_attn", q, *where, work.data_ptr(), floats)
+            work = torch.empty(floats, device=q.device, dtype=torch.float32)
+            self._launch("kb_tree_attn", dev, *where, work.data_ptr(), floats)
             self.launches += 1
         else:
-            self._launch("kb_tree_attn_plain", q, *where, _TYPE[dtype])
+            self._launch("kb_tree_attn_plain", dev, *where, _TYPE[dtype])
         return out
 
     delta_short = 16        # most tokens of a sequence in one pass for which the recurrence is walked token by token
