@@ -25,6 +25,7 @@ struct TreeParams {
     int max_pages, num_pages, B, N, H, G, n_kv, max_q, max_ctx;
     float scale_log2;
     int* status;
+    int row_blocks, zero_tail;                         // a block of threads per unit: blocks of rows that a sequence may have; rows that are no sequence's -> 0
 };
 
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {

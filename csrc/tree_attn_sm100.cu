@@ -12,7 +12,7 @@
 // warp (in tree_attn_tile_sm100.cu a CTA): it copies its tiles into a ring of its own, 16 bytes per lane, and waits for no other warp.
 // A unit that lies inside a part is finished there, the others leave partial results (unnormalised output, maximum, sum per row)
 // that the merge kernel puts together.  A worker has at most two such partial units: the one it enters with (slot 0) and the one it
-// leaves with (slot 1).
+// leaves with (slot 1).  Short contexts are cut differently: a block of threads per unit, no merge (DIRECT below).
 //
 // 8-bit pages.  Codes become f16 (exact) on the way to the tensor cores.  Keys: the score's accumulator is scaled by the token's power of two.
 // Values: the probability is scaled by the token's power of two relative to E, the largest seen so far by the warp, times 2^4, and
@@ -75,7 +75,16 @@ struct Cfg {
     static constexpr int SMEM = RING + EXPS + FACT;
 };
 
-template <bool FP8, int HD>
+// n rows of G heads from row c0 on, head h * G -> zero, by all threads of the block.
+__device__ __forceinline__ void zero_rows(const TreeParams& p, int c0, int n, int head, int dims) {
+    for (int row = 0; row < n; ++row) {
+        bf16* dst = p.out + (long long)(c0 + row) * p.out_stride + (long long)head;
+        for (int d = threadIdx.x * 4; d < dims; d += THREADS * 4) *reinterpret_cast<uint2*>(dst + d) = make_uint2(0u, 0u);
+    }
+}
+
+// DIRECT: a block of threads per unit, whose tiles its warps share; nothing is left for a merge.  Else the line of tiles of all units.
+template <bool FP8, int HD, bool DIRECT>
 __global__ void __launch_bounds__(THREADS, CTAS)
 tree_attn_kernel(const TreeParams p) {
     using C = Cfg<FP8, HD>;
@@ -93,21 +102,51 @@ tree_attn_kernel(const TreeParams p) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, qd = lane & 3;
     kb_dep_wait();
     kb_dep_trigger();
-    count_tiles<C::ROWS, TILE, THREADS>(p, uoff, wsum);
     const int worker = blockIdx.x * WARPS + warp;
-    const int2 part = part_of_line(uoff[p.B], worker, gridDim.x * WARPS);
+    Segment whole_unit = {};                           // (DIRECT)
+    if constexpr (DIRECT) {
+        const int bh = blockIdx.x / p.row_blocks, b = bh / p.n_kv, end = p.cu ? p.cu[p.B] : p.B;
+        whole_unit.b = b;
+        whole_unit.h = bh % p.n_kv;
+        whole_unit.rb = blockIdx.x % p.row_blocks;
+        if (p.zero_tail) {                             // rows behind the last sequence, and in front of the first
+            for (int n = max(end, 0) + blockIdx.x; n < p.N; n += gridDim.x) zero_rows(p, n, 1, 0, p.H * HD);
+            for (int n = blockIdx.x; p.cu && n < min(p.cu[0], p.N); n += gridDim.x) zero_rows(p, n, 1, 0, p.H * HD);
+        }
+        const bool first = whole_unit.rb == 0;
+        const int2 sp = span_of(p, b, first && whole_unit.h == 0 && threadIdx.x == 0);
+        if (sp.x == 0) {
+            const int c0 = max(p.cu ? p.cu[b] : b, 0), c1 = min(p.cu ? p.cu[b + 1] : b + 1, p.N);
+            if (first) zero_rows(p, c0, c1 - c0, whole_unit.h * p.G * HD, p.G * HD);
+            return;
+        }
+        if (whole_unit.rb * C::ROWS >= sp.x * p.G) return;
+        whole_unit.n = sp.x;
+        whole_unit.ctx = sp.y;
+        whole_unit.T = (sp.y + TILE - 1) / TILE;
+    } else {
+        count_tiles<C::ROWS, TILE, THREADS>(p, uoff, wsum);
+        if (uoff[p.B] == 0) return;
+    }
+    const int2 part = DIRECT ? make_int2(whole_unit.T * warp / WARPS, whole_unit.T * (warp + 1) / WARPS) : part_of_line(uoff[p.B], worker, gridDim.x * WARPS);
     const int lo = part.x, hi = part.y;
-    if (uoff[p.B] == 0) return;
-    auto segment = [&](int x) { return segment_at<C::ROWS, TILE>(p, uoff, x, hi); };
+    auto segment = [&](int x) {
+        if constexpr (!DIRECT) return segment_at<C::ROWS, TILE>(p, uoff, x, hi);
+        Segment s = whole_unit;
+        s.t0 = x;
+        s.t1 = hi;
+        return s;
+    };
 
     // ---- this warp's ring: item k is tile lo + k
     uint8_t* ring = ring_all + (size_t)warp * C::NST * C::STAGE;
     uint8_t* exps = exps_all + warp * C::NST * 2 * TILE;
-    const Segment unit = segment(min(lo, uoff[p.B] - 1));      // the first unit of the part
+    const Segment unit = segment(DIRECT ? lo : min(lo, uoff[p.B] - 1));        // the first unit of the part
     Segment ps = unit;
     // Whether the block's four parts lie in one unit: their results then meet in shared memory, and the merge has a quarter of the parts.
-    const int2 cta_first = part_of_line(uoff[p.B], blockIdx.x * WARPS, gridDim.x * WARPS), cta_last = part_of_line(uoff[p.B], blockIdx.x * WARPS + WARPS - 1, gridDim.x * WARPS);
-    const bool together = cta_last.y > 0 && cta_first.x >= lo - unit.t0 && cta_last.y <= lo - unit.t0 + unit.T;
+    const int2 cta_first = DIRECT ? make_int2(0, 0) : part_of_line(uoff[p.B], blockIdx.x * WARPS, gridDim.x * WARPS);
+    const int2 cta_last = DIRECT ? make_int2(0, unit.T) : part_of_line(uoff[p.B], blockIdx.x * WARPS + WARPS - 1, gridDim.x * WARPS);
+    const bool together = DIRECT || cta_last.y > 0 && cta_first.x >= lo - unit.t0 && cta_last.y <= lo - unit.t0 + unit.T;
     int px = lo, pfirst = lo;                          // next tile to issue; tile at which ps begins
     int next_page = -1;                                // lane l < PAGES: page number of the next item (fetched one item ahead)
     auto fetch_page = [&]() {
@@ -460,7 +499,8 @@ tree_attn_kernel(const TreeParams p) {
     copy_wait<0>();
     if (!together) return;
     __syncthreads();
-    const int x0 = cta_first.x - (lo - unit.t0), x1 = cta_last.y - (lo - unit.t0);     // the block's tiles of the unit
+    const int x0 = DIRECT ? 0 : cta_first.x - (lo - unit.t0), x1 = DIRECT ? unit.T : cta_last.y - (lo - unit.t0);      // the block's tiles of the unit
+    auto idle = [&](int w) { return DIRECT && unit.T * w / WARPS == unit.T * (w + 1) / WARPS; };       // a warp without a tile has left nothing
     const bool done = x0 == 0 && x1 == unit.T;
     const long long slot = 2ll * blockIdx.x * WARPS + (x0 == 0);
     const int M = unit.n * p.G - unit.rb * C::ROWS, c0 = p.cu ? p.cu[unit.b] : unit.b;
@@ -468,11 +508,13 @@ tree_attn_kernel(const TreeParams p) {
         const int row = i / (HD / 4), d = i % (HD / 4) * 4;
         float top = -INFINITY, sum = 0.f;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, wml[w][row].x);
+        for (int w = 0; w < WARPS; ++w)
+            if (!idle(w)) top = fmaxf(top, wml[w][row].x);
         const float at = top == -INFINITY ? 0.f : top;
         float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
+            if (idle(w)) continue;
             const float2 ml = wml[w][row];
             const float g = exp2f(ml.x - at);
             sum += ml.x == -INFINITY ? ml.y : ml.y * g;                    // a sum without a maximum is zero, or NaN and has to get through
@@ -616,7 +658,7 @@ int tree::sm_count() {
 namespace {
 
 struct Plan {
-    int rows, tile, grid, workers, per_cta, merge_warps;
+    int rows, tile, grid, workers, per_cta, merge_warps, row_blocks;       // row_blocks: > 0 where a block of threads takes a unit
 };
 // Which kernel, and how many CTAs: as many as there are tiles for, at most what fits the GPU at once.  The 128-row kernel pays for 128 rows
 // whatever there are, this one for units of 16 rows, of which each reads the keys and values again.  Measured (us, this kernel / the 128-row one), 64
@@ -624,6 +666,10 @@ struct Plan {
 // bf16 pages 89 / 114, 139 / 120, -, 237 / 136.  So: up to 48 rows on 8-bit pages, up to 16 on bf16 pages.
 // The merge walks a unit's parts with one warp per row where there are about eight of them, else with 8 or 32: (us, 1 / 8 / 32 warps) one token of 64
 // sequences over 2048 tokens 52 / 59 / 98, one of one sequence over 4000 tokens 20 / 13 / 14, of four over 8000 35 / 30 / 30.
+// Short contexts: a block of threads per unit where the units run at once, which needs no count of tiles, no partial results and no merge.  (us, so / the line
+// of tiles) one token, 24 query and 8 KV heads: 1 sequence over 250 tokens 8.2 / 11.1 (bf16), 500 10.5 / 11.7, 1000 15.3 / 12.8, 2000 24.9 / 11.8; 16 over 500
+// 11.1 / 15.4, bf16 (32 tiles) 11.5 / 17.4; 50 over 1000 25.6 / 33.5, over 2000 40.6 / 45.7.  Up to 16 tiles, or 32 where there are at least 64 units; more would
+// lose twice what it gains when one sequence is long and the others short.
 Plan plan_for(int B, int N, int n_kv, int G, int hd, int max_q, int max_ctx, bool fp8) {
     Plan pl;
     const int most_rows = max_q * G;
@@ -636,6 +682,13 @@ Plan plan_for(int B, int N, int n_kv, int G, int hd, int max_q, int max_ctx, boo
     const long long want = (tiles + pl.per_cta - 1) / pl.per_cta, most = (long long)(pl.rows == 128 ? 1 : CTAS) * sm_count();
     pl.grid = (int)(want < most ? want : most);
     pl.workers = pl.grid * pl.per_cta;
+    const long long all = (long long)B * n_kv * one;
+    pl.row_blocks = 0;
+    if (pl.rows == 16 && all <= (long long)CTAS * sm_count() && max_ctx <= (all >= 64 ? 32 : 16) * pl.tile) {
+        pl.row_blocks = (int)one;
+        pl.grid = (int)all;
+        pl.workers = 0;
+    }
     pl.merge_warps = pl.grid <= 8 * units ? 1 : pl.grid <= 64 * units ? 8 : 32;
     return pl;
 }
@@ -665,28 +718,32 @@ int merge(const TreeParams& p, const Plan& pl, int zero_tail, cudaStream_t st) {
                                  : launch_merge<HD, 32, ROW_MAJOR>(p, pl, zero_tail, st);
 }
 
-template <bool FP8, int HD>
-int launch_tree(const TreeParams& p, const Plan& pl, cudaStream_t st) {
+template <bool FP8, int HD, bool DIRECT>
+int launch_form(const TreeParams& p, const Plan& pl, cudaStream_t st) {
     static bool flags[64] = {};
     bool* set = kb_device_flag(flags);
     if (!set) return 7;
     if (!*set) {
-        if (cudaFuncSetAttribute(tree_attn_kernel<FP8, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<FP8, HD>::SMEM) != cudaSuccess) return 7;
+        if (cudaFuncSetAttribute(tree_attn_kernel<FP8, HD, DIRECT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<FP8, HD>::SMEM) != cudaSuccess) return 7;
         *set = true;
     }
-    return kb_launch_dep(tree_attn_kernel<FP8, HD>, dim3(pl.grid), dim3(THREADS), Cfg<FP8, HD>::SMEM, st, p);
+    return kb_launch_dep(tree_attn_kernel<FP8, HD, DIRECT>, dim3(pl.grid), dim3(THREADS), Cfg<FP8, HD>::SMEM, st, p);
+}
+template <bool FP8, int HD>
+int launch_tree(const TreeParams& p, const Plan& pl, cudaStream_t st) {
+    return pl.row_blocks ? launch_form<FP8, HD, true>(p, pl, st) : launch_form<FP8, HD, false>(p, pl, st);
 }
 
 }  // namespace
 
-// Floats of workspace that kb_tree_attn wants, 0 where the call is not one for it (the plain form takes it).
+// Floats of workspace that kb_tree_attn wants (-1: none), 0 where the call is not one for it (the plain form takes it).
 KB_API long long kb_tree_attn_floats(int N, int B, int H, int n_kv, int hd, int max_q, int max_ctx, int fp8) {
     if (N < 1 || B < 1 || B > MAX_B || n_kv < 1 || H < n_kv || H % n_kv || (hd != 64 && hd != 128) || max_q < 1 || max_q > 64 || max_ctx < 1 ||
         (long long)N * H > 0x7fffffffll ||
         (long long)B * n_kv * ((max_q * (long long)(H / n_kv) + 15) / 16) * ((max_ctx + 15ll) / 16) > 0x7fffffffll / 64)
         return 0;
     const Plan pl = plan_for(B, N, n_kv, H / n_kv, hd, max_q, max_ctx, fp8 != 0);
-    return 2ll * pl.workers * pl.rows * (hd + 2) + B + 4;
+    return pl.row_blocks ? -1 : 2ll * pl.workers * pl.rows * (hd + 2) + B + 4;
 }
 
 // As kb_tree_attn_plain for bf16 and heads of 64 and 128; query rows 16-byte, output rows 8-byte aligned; `work` has kb_tree_attn_floats
@@ -700,7 +757,7 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
         ((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)ke | (uintptr_t)ve | (uintptr_t)work) % 16 || (uintptr_t)out % 8)
         return 5;
     const long long need = kb_tree_attn_floats(N, B, H, n_kv, hd, max_q, max_ctx, fp8);
-    if (need == 0 || work_floats < need) return 5;
+    if (need == 0 || (need > 0 && (work_floats < need || !work))) return 5;
     const Plan pl = plan_for(B, N, n_kv, H / n_kv, hd, max_q, max_ctx, fp8);
     TreeParams p;
     p.q = (const bf16*)q;
@@ -729,12 +786,14 @@ KB_API int kb_tree_attn(const void* q, long long q_stride, const void* k, const 
     p.max_ctx = max_ctx;
     p.scale_log2 = scale * 1.4426950408889634f;
     p.status = status;
+    p.row_blocks = pl.row_blocks;
+    p.zero_tail = zero_tail;
     const int r = pl.rows == 128      ? launch_tile(p, hd, fp8, pl.grid, st)
                   : fp8 && hd == 128 ? launch_tree<true, 128>(p, pl, st)
                   : fp8              ? launch_tree<true, 64>(p, pl, st)
                   : hd == 128        ? launch_tree<false, 128>(p, pl, st)
                                      : launch_tree<false, 64>(p, pl, st);
-    if (r) return r;
+    if (r || pl.row_blocks) return r;
     if (pl.rows == 128) return hd == 128 ? merge<128, false>(p, pl, zero_tail, st) : merge<64, false>(p, pl, zero_tail, st);
     return hd == 128 ? merge<128, true>(p, pl, zero_tail, st) : merge<64, true>(p, pl, zero_tail, st);
 }

@@ -1091,7 +1091,9 @@ class CudaOps(TorchOps):
             floats = self._tree_floats(N, B, H, n_kv, hd, max_q, max_ctx, int(fp8))
         where = (q_at, row, kp, ke, vp, ve, page_table.data_ptr(), width, pages, ctx_lens.data_ptr(), cu, B, tree, out_at, out_row, N, H, n_kv, hd,
                  max_q, max_ctx, scale, int(not given))
-        if floats:
+        if floats < 0:
+            self._launch("kb_tree_attn", dev, *where, None, 0)
+        elif floats:
             work = torch.empty(floats, device=q.device, dtype=torch.float32)
             self._launch("kb_tree_attn", dev, *where, work.data_ptr(), floats)
             self.launches += 1

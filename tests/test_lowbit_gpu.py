@@ -87,6 +87,7 @@ def test_tree_attention(case, fp8, dtype):
 
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("H,G,hd,n,most,rows", [(16, 4, 128, 45, 700, 3), (8, 2, 64, 200, 90, 1), (8, 1, 128, 30, 500, 20), (24, 2, 64, 21, 300, 64), (12, 4, 128, 25, 600, 13),
+                                                (16, 4, 128, 45, 1500, 3), (8, 2, 64, 300, 90, 1), (4, 2, 64, 9, 2100, 4), (12, 4, 128, 25, 1700, 13),
                                                 (12, 1, 128, 1, 9000, 64)])
 def test_ragged_batches(H, G, hd, n, most, rows, fp8):
     """Many sequences per block of threads and many blocks per sequence, empty ones among them, on both tensor-core kernels."""
@@ -264,6 +265,34 @@ def verification_step(ops, seed=0):
         return o.reshape(12, -1).bfloat16().to(f) @ dense[1].t().cpu() + x.to(f).cpu()
 
     return run, plain, [rand(12, D).bfloat16() for _ in range(3)]
+
+
+@pytest.mark.parametrize("H", [4, 64])                   # 6 and 96 rows per KV head: both tensor-core kernels, with partial results and a merge
+def test_long_contexts_captured_on_two_streams(H):
+    ops = get_ops("cuda")
+    runs = []
+    for seed in (0, 1):
+        c = cases.tree_case(H, 2, 64, [3, 1, 2], [3000, 40, 1700], True, torch.bfloat16, seed)
+        t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        q, args = c["q"].cuda(), (cases._put(c["k"], "cuda"), cases._put(c["v"], "cuda"), c["table"].cuda(), t(c["lens"]), t(c["cu"]), 3, 3000, 0.125)
+        runs.append((q, args, ops.paged_tree_attention(q, *args), ops.paged_tree_attention(-q, *args)))
+    graphs = []
+    for q, args, _, _ in runs:
+        x, g = q.clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g), ops.dependent_launch():
+            y = ops.paged_tree_attention(x, *args)
+        graphs.append((x, g, y))
+    streams = [torch.cuda.Stream() for _ in runs]
+    for sign in (1, -1, 1):
+        for (x, g, _), (q, *_), st in zip(graphs, runs, streams):
+            st.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(st):
+                x.copy_(q * sign)
+                g.replay()
+        torch.cuda.synchronize()
+        for (_, _, y), (_, _, plus, minus) in zip(graphs, runs):
+            assert torch.equal(y, plus if sign > 0 else minus)
+    ops.check_status()
 
 
 def test_operands_on_the_host_are_refused():
