@@ -669,26 +669,23 @@ struct Plan {
 // Short contexts: a block of threads per unit where the units run at once, which needs no count of tiles, no partial results and no merge.  (us, so / the line
 // of tiles) one token, 24 query and 8 KV heads: 1 sequence over 250 tokens 8.2 / 11.1 (bf16), 500 10.5 / 11.7, 1000 15.3 / 12.8, 2000 24.9 / 11.8; 16 over 500
 // 11.1 / 15.4, bf16 (32 tiles) 11.5 / 17.4; 50 over 1000 25.6 / 33.5, over 2000 40.6 / 45.7.  Up to 16 tiles, or 32 where there are at least 64 units; more would
-// lose twice what it gains when one sequence is long and the others short.
+// lose twice what it gains when one sequence is long and the others short.  That holds for many rows as well (us, so / the 128-row kernel): 8 sequences of 8
+// drafted tokens, 24 rows, bf16, over 500 tokens 14.7 / 23.3; 4 of 64, 192 rows, 17.3 / 33.3 (8 bits), 22.8 / 29.6 (bf16).
 Plan plan_for(int B, int N, int n_kv, int G, int hd, int max_q, int max_ctx, bool fp8) {
     Plan pl;
-    const int most_rows = max_q * G;
-    pl.rows = most_rows <= (fp8 ? 48 : 16) ? 16 : 128;
-    pl.tile = pl.rows == 128 ? 128 : fp8 || hd == 64 ? 32 : 16;
+    const int most_rows = max_q * G, tile16 = fp8 || hd == 64 ? 32 : 16;
+    const long long direct = (long long)B * n_kv * ((most_rows + 15) / 16);            // blocks of threads, one per unit of 16 rows
+    const bool take = direct <= (long long)CTAS * sm_count() && max_ctx <= (direct >= 64 ? 32 : 16) * tile16;
+    pl.rows = take || most_rows <= (fp8 ? 48 : 16) ? 16 : 128;
+    pl.tile = pl.rows == 128 ? 128 : tile16;
     const long long blocks = B + (long long)N * G / pl.rows;                            // units per KV head, at most
     const long long one = (most_rows + pl.rows - 1) / pl.rows;
     const long long units = n_kv * (blocks < B * one ? blocks : B * one), tiles = units * ((max_ctx + pl.tile - 1) / pl.tile);
     pl.per_cta = pl.rows == 128 ? 1 : WARPS;
     const long long want = (tiles + pl.per_cta - 1) / pl.per_cta, most = (long long)(pl.rows == 128 ? 1 : CTAS) * sm_count();
-    pl.grid = (int)(want < most ? want : most);
-    pl.workers = pl.grid * pl.per_cta;
-    const long long all = (long long)B * n_kv * one;
-    pl.row_blocks = 0;
-    if (pl.rows == 16 && all <= (long long)CTAS * sm_count() && max_ctx <= (all >= 64 ? 32 : 16) * pl.tile) {
-        pl.row_blocks = (int)one;
-        pl.grid = (int)all;
-        pl.workers = 0;
-    }
+    pl.grid = (int)(take ? direct : want < most ? want : most);
+    pl.workers = take ? 0 : pl.grid * pl.per_cta;
+    pl.row_blocks = take ? (int)one : 0;
     pl.merge_warps = pl.grid <= 8 * units ? 1 : pl.grid <= 64 * units ? 8 : 32;
     return pl;
 }

@@ -286,23 +286,23 @@ def tree_tolerance(c, want, mass, scale):
     return (2.0 ** -8 + 4 * sums) * mass + 2.0 ** -8 * want.abs() + 1e-30
 
 
-def check_tree(ops, device, H, G, hd, sizes, lens, fp8, dtype, masked, seed=0, spread=1.0):
+def check_tree(ops, device, H, G, hd, sizes, lens, fp8, dtype, masked, seed=0, spread=1.0, bound=None):
     c = tree_case(H, G, hd, sizes, lens, fp8, dtype, seed, spread=spread)
     empty = [i for i in (1,) if masked and sum(sizes) > 2]
     masks = tree_masks(sizes, seed + 1, empty) if masked else None
     scale = 1.0 / math.sqrt(hd)
     want, mass = plain_tree(c["q"], _dense(c["k"]), _dense(c["v"]), c["table"].tolist(), c["lens"], c["cu"], scale, masks)
     tol = tree_tolerance(c, want, mass, scale)
-    got = run_tree(ops, device, c, masks, scale, tail=3).cpu()
+    got = run_tree(ops, device, c, masks, scale, tail=3, max_ctx=bound).cpu()
     N = c["q"].shape[0]
     assert got.shape == (N + 3, H * hd) and torch.equal(got[N:], torch.zeros_like(got[N:]))
     err = (got[:N].to(F64).view(N, H, hd) - want).abs()
     assert bool((err <= tol).all()), (float((err / tol).max()), (err / tol).amax((1, 2)).tolist())
     kept = torch.full((N + 3, H * hd + 8), 5.0, dtype=dtype, device=device)         # a given output: strided, rows behind the last are left
-    run_tree(ops, device, c, masks, scale, tail=3, out=kept[:, : H * hd])
+    run_tree(ops, device, c, masks, scale, tail=3, out=kept[:, : H * hd], max_ctx=bound)
     assert torch.equal(kept[:N, : H * hd].cpu(), got[:N]) and bool((kept[N:] == 5).all()) and bool((kept[:, H * hd:] == 5).all())
     if max(sizes) == 1 and min(sizes) == 1 and not masked:
-        assert torch.equal(run_tree(ops, device, c, None, scale, decode=True).cpu(), got[:N])
+        assert torch.equal(run_tree(ops, device, c, None, scale, decode=True, max_ctx=bound).cpu(), got[:N])
 
 
 TREE_CASES = [  # heads, kv heads, head size, rows per sequence, tokens per sequence, masks
@@ -314,13 +314,13 @@ TREE_CASES = [  # heads, kv heads, head size, rows per sequence, tokens per sequ
 TREE_PLAIN_CASES = [(2, 1, 80, [3, 1], [40, 7], True), (3, 3, 16, [1], [200], False), (4, 2, 256, [9], [77], True)]
 
 
-def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128, H=4, G=2):
+def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128, H=4, G=2, bound=None):
     """A drafted token whose keys or values are not finite reaches the rows that see it and no other; of its values, in a row that sees
     it, only the dimensions that are not finite are lost."""
     sizes, lens = [6, 2], [70, 33]
     masks = [1, 3, 5, 11, 21, 33, 1, 3]
     c = tree_case(H, G, hd, sizes, lens, fp8, dtype, 11)
-    clean = run_tree(ops, device, c, masks, 0.1).cpu()
+    clean = run_tree(ops, device, c, masks, 0.1, max_ctx=bound).cpu()
     prefix = lens[0] - sizes[0]
     page, off = int(c["table"][0, (prefix + 1) // PAGE]), (prefix + 1) % PAGE      # drafted token 1: rows 1 and 3 see it
     for name in ("k", "v"):
@@ -333,7 +333,7 @@ def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128,
             else:
                 d[name] = c[name].clone()
                 d[name][page, :, off] = what
-            got = run_tree(ops, device, d, masks, 0.1).cpu()
+            got = run_tree(ops, device, d, masks, 0.1, max_ctx=bound).cpu()
             hit = [1, 3]
             rest = [0, 2, 4, 5, 6, 7]
             assert torch.equal(got[rest], clean[rest]), (name, what)
@@ -341,7 +341,7 @@ def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128,
     if not fp8:
         d = {**c, "v": c["v"].clone()}
         d["v"][page, :, off, 3] = math.inf
-        got = run_tree(ops, device, d, masks, 0.1).cpu().view(-1, H, hd)
+        got = run_tree(ops, device, d, masks, 0.1, max_ctx=bound).cpu().view(-1, H, hd)
         want, mass = plain_tree(c["q"], _dense(c["k"]), _dense(c["v"]), c["table"].tolist(), lens, c["cu"], 0.1, masks)
         tol = tree_tolerance(c, want, mass, 0.1)
         dims = [i for i in range(hd) if i != 3]
@@ -350,10 +350,14 @@ def check_tree_masked_not_finite(ops, device, fp8, dtype=torch.bfloat16, hd=128,
         assert bool(((got[hit].to(F64) - want[hit]).abs() <= tol[hit])[..., dims].all())
 
 
-def check_tree_bad_sequences(ops, device, fp8, H=4, G=2):
-    """Sequences that break the rules get zero rows, tokens on pages that are not there are not seen; the other sequences are as ever."""
+def check_tree_bad_sequences(ops, device, fp8, H=4, G=2, empty=0):
+    """Sequences that break the rules get zero rows, tokens on pages that are not there are not seen; the other sequences are as ever.
+    ``empty``: so many sequences without rows behind them (which are then too many for a block of threads each)."""
     hd = 64
     c = tree_case(H, G, hd, [2, 3, 1, 2], [40, 2, 50, 90], fp8, torch.bfloat16, 5)      # 3 rows in 2 tokens
+    c["lens"] = list(c["lens"]) + [0] * empty
+    c["cu"] = list(c["cu"]) + [c["cu"][-1]] * empty
+    c["table"] = torch.cat([c["table"], torch.zeros(empty, c["table"].shape[1], dtype=c["table"].dtype)])
     c["table"][2, 1] = c["k"].shape[0]                              # page past the cache: tokens 16 .. 31 of sequence 2
     c["table"][2, 2] = -1
     got = run_tree(ops, device, c, None, 0.125, max_ctx=60).cpu().view(-1, H, hd)        # sequence 3 is longer than 60

@@ -79,9 +79,10 @@ def test_indices_out_of_range_are_reported():
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("case", cases.TREE_CASES + cases.TREE_PLAIN_CASES, ids=str)
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_tree_attention(case, fp8, dtype):
+@pytest.mark.parametrize("bound", [None, 5000])          # how long contexts may be: a block of threads per unit, or the line of tiles and a merge
+def test_tree_attention(case, fp8, dtype, bound):
     H, G, hd, sizes, lens, masked = case
-    guarded(lambda ops: cases.check_tree(ops, "cuda", H, G, hd, sizes, lens, fp8, dtype, masked))
+    guarded(lambda ops: cases.check_tree(ops, "cuda", H, G, hd, sizes, lens, fp8, dtype, masked, bound=bound))
     get_ops("cuda").check_status()
 
 
@@ -89,10 +90,11 @@ def test_tree_attention(case, fp8, dtype):
 @pytest.mark.parametrize("H,G,hd,n,most,rows", [(16, 4, 128, 45, 700, 3), (8, 2, 64, 200, 90, 1), (8, 1, 128, 30, 500, 20), (24, 2, 64, 21, 300, 64), (12, 4, 128, 25, 600, 13),
                                                 (16, 4, 128, 45, 1500, 3), (8, 2, 64, 300, 90, 1), (4, 2, 64, 9, 2100, 4), (12, 4, 128, 25, 1700, 13),
                                                 (12, 1, 128, 1, 9000, 64)])
-def test_ragged_batches(H, G, hd, n, most, rows, fp8):
+@pytest.mark.parametrize("bound", [None, 9000])
+def test_ragged_batches(H, G, hd, n, most, rows, fp8, bound):
     """Many sequences per block of threads and many blocks per sequence, empty ones among them, on both tensor-core kernels."""
     sizes, lens = cases.ragged(n, most, rows, 7 * n + rows) if n > 1 else ([rows], [most])
-    guarded(lambda ops: cases.check_tree(ops, "cuda", H, G, hd, sizes, lens, fp8, torch.bfloat16, rows > 1))
+    guarded(lambda ops: cases.check_tree(ops, "cuda", H, G, hd, sizes, lens, fp8, torch.bfloat16, rows > 1, bound=bound))
     get_ops("cuda").check_status()
 
 
@@ -125,15 +127,17 @@ def test_calls_that_take_the_plain_kernel(fp8):
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("H", [4, 10, 32])                # 12, 30 and 96 rows per KV head: the three forms of the kernel
-def test_masked_tokens_that_are_not_finite(fp8, dtype, hd, H):
-    cases.check_tree_masked_not_finite(get_ops("cuda"), "cuda", fp8, dtype, hd, H, 2)
+@pytest.mark.parametrize("bound", [None, 5000])
+def test_masked_tokens_that_are_not_finite(fp8, dtype, hd, H, bound):
+    cases.check_tree_masked_not_finite(get_ops("cuda"), "cuda", fp8, dtype, hd, H, 2, bound)
 
 
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("H", [4, 16, 64])
-def test_bad_sequences(fp8, H):
+@pytest.mark.parametrize("empty", [0, 230])
+def test_bad_sequences(fp8, H, empty):
     ops = get_ops("cuda")
-    cases.check_tree_bad_sequences(ops, "cuda", fp8, H, 2)
+    cases.check_tree_bad_sequences(ops, "cuda", fp8, H, 2, empty)
     with pytest.raises(KernelError, match="status 6"):
         ops.check_status()
     ops.check_status()
@@ -333,7 +337,8 @@ def test_caches_of_more_than_4_gigabytes(fp8):
         for H in (16, 64):                            # 6, 24, 24 and 96 rows per KV head
             for rows in (3, 12):
                 q = torch.randn(2 * rows, H, hd, device="cuda", generator=torch.Generator(device="cuda").manual_seed(H + rows)).bfloat16()
-                out.append(ops.paged_tree_attention(q, kp, vp, table + at, t(46, 33), t(0, rows, 2 * rows), rows, 48, 0.09))
+                for bound in (48, 5000):              # a block of threads per unit, the line of tiles
+                    out.append(ops.paged_tree_attention(q, kp, vp, table + at, t(46, 33), t(0, rows, 2 * rows), rows, bound, 0.09))
         got.append(out)
         del kp, vp
     assert all(torch.equal(a, b) for a, b in zip(*got)) and bool((got[0][0] != 0).any())
