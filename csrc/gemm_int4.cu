@@ -283,8 +283,11 @@ KB_API int kb_gemm_int4(const void* x, long long x_stride, const void* packed, c
     // 8 tokens, K 4096, with 1 / 2 / 3 / 4 at once: N 4096 (two tiles a block) 5.8 / 4.9 / - / 4.9, N 6144 (three) 7.5 / 7.1 / 5.9 / 6.4, N 28672 (thirteen)
     // 25.3 / 20.2 / 18.6 / 18.0.  16 tokens: the second half of the columns doubles the copies; 12 and 8 warps leave room for three and four tiles.
     // More than 16 go to tcgen05: 16 tokens take 7.1 us here and 9.9 there at N 6144, 25 and 28 at N 28672; 32 tokens 13.3 and 10.2, 47 and 29.
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 7;
+    static int count[64];                              // SMs of each device, once asked
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 7;
+    if (!count[dev] && cudaDeviceGetAttribute(&count[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 7;
+    const int sms = count[dev];
     const int per = (s.nt + sms - 1) / sms;
     if (M <= 8) {
         if (per == 1) INT4_RUN(1, 1, 16, 3);
