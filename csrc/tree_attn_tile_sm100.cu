@@ -542,7 +542,10 @@ tree_tile_kernel(const TreeParams p) {
             const bool live = sg.rb * TT + (warp & 3) * 32 < M;            // the warp has rows
             const int row_i = min(R, M - 1) / p.G, row_g = min(R, M - 1) % p.G;
             float scale = p.scale_log2;
-            if constexpr (FP8) {
+            // A group without a tile of the segment does not wait for its queries: it could come so late that the queries two segments on have
+            // turned the barrier's parity once more (they are loaded when the segment's products have run, for which only groups with a tile
+            // are needed)
+            if (FP8 && (len > 1 || g == (j0 & 1))) {
                 if (!tc::mbar_wait(&q_ready[seg & 1], (uint32_t)(seg >> 1) & 1u, abort_flag)) { ok = false; break; }
                 scale *= q_scale[(seg & 1) * TT + r];
             }
