@@ -53,14 +53,14 @@ __device__ __forceinline__ void split_e4m3(uint2 q, float inv, uint32_t& hi, uin
     hi = h[0] | h[1] << 16;
     lo = l[0] | l[1] << 16;
 }
+// Least biased exponent of the power of two that is taken out of a query row (rows of zeros and of numbers below 2^-119 have this one): its
+// place below is then a normal number, which arithmetic that takes denormal numbers for zero keeps, and no hidden score (-infinity) meets a zero.
+constexpr int Q_LEAST = 8;
 // The power of two that brings a row's largest number to [2^7, 2^8), from the largest magnitude's bits, and its inverse; NaN where the row is not finite.
 __device__ __forceinline__ float q_down(uint32_t big) {
-    return big >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)min(254 - (int)(big >> 7) + 7, 254) << 23);
+    return big >= 0x7f80u ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(261 - max((int)(big >> 7), Q_LEAST)) << 23);
 }
-__device__ __forceinline__ float q_up(uint32_t big) {
-    const int b = 254 - min(254 - (int)(big >> 7) + 7, 254);
-    return __uint_as_float(b > 0 ? (uint32_t)b << 23 : 0x00400000u);
-}
+__device__ __forceinline__ float q_up(uint32_t big) { return __uint_as_float((uint32_t)(max((int)(big >> 7), Q_LEAST) - 7) << 23); }
 // four e4m3 codes -> two f16 pairs
 __device__ __forceinline__ void codes_to_f16(uint32_t c, uint32_t& lo, uint32_t& hi) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(c));

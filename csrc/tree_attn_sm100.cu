@@ -201,7 +201,7 @@ tree_attn_kernel(const TreeParams p) {
         const int c0 = p.cu ? p.cu[sg.b] : sg.b;
         // ---- the unit's queries as A fragments
         uint32_t qa[KS][4];
-        float rs[2];                                   // scores of rows r, r + 8 in log2 units per accumulator unit
+        float rs[2];                                   // 8-bit pages: the power of two taken out of rows r, r + 8
 #pragma unroll
         for (int hf = 0; hf < 2; ++hf) {
             const int R = row0 + hf * 8 + r;
@@ -215,16 +215,16 @@ tree_attn_kernel(const TreeParams p) {
                     else raw[ks] = make_uint2(*reinterpret_cast<const uint32_t*>(src + ks * 16 + 2 * qd), *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8 + 2 * qd));
                 }
             }
-            rs[hf] = p.scale_log2;
+            rs[hf] = 1.f;
             if constexpr (FP8) {                       // take a power of two out of the row, then f16
                 uint32_t big = 0;
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks) big = max(big, max(max(raw[ks].x & 0x7fffu, (raw[ks].x >> 16) & 0x7fffu), max(raw[ks].y & 0x7fffu, (raw[ks].y >> 16) & 0x7fffu)));
                 big = max(big, __shfl_xor_sync(0xffffffffu, big, 1));
                 big = max(big, __shfl_xor_sync(0xffffffffu, big, 2));
-                const int e = min(max((int)(big >> 7), 1), 253);           // biased exponent of the largest number
+                const int e = min(max((int)(big >> 7), Q_LEAST), 253);     // biased exponent of the largest number
                 const float inv = pow2_biased(254 - e);
-                rs[hf] = p.scale_log2 * pow2_biased(e);
+                rs[hf] = pow2_biased(e);
 #pragma unroll
                 for (int ks = 0; ks < KS; ++ks)
                     raw[ks] = make_uint2(pack_f16(__uint_as_float(raw[ks].x << 16) * inv, __uint_as_float(raw[ks].x & 0xffff0000u) * inv),
@@ -264,7 +264,7 @@ tree_attn_kernel(const TreeParams p) {
                         grow = exp2f((float)(E - top));
                         E = top;
                     }
-                    fk[lane] = pow2_biased(ek);
+                    fk[lane] = pow2_biased(ek) * p.scale_log2;
                     const int w = min(ev - E, 0) + UP + 127;
                     fk[TILE + lane] = counts ? (w > 0 ? __uint_as_float((uint32_t)w << 23) : 0.f) : 1.f;
                     __syncwarp();
@@ -300,9 +300,13 @@ tree_attn_kernel(const TreeParams p) {
                             mma<false>(s[2 * pg + 1], qa[ks], b[2], b[3]);
                         }
                 }
+                // In log2 units (8-bit pages: but for the row's power of two, which rounds nothing) before anything is hidden or subtracted: a scale
+                // that vanishes would make NaN of a hidden score, one inside the subtraction would leave its product's rounding, which for
+                // scores from 2^32 on is more than an exponential holds
 #pragma unroll
-                for (int j = 0; j < NT && FP8; ++j) {
-                    const float2 f = *reinterpret_cast<const float2*>(fk + 8 * j + 2 * qd);
+                for (int j = 0; j < NT; ++j) {
+                    float2 f = make_float2(p.scale_log2, p.scale_log2);
+                    if constexpr (FP8) f = *reinterpret_cast<const float2*>(fk + 8 * j + 2 * qd);
                     s[j][0] *= f.x;
                     s[j][1] *= f.y;
                     s[j][2] *= f.x;
@@ -346,7 +350,7 @@ tree_attn_kernel(const TreeParams p) {
                     mx[hf] = fmaxf(s[0][2 * hf], s[0][2 * hf + 1]);
 #pragma unroll
                     for (int j = 1; j < NT; ++j) mx[hf] = fmaxf(mx[hf], fmaxf(s[j][2 * hf], s[j][2 * hf + 1]));
-                    mx[hf] *= rs[hf];                  // (rs is positive)
+                    if constexpr (FP8) mx[hf] *= rs[hf];
                 }
                 if (__any_sync(0xffffffffu, mx[0] > m[0] + GROW || mx[1] > m[1] + GROW || (FP8 && grow != 1.f))) {
                     float f[2];
@@ -374,7 +378,8 @@ tree_attn_kernel(const TreeParams p) {
                     const float at = m[hf] == -INFINITY ? 0.f : m[hf];
 #pragma unroll
                     for (int j = 0; j < NT; ++j) {
-                        float a = exp2f(fmaf(s[j][2 * hf], rs[hf], -at)), z = exp2f(fmaf(s[j][2 * hf + 1], rs[hf], -at));
+                        float a = exp2f(FP8 ? fmaf(s[j][2 * hf], rs[hf], -at) : s[j][2 * hf] - at);
+                        float z = exp2f(FP8 ? fmaf(s[j][2 * hf + 1], rs[hf], -at) : s[j][2 * hf + 1] - at);
                         l[hf] += a + z;
                         if constexpr (FP8) {
                             const float2 w = *reinterpret_cast<const float2*>(fk + TILE + 8 * j + 2 * qd);

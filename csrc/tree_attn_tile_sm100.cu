@@ -129,7 +129,7 @@ tree_tile_kernel(const TreeParams p) {
     uint8_t* sR = sK + L::KST * L::KT;                                 // staged values
     uint8_t* sV = FP8 ? sR + L::RST * L::KT : sR;                      // value operand tiles
     uint8_t* exps = smem + L::RING;                                    // [RST][2][TT] exponents of keys and values
-    float* fact = reinterpret_cast<float*>(exps + L::EXPS);            // [SLOTS][TT] factors of scores
+    float* fact = reinterpret_cast<float*>(exps + L::EXPS);            // [SLOTS][TT] factors of scores, to log2 units
     uint8_t* sQ = smem + L::RING - 2 * L::QT;                          // two query tiles, staged like keys
     float* row_buf = reinterpret_cast<float*>(exps + L::EXPS + L::FACT);   // [2 groups][TT] maxima, then sums
     __shared__ int uoff[MAX_B + 1];
@@ -366,7 +366,7 @@ tree_tile_kernel(const TreeParams p) {
                 const int t = w * 32 + lane, tok = base + t;
                 const bool valid = !edge || (tok < sg.ctx && (have >> (t / PAGE) & 1u));
                 if constexpr (FP8) {
-                    fact[(j % SLOTS) * TT + t] = pow2_biased(e[t]);
+                    fact[(j % SLOTS) * TT + t] = pow2_biased(e[t]) * p.scale_log2;
                     const uint32_t ev = e[TT + t];
                     if (valid && ev != 255u) top = max(top, ev);
                 }
@@ -541,13 +541,13 @@ tree_tile_kernel(const TreeParams p) {
             const int len = sg.t1 - sg.t0, M = sg.n * p.G, R = sg.rb * TT + r, c0 = p.cu ? p.cu[sg.b] : sg.b, prefix = sg.ctx - sg.n;
             const bool live = sg.rb * TT + (warp & 3) * 32 < M;            // the warp has rows
             const int row_i = min(R, M - 1) / p.G, row_g = min(R, M - 1) % p.G;
-            float scale = p.scale_log2;
+            float scale = FP8 ? 1.f : p.scale_log2;        // 8-bit pages: the row's power of two, which rounds nothing
             // A group without a tile of the segment does not wait for its queries: it could come so late that the queries two segments on have
             // turned the barrier's parity once more (they are loaded when the segment's products have run, for which only groups with a tile
             // are needed)
             if (FP8 && (len > 1 || g == (j0 & 1))) {
                 if (!tc::mbar_wait(&q_ready[seg & 1], (uint32_t)(seg >> 1) & 1u, abort_flag)) { ok = false; break; }
-                scale *= q_scale[(seg & 1) * TT + r];
+                scale = q_scale[(seg & 1) * TT + r];
             }
             float m_used = -INFINITY, l = 0.f;
             int E = 0;
@@ -593,6 +593,13 @@ tree_tile_kernel(const TreeParams p) {
                                 x[i + 2] = v.x;
                                 x[i + 3] = v.y;
                             }
+                        } else {                       // (before anything is hidden or subtracted: see tree_attn_sm100.cu)
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                const float2 u = __fmul2_rn(make_float2(x[i], x[i + 1]), sc2);
+                                x[i] = u.x;
+                                x[i + 1] = u.y;
+                            }
                         }
                         const uint32_t sees32 = (uint32_t)(seen[q >> 1] >> (32 * (q & 1)));
                         if (edge) {                    // what is not seen
@@ -609,7 +616,7 @@ tree_tile_kernel(const TreeParams p) {
                         }
                         m4[0] = attn::fmax3(m4[0], x[28], x[29]);
                         m4[1] = attn::fmax3(m4[1], x[30], x[31]);
-                        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * scale;
+                        const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * (FP8 ? scale : 1.f);
                         if (__any_sync(0xffffffffu, mx > m_used + GROW)) {
                             // move to the new maximum what has been summed against the old one: O (S(j) follows the product of the
                             // group's last tile, so O is complete), the sum, and this tile's probabilities so far
@@ -625,7 +632,7 @@ tree_tile_kernel(const TreeParams p) {
                         const float2 nm2 = make_float2(-mb, -mb);
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            const float2 y = __ffma2_rn(make_float2(x[i], x[i + 1]), sc2, nm2);
+                            const float2 v = make_float2(x[i], x[i + 1]), y = FP8 ? __ffma2_rn(v, sc2, nm2) : __fadd2_rn(v, nm2);
                             x[i] = exp2f(y.x);
                             x[i + 1] = exp2f(y.y);
                         }

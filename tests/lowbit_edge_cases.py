@@ -1,0 +1,74 @@
+"""Checks of tree attention and 4-bit products at the ends of their number ranges, on either back end, against the plain float64
+forms of ``lowbit_cases``."""
+import math
+
+import torch
+
+import lowbit_cases as cases
+from kotodama_b200.ops import Fp8Pages
+
+F64 = torch.float64
+PAGE = cases.PAGE
+
+
+def compare_tree(ops, device, c, masks, scale, bound=None):
+    """The call's rows against the plain form within the tolerance of the operator's roundings; returns them."""
+    N, H, hd = c["q"].shape
+    dense = [cases._dense(c[n]) for n in ("k", "v")]
+    want, mass = cases.plain_tree(c["q"], *dense, c["table"].tolist(), c["lens"], c["cu"], scale, masks)
+    got = cases.run_tree(ops, device, c, masks, scale, max_ctx=bound).cpu().to(F64).view(N, H, hd)
+    tol = cases.tree_tolerance(c, want, mass, scale)
+    err = (got - want).abs()
+    assert bool((err <= tol).all()), (err / tol).nan_to_num(math.inf).amax((1, 2)).tolist()
+    return got
+
+
+# ------------------------------------------------------------------ query rows of zeros, scales that are nearly zero
+def check_tree_tiny_queries(ops, device, fp8, dtype, hd, H, G=2, bound=None):
+    """A row of zeros gives the mean of what it sees; rows of numbers near the types' lower end and scales near it nearly so.  Masks hide
+    drafted tokens, and the contexts end inside a tile and inside a page."""
+    masks = [1, 3, 5, 11, 21, 33, 1, 3]
+    c = cases.tree_case(H, G, hd, [6, 2], [70, 33], fp8, dtype, 21)
+    q = c["q"] = c["q"].clone()
+    q[0] = 0.0
+    q[2, 0] = 0.0
+    q[2, 1:] *= 2.0 ** -126
+    q[3] *= 2.0 ** -124
+    q[4] *= 2.0 ** -110
+    q[7] = 0.0
+    compare_tree(ops, device, c, masks, 1.0 / math.sqrt(hd), bound)
+    compare_tree(ops, device, c, None, 1.0 / math.sqrt(hd), bound)
+    for scale in (1e-30, 1e-38, 1e-42):
+        compare_tree(ops, device, c, masks, scale, bound)
+
+
+# ------------------------------------------------------------------ scores of any size
+def scaled_token(pages, page, off, power):
+    """The pages with the numbers of one token (all heads) times 2^power."""
+    if isinstance(pages, Fp8Pages):
+        r = Fp8Pages(pages.codes.clone(), pages.exps.clone())
+        r.exps[page, :, off] = (r.exps[page, :, off].int() + power).to(torch.uint8)
+        return r
+    r = pages.clone()
+    r[page, :, off] = (r[page, :, off].to(F64) * 2.0 ** power).to(r.dtype)
+    return r
+
+
+def check_tree_large_scores(ops, device, fp8, dtype, hd, H, power, G=2, bound=None):
+    """A drafted token whose keys are 2^power times the others' takes everything in the rows that see it with a positive score and nothing
+    where the score is negative; the rows that do not see it do not notice, wherever it lies against the tiles."""
+    masks = [1, 3, 5, 11, 21, 33, 1, 3]
+    for lens in ([70, 33], [38, 131], [640, 130]):
+        c = cases.tree_case(H, G, hd, [6, 2], lens, fp8, dtype, 31, spread=0.25)
+        at = lens[0] - 6 + 1                                            # drafted token 1: rows 1 and 3 see it
+        c["k"] = scaled_token(c["k"], int(c["table"][0, at // PAGE]), at % PAGE, power)
+        hit = compare_tree(ops, device, c, masks, 0.1, bound)
+        if power < 30:
+            continue
+        # (the tolerance above grows with the scores; a score of 2^power leaves one token or none, and no rounding but the result's)
+        k, v = (cases._dense(c[n])[int(c["table"][0, at // PAGE]), :, at % PAGE] for n in ("k", "v"))
+        for row in (1, 3):
+            for h in range(H):
+                if float(k[h * G // H] @ c["q"][row, h].to(F64)) > 0:
+                    want = v[h * G // H]
+                    assert bool(((hit[row, h] - want).abs() <= 2.0 ** -7 * want.abs()).all()), (row, h)

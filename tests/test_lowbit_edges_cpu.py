@@ -1,0 +1,17 @@
+"""Tree attention and 4-bit products at the ends of their ranges: the plain PyTorch back end."""
+import pytest
+import torch
+
+import lowbit_edge_cases as edges
+from kotodama_b200.ops import TORCH_OPS
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_tiny_queries(fp8):
+    edges.check_tree_tiny_queries(TORCH_OPS, "cpu", fp8, torch.float32, 64, 4)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("power", [12, 40, 100])
+def test_large_scores(fp8, power):
+    edges.check_tree_large_scores(TORCH_OPS, "cpu", fp8, torch.float32, 64, 4, power)

@@ -3,9 +3,13 @@ import pytest
 import torch
 
 import lowbit_cases as cases
+import lowbit_edge_cases as edges
 from kotodama_b200.ops import get_ops
 
 pytestmark = pytest.mark.gpu
+DTYPES = [torch.bfloat16, torch.float32]
+HEADS = [4, 10, 32]                  # 12, 30 and 96 rows per KV head: one block of 16 rows, two, the kernel of 128 rows
+BOUNDS = [None, 5000]                # a block of threads per unit, the line of tiles
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -16,3 +20,24 @@ def test_many_units_of_one_tile(fp8, hd):
     sizes, lens = cases.ragged(300, 140, 6, 12)
     cases.check_tree(ops, "cuda", 40, 2, hd, sizes, lens, fp8, torch.bfloat16, True, bound=400)
     ops.check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H", HEADS)
+@pytest.mark.parametrize("bound", BOUNDS)
+def test_tiny_queries(fp8, dtype, hd, H, bound):
+    edges.check_tree_tiny_queries(get_ops("cuda"), "cuda", fp8, dtype, hd, H, bound=bound)
+    get_ops("cuda").check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H", HEADS)
+@pytest.mark.parametrize("bound", BOUNDS)
+def test_large_scores(fp8, dtype, hd, H, bound):
+    for power in (12, 40, 100):
+        edges.check_tree_large_scores(get_ops("cuda"), "cuda", fp8, dtype, hd, H, power, bound=bound)
+    get_ops("cuda").check_status()
