@@ -10,6 +10,11 @@ typedef __nv_bfloat16 bf16;
 namespace tree {
 
 constexpr int PAGE = 16, MAX_B = 1024;
+// 8-bit pages: most binary orders of magnitude between the powers of two of a unit's values for one unit of the output for all rows, so that
+// a probability near the maximum keeps f16's eleven bits beside the smallest of them.  Values further apart (hidden tokens count: what they
+// hold is not known to be small) have a unit per row, which depends on nothing that the row does not see or gives no weight.
+constexpr int SPREAD = 16;
+constexpr float NO_UNIT = -1e30f;                      // log2 of the unit of an output without a term
 
 struct TreeParams {
     const bf16* q;

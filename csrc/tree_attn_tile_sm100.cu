@@ -18,6 +18,8 @@
 //                need nothing from one another before the end of a unit.  8-bit pages: P is f16 in units of 2^-4 (at most 2^15 with the
 //                2^11 of lazy maxima: eleven bits down to 2^-18, off by at most 2^-29 below); the values' f16 carry the token's power
 //                of two relative to E, the unit's largest so far (off by at most 2^-39 of the largest); O is in units of 2^(E - 6).
+//                Values whose powers lie more than 2^SPREAD apart: as their codes, with a unit of O per row (apart_tile), so that a token
+//                that a row does not see or gives no weight takes nothing from it, however large it is.
 //
 // The groups run out of step: one computes while the products of the other run.  Query rows are double-buffered by unit.
 // Tokens that do not exist are masked in S and zeroed in the value tile (whatever the cache holds there).  Values of drafted tokens that
@@ -49,8 +51,9 @@ struct Lay {
     static constexpr int RING = KST * KT + RST * KT + (FP8 ? VST * VT : 0) + 2 * QT;
     static constexpr int EXPS = FP8 ? RST * 2 * TT : 0;
     static constexpr int FACT = FP8 ? SLOTS * TT * 4 : 0;
-    static constexpr int ROWBUF = 4 * TT * 4;
-    static constexpr int SMEM = 1024 + RING + EXPS + FACT + ROWBUF;
+    static constexpr int ROWBUF = (FP8 ? 6 : 4) * TT * 4;
+    static constexpr int VEXPS = FP8 ? SLOTS * TT : 0;
+    static constexpr int SMEM = 1024 + RING + EXPS + FACT + ROWBUF + VEXPS;
 };
 
 __device__ __forceinline__ void mma_f8_h(uint32_t d_tmem, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t acc) {
@@ -114,10 +117,62 @@ __device__ __noinline__ void scale_packed(uint32_t addr, int n, float f) {
     tc::tmem_st_wait();
 }
 
+constexpr int APART = -1;                              // for TileMeta::E: a unit per row, values as their codes
 struct TileMeta {
     uint32_t valid[4], odd[4];                         // bits of the tile's tokens: exist; drafted with values that are not finite
-    int E;                                             // biased exponent of the output's unit (8-bit pages)
+    int E;                                             // 8-bit pages: biased exponent of the output's unit, or APART
 };
+
+// A tile's softmax with a unit of O per row, 2^D times that of the sums (SPREAD in tree_attn.cuh): probabilities carry their value's power
+// of two relative to it.  The maximum m as it is, the sum l in units of 2^-SHIFT, by the threads of a warp, a row each.
+struct RowState {
+    float m, l, D;
+};
+template <int HD>
+__device__ __noinline__ RowState apart_tile(uint32_t tmem_s, uint32_t tmem_o, const float* kf, const uint8_t* ev, unsigned long long seen0,
+                                            unsigned long long seen1, float scale, bool begun, RowState st) {
+    float mx = -INFINITY, y = -INFINITY;
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t sees32 = (uint32_t)((q & 2 ? seen1 : seen0) >> (32 * (q & 1)));
+        float x[32];
+        tc::tmem_ld32(tmem_s + 32 * q, reinterpret_cast<uint32_t*>(x));
+        tc::tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            const float v = sees32 >> i & 1u ? x[i] * kf[32 * q + i] * scale : -INFINITY;
+            mx = fmaxf(mx, v);
+            y = fmaxf(y, v + (float)((int)ev[32 * q + i] - 127));
+        }
+    }
+    const float m = fmaxf(st.m, mx), at = m == -INFINITY ? 0.f : m;
+    if (m != -INFINITY) st.l *= exp2f(st.m - m);
+    const float D = fmaxf(st.D + (st.m - m), NO_UNIT), to = y - at > D + 11.f ? y - at - 4.f : D;      // (NaN: no maximum yet)
+    if (begun && __any_sync(0xffffffffu, to != D)) scale_columns(tmem_o, HD, exp2f(D - to));
+    float sum = 0.f;
+#pragma unroll 1
+    for (int q = 0; q < 4; ++q) {
+        const uint32_t sees32 = (uint32_t)((q & 2 ? seen1 : seen0) >> (32 * (q & 1)));
+        float x[32];
+        tc::tmem_ld32(tmem_s + 32 * q, reinterpret_cast<uint32_t*>(x));
+        tc::tmem_ld_wait();
+        uint32_t pk[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+            float p[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const float a = sees32 >> (i + e) & 1u ? x[i + e] * kf[32 * q + i + e] * scale - at : -INFINITY;
+                sum += exp2f(a);
+                p[e] = exp2f(a + ((float)((int)ev[32 * q + i + e] - 127) - to));
+            }
+            pk[i >> 1] = pack_f16(p[0], p[1]);
+        }
+        tc::tmem_st16(tmem_s + 16 * q, pk);
+    }
+    tc::tmem_st_wait();
+    return RowState{m, st.l + 16.f * sum, to};
+}
 
 template <bool FP8, int HD>
 __global__ void __launch_bounds__(THREADS, 1)
@@ -131,7 +186,8 @@ tree_tile_kernel(const TreeParams p) {
     uint8_t* exps = smem + L::RING;                                    // [RST][2][TT] exponents of keys and values
     float* fact = reinterpret_cast<float*>(exps + L::EXPS);            // [SLOTS][TT] factors of scores, to log2 units
     uint8_t* sQ = smem + L::RING - 2 * L::QT;                          // two query tiles, staged like keys
-    float* row_buf = reinterpret_cast<float*>(exps + L::EXPS + L::FACT);   // [2 groups][TT] maxima, then sums
+    float* row_buf = reinterpret_cast<float*>(exps + L::EXPS + L::FACT);   // [2 groups][TT] maxima, then sums, then (8-bit pages) units of O
+    uint8_t* vexps = exps + L::EXPS + L::FACT + L::ROWBUF;             // [SLOTS][TT] exponents of values, of tiles with a unit per row
     __shared__ int uoff[MAX_B + 1];
     __shared__ int wsum[THREADS / 32];
     __shared__ uint64_t k_full[L::KST], k_empty[L::KST], r_full[L::RST], r_empty[L::RST], v_ready[L::VST], f_ready[SLOTS], pv_done[L::VST], s_full[2], p_ready[2], q_ready[2],
@@ -140,7 +196,6 @@ tree_tile_kernel(const TreeParams p) {
     __shared__ uint32_t there_k[SLOTS];                // the same of key tile j % SLOTS
     __shared__ TileMeta meta[SLOTS];                   // of tile j at j % SLOTS
     __shared__ uint32_t tmem_slot;
-    __shared__ int unit_E[2];
     __shared__ Segment segs[SEGS];
     __shared__ float q_scale[FP8 ? 2 * TT : 1];        // the power of two taken out of a query row
     __shared__ uint64_t seg_ready[SEGS];
@@ -344,7 +399,7 @@ tree_tile_kernel(const TreeParams p) {
         // ------------------------------------------------------------ what of a tile exists, which drafted tokens are odd, factors
         Segment sg = segment(0);
         int first = 0, seg = 0;                        // tile at which sg begins, its number
-        uint32_t E = 0;
+        uint32_t E = 0, low = 255;
         for (int j = 0; j < n_tiles; ++j) {
             if (j - first == sg.t1 - sg.t0) {
                 sg = segment(++seg);
@@ -360,7 +415,7 @@ tree_tile_kernel(const TreeParams p) {
             const bool edge = have != 0xffu || base + TT > prefix;
             const uint8_t* e = exps + rst * 2 * TT;
             TileMeta& mt = meta[j % SLOTS];
-            uint32_t top = 0;
+            uint32_t top = 0, bot = 255;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {              // 32 tokens at a time
                 const int t = w * 32 + lane, tok = base + t;
@@ -368,7 +423,10 @@ tree_tile_kernel(const TreeParams p) {
                 if constexpr (FP8) {
                     fact[(j % SLOTS) * TT + t] = pow2_biased(e[t]) * p.scale_log2;
                     const uint32_t ev = e[TT + t];
-                    if (valid && ev != 255u) top = max(top, ev);
+                    if (valid && ev != 255u) {
+                        top = max(top, ev);
+                        bot = min(bot, ev);
+                    }
                 }
                 uint32_t vword = 0xffffffffu, oword = 0u;
                 if (edge) {
@@ -393,8 +451,14 @@ tree_tile_kernel(const TreeParams p) {
             }
             if constexpr (FP8) {                       // the unit of the output: largest exponent of the unit's values so far
                 top = __reduce_max_sync(0xffffffffu, top);
+                bot = __reduce_min_sync(0xffffffffu, bot);
                 E = j == first ? top : max(E, top);
-                if (lane == 0) mt.E = (int)E;
+                low = j == first ? bot : min(low, bot);
+                const bool apart = (int)E - (int)low > SPREAD;
+                if (lane == 0) mt.E = apart ? APART : (int)E;
+                if (apart)
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) vexps[(j % SLOTS) * TT + w * 32 + lane] = e[TT + w * 32 + lane];
             }
             __syncwarp();
             if (lane == 0) {
@@ -469,9 +533,9 @@ tree_tile_kernel(const TreeParams p) {
             const uint32_t vword = mt.valid[warp - W_VAL];
             uint8_t* op = sV + vs * L::VT;
             if constexpr (FP8) {
-                // the token's factor, an f16 power of two of at most 2^6 (twice)
+                // the token's factor, an f16 power of two of at most 2^6 (twice); none where the probabilities carry it
                 const uint8_t* raw = sR + rst * L::KT;
-                const int ev = exps[rst * 2 * TT + TT + t], w = ev == 255 ? 0 : min(ev - mt.E, 0) + 6;
+                const int ev = exps[rst * 2 * TT + TT + t], w = ev == 255 || mt.E == APART ? 0 : min(ev - mt.E, 0) + 6;
                 const uint32_t one = !(vword >> lane & 1u) || w < -24 ? 0u : w >= -14 ? (uint32_t)(w + 15) << 10 : 1u << (w + 24);
                 const uint32_t mine = one | one << 16;
                 // codes -> f16: a warp takes whole rows, 16 codes per lane, so that loads and stores use all banks
@@ -551,6 +615,8 @@ tree_tile_kernel(const TreeParams p) {
             }
             float m_used = -INFINITY, l = 0.f;
             int E = 0;
+            constexpr int OWN = -2;                    // for E: O is in units of 2^D times that of the sums, not of 2^(E - 137)
+            float& D = row_buf[(FP8 ? 4 + g : 0) * TT + r];        // (E == OWN)
             bool begun = false;                        // the group has had a tile of this segment
             for (int at = (g ^ j0) & 1; at < len; at += 2) {
                 const int j = j0 + at, vs = j % L::VST, base = (sg.t0 + at) * TT;
@@ -572,13 +638,27 @@ tree_tile_kernel(const TreeParams p) {
                 if (live) {
                     const float* kf = fact + (j % SLOTS) * TT;
                     const int E_new = FP8 ? mt.E : 0;
-                    if (FP8 && begun && E_new != E) scale_columns(tmem_o, HD, exp2f((float)(E - E_new)));
-                    E = E_new;
+                    int q0 = 0;
+                    if (FP8 && E_new != E) {
+                        if (E_new == APART) {
+                            if (E != OWN) D = begun ? (float)(E - 137) : NO_UNIT;
+                            const RowState rs = apart_tile<HD>(tmem_s, tmem_o, kf, vexps + (j % SLOTS) * TT, seen[0], seen[1], scale, begun,
+                                                               RowState{m_used, l, D});
+                            m_used = rs.m;
+                            l = rs.l;
+                            D = rs.D;
+                            E = OWN;
+                            q0 = 4;
+                        } else {
+                            if (begun) scale_columns(tmem_o, HD, exp2f((float)(E - E_new)));
+                            E = E_new;
+                        }
+                    }
                     const float2 sc2 = make_float2(scale, scale);
                     float2 sum2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
                     // 32 columns at a time.  The loop stays rolled: unrolled, the instruction cache is what bounds this kernel
 #pragma unroll 1
-                    for (int q = 0; q < 4; ++q) {
+                    for (int q = q0; q < 4; ++q) {
                         float x[32];
                         tc::tmem_ld32(tmem_s + 32 * q, reinterpret_cast<uint32_t*>(x));
                         tc::tmem_ld_wait();
@@ -696,7 +776,7 @@ tree_tile_kernel(const TreeParams p) {
             // ---- the unit's rows, as far as this part has them: the groups' results together
             row_buf[g * TT + r] = m_used;
             row_buf[(2 + g) * TT + r] = FP8 ? l * 0.0625f : l;
-            if (lane == 0 && (warp & 3) == 0) unit_E[g] = E;
+            if (FP8) D = E == OWN ? exp2f(D) : pow2_biased(E) * 9.765625e-4f;     // 2^(E - 127 - 6) and the 2^4 of P
             if (!exchange(&xch, n_x)) { ok = false; break; }
             const int j_last = j0 + len - 1;
             if (!tc::mbar_wait(&pv_done[j_last % L::VST], (uint32_t)(j_last / L::VST) & 1u, abort_flag)) { ok = false; break; }
@@ -709,9 +789,9 @@ tree_tile_kernel(const TreeParams p) {
                 // (a sum without a maximum is zero, or NaN and has to get through)
                 const float sum = (m0 == -INFINITY ? row_buf[2 * TT + r] : row_buf[2 * TT + r] * f0) +
                                   (m1 == -INFINITY ? row_buf[3 * TT + r] : row_buf[3 * TT + r] * f1);
-                if constexpr (FP8) {                   // 2^(E - 127 - 6) and the 2^4 of P
-                    f0 *= pow2_biased(unit_E[0]) * 9.765625e-4f;
-                    f1 *= pow2_biased(unit_E[1]) * 9.765625e-4f;
+                if constexpr (FP8) {
+                    f0 *= row_buf[4 * TT + r];
+                    f1 *= row_buf[5 * TT + r];
                 }
                 if (done) {
                     const float inv = sum == 0.f ? 0.f : 1.f / sum;

@@ -72,3 +72,38 @@ def check_tree_large_scores(ops, device, fp8, dtype, hd, H, power, G=2, bound=No
                 if float(k[h * G // H] @ c["q"][row, h].to(F64)) > 0:
                     want = v[h * G // H]
                     assert bool(((hit[row, h] - want).abs() <= 2.0 ** -7 * want.abs()).all()), (row, h)
+
+
+# ------------------------------------------------------------------ values of any size
+def check_tree_hidden_large(ops, device, fp8, dtype, hd, H, power, G=2, bound=None):
+    """A drafted token with finite values of 2^power times the others' does not reach the rows that do not see it, wherever it lies
+    against the tiles."""
+    masks = [1, 3, 5, 11, 21, 33, 1, 3]
+    for lens in ([70, 33], [38, 131], [640, 130]):
+        c = cases.tree_case(H, G, hd, [6, 2], lens, fp8, dtype, 31, spread=0.25)
+        at = lens[0] - 6 + 1                                            # drafted token 1: rows 1 and 3 see it
+        page, off = int(c["table"][0, at // PAGE]), at % PAGE
+        c["v"] = scaled_token(c["v"], page, off, power)
+        compare_tree(ops, device, c, masks, 0.1, bound)
+
+
+def check_tree_unlikely_large(ops, device, fp8, dtype, hd, H, power, where, G=2, bound=None):
+    """A seen token whose probability is nearly zero and whose values are huge weighs just their product."""
+    lens = [400, 37]
+    c = cases.tree_case(H, G, hd, [6, 2], lens, fp8, dtype, 41, spread=0.25)
+    c["q"] = (c["q"].float().abs() + 0.5).to(dtype)
+    page, off = int(c["table"][0, where // PAGE]), where % PAGE
+    c["v"] = scaled_token(c["v"], page, off, power)
+    if fp8:
+        c["k"] = Fp8Pages(c["k"].codes.clone(), c["k"].exps.clone())
+        c["k"].codes[page, :, off] = torch.tensor(-256.0).to(torch.float8_e4m3fn)
+        c["k"].exps[page, :, off] = 127 - 6                             # -4
+    else:
+        c["k"] = c["k"].clone()
+        c["k"][page, :, off] = -4.0
+    compare_tree(ops, device, c, [1, 3, 5, 11, 21, 33, 1, 3], 0.125 * (64 / hd), bound)
+
+
+def check_tree_wide_values(ops, device, hd, H, G=2, bound=None):
+    """Values of every size from token to token."""
+    cases.check_tree(ops, device, H, G, hd, [6, 0, 2, 9], [700, 5, 33, 300], True, torch.bfloat16, True, seed=3, spread=7.0, bound=bound)

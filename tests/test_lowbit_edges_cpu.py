@@ -15,3 +15,15 @@ def test_tiny_queries(fp8):
 @pytest.mark.parametrize("power", [12, 40, 100])
 def test_large_scores(fp8, power):
     edges.check_tree_large_scores(TORCH_OPS, "cpu", fp8, torch.float32, 64, 4, power)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("power", [12, 40, 100])
+def test_hidden_large_values(fp8, power):
+    edges.check_tree_hidden_large(TORCH_OPS, "cpu", fp8, torch.float32, 64, 4, power)
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("power,where", [(40, 3), (60, 200), (80, 250)])
+def test_large_values_of_unlikely_tokens(fp8, power, where):
+    edges.check_tree_unlikely_large(TORCH_OPS, "cpu", fp8, torch.float32, 64, 4, power, where)

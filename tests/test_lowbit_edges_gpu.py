@@ -41,3 +41,33 @@ def test_large_scores(fp8, dtype, hd, H, bound):
     for power in (12, 40, 100):
         edges.check_tree_large_scores(get_ops("cuda"), "cuda", fp8, dtype, hd, H, power, bound=bound)
     get_ops("cuda").check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H", HEADS)
+@pytest.mark.parametrize("bound", BOUNDS)
+def test_hidden_large_values(fp8, dtype, hd, H, bound):
+    for power in (12, 17, 24, 40, 100):
+        edges.check_tree_hidden_large(get_ops("cuda"), "cuda", fp8, dtype, hd, H, power, bound=bound)
+    get_ops("cuda").check_status()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H", HEADS)
+@pytest.mark.parametrize("bound", BOUNDS)
+def test_large_values_of_unlikely_tokens(fp8, dtype, hd, H, bound):
+    for power, where in ((40, 3), (60, 3), (60, 200), (80, 250)):
+        edges.check_tree_unlikely_large(get_ops("cuda"), "cuda", fp8, dtype, hd, H, power, where, bound=bound)
+    get_ops("cuda").check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("H", HEADS)
+@pytest.mark.parametrize("bound", BOUNDS)
+def test_values_of_every_size(hd, H, bound):
+    edges.check_tree_wide_values(get_ops("cuda"), "cuda", hd, H, bound=bound)
+    get_ops("cuda").check_status()
