@@ -332,6 +332,8 @@ class CudaOps(TorchOps):
         M, K = a.shape
         N, inputs = b.shape
         dtype, dev, packed = a.dtype, a.get_device(), b.packed
+        if accumulate and out is None:
+            raise KernelError("a product that is added to its output needs one")
         if out is None:
             out = torch.empty(M, N, device=a.device, dtype=dtype)
             good = True

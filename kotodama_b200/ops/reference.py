@@ -230,6 +230,8 @@ class TorchOps:
         an ``Fp8Weight``: the product then runs in block-scaled fp8; or an ``Int4Weight``: 4-bit codes times the
         activations, sums and scales in fp32."""
         if isinstance(b, Int4Weight):
+            if accumulate and out is None:
+                raise ValueError("a product that is added to its output needs one")
             r = _f(a) @ b.dense().to(_f(a).dtype).t()
             if residual is not None:
                 r = r + _f(residual)

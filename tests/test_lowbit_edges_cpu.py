@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import lowbit_cases as cases
 import lowbit_edge_cases as edges
 from kotodama_b200.ops import TORCH_OPS
 
@@ -27,3 +28,10 @@ def test_hidden_large_values(fp8, power):
 @pytest.mark.parametrize("power,where", [(40, 3), (60, 200), (80, 250)])
 def test_large_values_of_unlikely_tokens(fp8, power, where):
     edges.check_tree_unlikely_large(TORCH_OPS, "cpu", fp8, torch.float32, 64, 4, power, where)
+
+
+# ------------------------------------------------------------------ 4-bit products
+def test_products_added_to_no_output_are_refused():
+    x, w = cases.int4_case(3, 32, 64, 64, 0)
+    with pytest.raises(ValueError, match="output"):
+        TORCH_OPS.gemm_nt(x.float(), w, accumulate=True)

@@ -4,7 +4,8 @@ import torch
 
 import lowbit_cases as cases
 import lowbit_edge_cases as edges
-from kotodama_b200.ops import get_ops
+from kotodama_b200.ops import Int4Weight, get_ops
+from kotodama_b200.ops.cuda import KernelError
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.bfloat16, torch.float32]
@@ -71,3 +72,13 @@ def test_large_values_of_unlikely_tokens(fp8, dtype, hd, H, bound):
 def test_values_of_every_size(hd, H, bound):
     edges.check_tree_wide_values(get_ops("cuda"), "cuda", hd, H, bound=bound)
     get_ops("cuda").check_status()
+
+
+# ------------------------------------------------------------------ 4-bit products
+def test_products_added_to_no_output_are_refused():
+    ops = get_ops("cuda")
+    for M in (3, 40):
+        x, w = cases.int4_case(M, 32, 64, 64, 0)
+        w = Int4Weight(w.packed.cuda(), w.scales.cuda(), w.shape, w.group)
+        with pytest.raises(KernelError, match="output"):
+            ops.gemm_nt(x.cuda(), w, accumulate=True)
