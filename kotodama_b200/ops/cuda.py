@@ -1085,9 +1085,11 @@ class CudaOps(TorchOps):
         if not good:
             raise KernelError(f"tree attention: {B} lengths, page lists {tuple(page_table.shape)}, boundaries "
                               f"{None if cu_seqlens is None else tuple(cu_seqlens.shape)}, {N} rows; tables are dense int32, masks int64 per row")
-        width = page_table.shape[1]
-        if N == 0 or B == 0 or width == 0:
+        if N == 0 or B == 0:
             return out if given else out.zero_()
+        if page_table.shape[1] == 0:                   # no sequence has a page: its rows are zero, and recorded
+            page_table = page_table.new_full((B, 1), -1)
+        width = page_table.shape[1]
         q_at, out_at, out_row, floats = q.data_ptr(), out.data_ptr(), out.stride(0), 0
         if dtype == torch.bfloat16 and scale > 0 and row % 8 == 0 and out_row % 4 == 0 and q_at % 16 == 0 and out_at % 8 == 0:
             floats = self._tree_floats(N, B, H, n_kv, hd, max_q, max_ctx, int(fp8))

@@ -107,3 +107,19 @@ def check_tree_unlikely_large(ops, device, fp8, dtype, hd, H, power, where, G=2,
 def check_tree_wide_values(ops, device, hd, H, G=2, bound=None):
     """Values of every size from token to token."""
     cases.check_tree(ops, device, H, G, hd, [6, 0, 2, 9], [700, 5, 33, 300], True, torch.bfloat16, True, seed=3, spread=7.0, bound=bound)
+
+
+# ------------------------------------------------------------------ a page list without columns
+def check_tree_without_pages(ops, device, fp8, dtype, H):
+    """Sequences have rows and no page lists: zero rows, in a given output too; what lies behind the last sequence is left."""
+    G, hd = 2, 64
+    pages = Fp8Pages.zeros(1, G, hd, device) if fp8 else torch.ones(1, G, PAGE, hd, device=device, dtype=dtype)
+    q = torch.ones(5, H, hd, device=device, dtype=dtype)
+    t = lambda *a: torch.tensor(a, dtype=torch.int32, device=device)
+    table = torch.zeros(2, 0, dtype=torch.int32, device=device)
+    for lens in ((3, 0), (40, 0)):
+        out = torch.full((5, H * hd), 7.0, device=device, dtype=dtype)
+        args = (q, pages, pages, table, t(*lens), t(0, 3, 3), 3, 40, 0.1)
+        got = ops.paged_tree_attention(*args, None, out)
+        assert got is out and bool((out[:3] == 0).all()) and bool((out[3:] == 7).all())
+        assert bool((ops.paged_tree_attention(*args) == 0).all())

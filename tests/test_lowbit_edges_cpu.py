@@ -30,6 +30,11 @@ def test_large_values_of_unlikely_tokens(fp8, power, where):
     edges.check_tree_unlikely_large(TORCH_OPS, "cpu", fp8, torch.float32, 64, 4, power, where)
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_page_lists_without_columns(fp8):
+    edges.check_tree_without_pages(TORCH_OPS, "cpu", fp8, torch.float32, 4)
+
+
 # ------------------------------------------------------------------ 4-bit products
 def test_products_added_to_no_output_are_refused():
     x, w = cases.int4_case(3, 32, 64, 64, 0)

@@ -74,6 +74,17 @@ def test_values_of_every_size(hd, H, bound):
     get_ops("cuda").check_status()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("H", [4, 64])
+def test_page_lists_without_columns(fp8, dtype, H):
+    ops = get_ops("cuda")
+    edges.check_tree_without_pages(ops, "cuda", fp8, dtype, H)
+    with pytest.raises(KernelError, match="status 6"):
+        ops.check_status()
+    ops.check_status()
+
+
 # ------------------------------------------------------------------ 4-bit products
 def test_products_added_to_no_output_are_refused():
     ops = get_ops("cuda")
