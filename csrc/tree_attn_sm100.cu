@@ -621,7 +621,10 @@ tree_merge_kernel(const TreeParams p, int ROWS, int TILE, int workers, int per, 
     __shared__ float so[WPR > 1 ? WPR : 1][HD], sml[WPR][2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % WPR;
     const long long row = (long long)blockIdx.x * RPB + warp / WPR;
-    if (row >= (long long)p.N * p.H) return;           // (with several warps per row the whole block)
+    if (row >= (long long)p.N * p.H) {                 // (with several warps per row the whole block)
+        kb_dep_wait();
+        return;
+    }
     // What the sequences are was known before the kernel ahead began (it lets this one start after its own wait)
     const int n = (int)(row / p.H), head = (int)(row % p.H), h = head / p.G;
     int b = n;
