@@ -125,7 +125,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
         // ------------------------------------------------------------ sums of a group times the row's scale
         const int row = (warp & 3) * 32 + lane, tile = (n0 + row) >> 4, col0 = (warp >> 2) * R::AC;
         const bool live = tile < s.nt;
-        const float unit = row & 8 ? UNIT1 : UNIT0;
+        const float unit = row & 8 ? UNIT1 : UNIT0;    // (of the sums, not of the scales: the largest of those times it would overflow)
         const uint32_t src = tmem_acc + ((uint32_t)((warp & 3) * 32) << 16) + col0;
         constexpr int G = 2 / PG, PIECE = R::AC > 32 ? 16 : 32;        // groups of a turn; columns of a load
         const int n_groups = PG == 2 ? turns : nb;
@@ -153,7 +153,7 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
                 copy_wait<SCALES - 2>();
                 const uint32_t both = ld_shared(slots + (g % SCALES) * (R::FLUSH * 128));              // (rows that do not exist: anything)
                 fetch(g + SCALES - 1);
-                f[h].x = f[h].y = __uint_as_float(row & 8 ? both & 0xffff0000u : both << 16) * unit;
+                f[h].x = f[h].y = __uint_as_float(row & 8 ? both & 0xffff0000u : both << 16);
             }
             ok = tc::mbar_wait(&acc_full[set], (uint32_t)(i / R::SETS) & 1u, abort_flag);
             if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
@@ -184,13 +184,13 @@ int4_tile_kernel(const __grid_constant__ CUtensorMap x, const uint4* packed, con
         const int n = n0 + row;
         if (slices > 1) {                              // (every product has read the ring: the last turn's sums were here)
 #pragma unroll
-            for (int i = 0; i < R::AC; ++i) part[(col0 + i) * PITCH + row] = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+            for (int i = 0; i < R::AC; ++i) part[(col0 + i) * PITCH + row] = (i & 1 ? acc[i / 2].y : acc[i / 2].x) * unit;
         } else if (n < s.N && ok) {
 #pragma unroll
             for (int i = 0; i < R::AC; ++i) {
                 const int m = m0 + col0 + i;
                 if (m >= s.M) break;
-                float v = i & 1 ? acc[i / 2].y : acc[i / 2].x;
+                float v = (i & 1 ? acc[i / 2].y : acc[i / 2].x) * unit;
                 if (c) v += __bfloat162float(c[(long long)m * s.c_stride + n]);
                 y[(long long)m * s.y_stride + n] = __float2bfloat16(v);
             }

@@ -21,8 +21,10 @@ OBJ_DIR = ROOT / "build" / "obj"
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden"]
-# sources of the 32-bit mode (and of fp32 statistics) keep IEEE division, square roots and full-precision functions
-PRECISE = {"block", "moe", "gemm_f32", "latent_attn", "paged_attn", "delta", "delta_sm100", "cache_fp8", "tree_attn"}
+# sources of the 32-bit mode (and of fp32 statistics) keep IEEE division, square roots and full-precision functions; 4-bit products keep
+# scales below the normal numbers
+PRECISE = {"block", "moe", "gemm_f32", "latent_attn", "paged_attn", "delta", "delta_sm100", "cache_fp8", "tree_attn", "gemm_int4",
+           "gemm_int4_tile_sm100"}
 
 _lib = None
 

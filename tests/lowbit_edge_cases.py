@@ -5,7 +5,7 @@ import math
 import torch
 
 import lowbit_cases as cases
-from kotodama_b200.ops import Fp8Pages
+from kotodama_b200.ops import Fp8Pages, Int4Weight
 
 F64 = torch.float64
 PAGE = cases.PAGE
@@ -123,3 +123,21 @@ def check_tree_without_pages(ops, device, fp8, dtype, H):
         got = ops.paged_tree_attention(*args, None, out)
         assert got is out and bool((out[:3] == 0).all()) and bool((out[3:] == 7).all())
         assert bool((ops.paged_tree_attention(*args) == 0).all())
+
+
+# ------------------------------------------------------------------ 4-bit products
+def check_int4_scales(ops, device, dtype, M, N, K, group, scale_power, x_power):
+    """Scales near the upper and below the lower end of bf16's normal numbers count as what they are."""
+    x, w = cases.int4_case(M, N, K, group, 3)
+    x = (x.to(F64) * 2.0 ** x_power).to(dtype)
+    w = Int4Weight(w.packed, (w.scales.to(F64) * 2.0 ** scale_power).to(torch.bfloat16), w.shape, group)
+    assert bool(torch.isfinite(w.scales).all()) and bool((w.scales != 0).all())
+    want = x.to(F64) @ cases.plain_int4(w)[0].t()
+    got = ops.gemm_nt(x.to(device), Int4Weight(w.packed.to(device), w.scales.to(device), w.shape, group)).cpu().to(F64)
+    held = 143 * (x.to(F64).abs() @ (w.scales.to(F64).permute(0, 3, 2, 1).reshape(-1, w.scales.shape[1])[:N].repeat_interleave(group, 1)[:, :K]).t())
+    tol = 2.0 ** -8 * want.abs() + 8 * 2.0 ** -22 * held if dtype == torch.bfloat16 else 2.0 ** -20 * held
+    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).nan_to_num(math.inf).max())
+
+
+INT4_SCALE_CASES = [(3, 40, 200, 128), (16, 96, 512, 64), (20, 130, 1032, 128), (64, 48, 768, 64), (100, 100, 1000, 128)]
+INT4_SCALE_POWERS = [(124, -100), (122, -60), (-128, 100), (-130, 60)]

@@ -40,3 +40,8 @@ def test_products_added_to_no_output_are_refused():
     x, w = cases.int4_case(3, 32, 64, 64, 0)
     with pytest.raises(ValueError, match="output"):
         TORCH_OPS.gemm_nt(x.float(), w, accumulate=True)
+
+
+@pytest.mark.parametrize("powers", edges.INT4_SCALE_POWERS)
+def test_scales_of_any_size(powers):
+    edges.check_int4_scales(TORCH_OPS, "cpu", torch.float32, 3, 40, 200, 128, *powers)

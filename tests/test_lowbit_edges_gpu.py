@@ -93,3 +93,11 @@ def test_products_added_to_no_output_are_refused():
         w = Int4Weight(w.packed.cuda(), w.scales.cuda(), w.shape, w.group)
         with pytest.raises(KernelError, match="output"):
             ops.gemm_nt(x.cuda(), w, accumulate=True)
+
+
+@pytest.mark.parametrize("case", edges.INT4_SCALE_CASES, ids=str)
+@pytest.mark.parametrize("powers", edges.INT4_SCALE_POWERS)
+def test_scales_of_any_size(case, powers):
+    ops = get_ops("cuda")
+    edges.check_int4_scales(ops, "cuda", torch.bfloat16, *case, *powers)
+    ops.check_status()
