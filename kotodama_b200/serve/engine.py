@@ -95,7 +95,7 @@ class ServingEngine:
                  max_ctx: Optional[int] = None, ops: Any = None, tp: Any = None,
                  prefill_batch_tokens: int = 8192, prefill_portion: int = 0, kv_dtype: Optional[str] = None, weight_bits: int = 16) -> None:
         """``kv_dtype`` "fp8": keys and values of the cache in 8 bits (one power of two per token and head); ``weight_bits`` 4: the layers'
-        projections in 4 bits (one scale per 128 inputs), in bf16 passes on CUDA.  Llama family, one GPU."""
+        projections in 4 bits (one scale per 128 inputs).  Llama family, one GPU, on CUDA in bf16 passes."""
         self.device = torch.device(device)
         self.dtype = dtype
         self.model = model.eval()
@@ -110,8 +110,8 @@ class ServingEngine:
         if kv_dtype is not None or weight_bits != 16:
             if not getattr(runner_class(self.model), "low_bits", False) or tp is not None:
                 raise ValueError("an 8-bit cache and 4-bit weights are for the Llama family, on one GPU")
-            if weight_bits == 4 and self.device.type == "cuda" and dtype != torch.bfloat16:
-                raise ValueError(f"4-bit weights on CUDA are for bf16 passes, not {dtype}")
+            if self.device.type == "cuda" and dtype != torch.bfloat16:
+                raise ValueError(f"an 8-bit cache and 4-bit weights on CUDA are for bf16 passes, not {dtype}")
             if kv_dtype == "fp8" and (self.cfg.head_dim % 16 or self.cfg.head_dim > 256):
                 raise ValueError(f"an 8-bit cache has heads of a multiple of 16, at most 256; not {self.cfg.head_dim}")
         self.runner = make_runner(self)

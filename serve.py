@@ -83,7 +83,7 @@ def main() -> None:
                     help="default: bfloat16 on CUDA, float32 on CPU; float32 on CUDA for families with 32-bit kernels")
     ap.add_argument("--prefill_portion", type=int, default=0,
                     help="most prompt tokens of one request per step (0: whole prompts); families that continue a cached context")
-    ap.add_argument("--kv_cache", default=None, choices=["fp8"], help="keys and values of the cache in 8 bits (Llama family, one GPU)")
+    ap.add_argument("--kv_cache", default=None, choices=["fp8"], help="keys and values of the cache in 8 bits (Llama family, one GPU; bfloat16 on CUDA)")
     ap.add_argument("--weight_bits", type=int, default=16, choices=[4, 16],
                     help="4: the layers' projections in 4 bits (Llama family, one GPU; bfloat16 on CUDA)")
     args = ap.parse_args()

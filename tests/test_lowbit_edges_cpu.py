@@ -4,7 +4,10 @@ import torch
 
 import lowbit_cases as cases
 import lowbit_edge_cases as edges
+from kotodama_b200.config import MODEL_PRESETS, ModelConfig
+from kotodama_b200.models.llama import KotodamaModel
 from kotodama_b200.ops import TORCH_OPS
+from kotodama_b200.serve.engine import ServingEngine
 
 
 @pytest.mark.parametrize("fp8", [False, True])
@@ -45,3 +48,13 @@ def test_products_added_to_no_output_are_refused():
 @pytest.mark.parametrize("powers", edges.INT4_SCALE_POWERS)
 def test_scales_of_any_size(powers):
     edges.check_int4_scales(TORCH_OPS, "cpu", torch.float32, 3, 40, 200, 128, *powers)
+
+
+# ------------------------------------------------------------------ the engine
+@pytest.mark.parametrize("low", [dict(kv_dtype="fp8"), dict(weight_bits=4)], ids=str)
+def test_low_bits_on_cuda_are_for_bf16_passes(low):
+    """The Llama family's kernels read and write bf16; refused before the GPU is asked for anything."""
+    model = KotodamaModel(ModelConfig(**MODEL_PRESETS["smoke"])).eval()
+    for dtype in (torch.float32, torch.float16):
+        with pytest.raises(ValueError, match="bf16"):
+            ServingEngine(model, device="cuda", dtype=dtype, ops=TORCH_OPS, max_batch=1, max_ctx=32, **low)
