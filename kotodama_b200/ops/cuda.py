@@ -1062,6 +1062,10 @@ class CudaOps(TorchOps):
             kp, ke, vp, ve = k_pages.data_ptr(), None, v_pages.data_ptr(), None
         pages, n_kv, size, d = k_pages.shape
         row, head, inner = q.stride()
+        if H == 1:                                     # (the stride of a dimension of one says nothing)
+            head = hd
+        if N == 1:
+            row = H * hd
         if given:
             good = out.shape == (N, H * hd) and out.dtype == dtype and out.stride(1) == 1 and out.get_device() == dev
         else:
@@ -1090,7 +1094,7 @@ class CudaOps(TorchOps):
         if page_table.shape[1] == 0:                   # no sequence has a page: its rows are zero, and recorded
             page_table = page_table.new_full((B, 1), -1)
         width = page_table.shape[1]
-        q_at, out_at, out_row, floats = q.data_ptr(), out.data_ptr(), out.stride(0), 0
+        q_at, out_at, out_row, floats = q.data_ptr(), out.data_ptr(), out.stride(0) if N > 1 else H * hd, 0
         if dtype == torch.bfloat16 and scale > 0 and row % 8 == 0 and out_row % 4 == 0 and q_at % 16 == 0 and out_at % 8 == 0:
             floats = self._tree_floats(N, B, H, n_kv, hd, max_q, max_ctx, int(fp8))
         where = (q_at, row, kp, ke, vp, ve, page_table.data_ptr(), width, pages, ctx_lens.data_ptr(), cu, B, tree, out_at, out_row, N, H, n_kv, hd,

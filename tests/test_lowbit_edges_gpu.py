@@ -85,6 +85,34 @@ def test_page_lists_without_columns(fp8, dtype, H):
     ops.check_status()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_single_head_or_row_has_any_stride(fp8):
+    """Whatever stride a dimension of one has, the call is the dense one's, by the same kernel."""
+    ops = get_ops("cuda")
+    names = []
+    launch = type(ops)._launch
+
+    class Listen(type(ops)):
+        def _launch(self, fn, *args):
+            names.append(fn)
+            return launch(self, fn, *args)
+
+    for H, G, sizes, lens in ((1, 1, [3, 2], [40, 9]), (4, 2, [1], [33]), (1, 1, [1], [20])):
+        c = cases.tree_case(H, G, 64, sizes, lens, fp8, torch.bfloat16, 4)
+        t = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+        args = (cases._put(c["k"], "cuda"), cases._put(c["v"], "cuda"), c["table"].cuda(), t(c["lens"]), t(c["cu"]), max(sizes), max(lens), 0.125)
+        q, N = c["q"].cuda(), sum(sizes)
+        odd = torch.empty(4096, device="cuda", dtype=torch.bfloat16).as_strided(q.shape, (H * 64 if N > 1 else 1003, 64 if H > 1 else 13, 1))
+        odd.copy_(q)
+        out = torch.empty(4096, device="cuda", dtype=torch.bfloat16).as_strided((N, H * 64), (H * 64 if N > 1 else 1001, 1))
+        want = ops.paged_tree_attention(q, *args)
+        listen = object.__new__(Listen)
+        listen.__dict__ = ops.__dict__
+        assert torch.equal(listen.paged_tree_attention(odd, *args, None, out), want)
+    assert names == ["kb_tree_attn"] * 3
+    ops.check_status()
+
+
 # ------------------------------------------------------------------ 4-bit products
 def test_products_added_to_no_output_are_refused():
     ops = get_ops("cuda")
