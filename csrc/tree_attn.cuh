@@ -43,8 +43,8 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 }
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) { return __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3); }
 __device__ __forceinline__ uint32_t largest(uint32_t two_bf16) { return max(two_bf16 & 0x7fffu, (two_bf16 >> 16) & 0x7fffu); }
-// Four bf16 numbers times `inv` as the sum of two e4m3 numbers each: together they hold the eight bits of a bf16 number (numbers within 2^-10
-// of the type's upper end; below, they are off by at most 2^-10).
+// Four bf16 numbers times `inv` as the sum of two e4m3 numbers each: together they hold the eight bits of a bf16 number from 2^-2 on; smaller
+// ones are off by at most 2^-10.
 __device__ __forceinline__ void split_e4m3(uint2 q, float inv, uint32_t& hi, uint32_t& lo) {
     uint32_t h[2], l[2];
 #pragma unroll

@@ -17,10 +17,10 @@
 // 8-bit pages.  Codes become f16 (exact) on the way to the tensor cores.  Keys: the score's accumulator is scaled by the token's power of two.
 // Values: the probability is scaled by the token's power of two relative to E, the largest seen so far by the warp, times 2^4, and
 // rounded to f16; the output is kept in units of 2^(E - 4).  Maxima are renewed when a score exceeds them by 2^11, so f16's largest is
-// 2^15, and a probability keeps eleven bits down to 2^-18 of the maximum and is off by at most 2^-29 below.
+// 2^15; a scaled probability keeps eleven bits down to 2^-18 and is off by at most 2^-29 below.
 // Values whose powers lie more than 2^SPREAD apart: a unit per row in E's place (apart_step), so that a token that a row does not see or gives no
 // weight takes nothing from it, however large it is.  (64 x 1 tokens over 2048: 53.6 us a call without that code in the kernel, 55.3 with it.)
-// Queries become f16 with a power of two per row taken out (exact down to 2^-24 of the row's largest).
+// Queries become f16 with a power of two per row taken out, which brings the largest number to [1, 2): exact from 2^-17 on, off by at most 2^-25 below.
 // bf16 pages: queries as they are, probabilities rounded to bf16.  Scores, maxima, sums and outputs are fp32.
 #include "tree_attn.cuh"
 
@@ -314,8 +314,7 @@ tree_attn_kernel(const TreeParams p) {
                         E = top;
                     }
                     fk[lane] = pow2_biased(ek) * p.scale_log2;
-                    const int w = min(ev - E, 0) + UP + 127;
-                    fk[TILE + lane] = E == APART ? (float)(ev - 127) : counts ? (w > 0 ? __uint_as_float((uint32_t)w << 23) : 0.f) : 1.f;
+                    fk[TILE + lane] = E == APART ? (float)(ev - 127) : counts ? __uint_as_float((uint32_t)(ev - E + UP + 127) << 23) : 1.f;
                     __syncwarp();
                 }
                 // ---- scores

@@ -10,14 +10,14 @@
 //
 //   S = Q K^T    both operands K-major in shared memory, one accumulator per group
 //                bf16 pages: kind::f16.  8-bit pages: kind::f8f6f4 on the codes as they lie in the cache; a query row, a power of two
-//                taken out, is the sum of two e4m3 numbers, hi + lo, which together hold bf16's eight bits (down to 2^-10 of the row's
-//                largest; below that the error is at most 2^-18 of the largest) - two products at twice the rate of one in 16 bits.
+//                taken out, is the sum of two e4m3 numbers, hi + lo, which together hold bf16's eight bits (down to 2^-9 of the row's
+//                largest; below that the error is at most 2^-17 of the largest) - two products at twice the rate of one in 16 bits.
 //   softmax      in fp32, a row at a time in one pass: exponentials against the maximum so far, which is renewed only when a
 //                score exceeds it by more than 2^11 (2^20 where P is bf16); P back to tensor memory in 16 bits
 //   O += P V     A = P in tensor memory, B = value tile in shared memory (MN-major), one accumulator per group, so that the groups
 //                need nothing from one another before the end of a unit.  8-bit pages: P is f16 in units of 2^-4 (at most 2^15 with the
 //                2^11 of lazy maxima: eleven bits down to 2^-18, off by at most 2^-29 below); the values' f16 carry the token's power
-//                of two relative to E, the unit's largest so far (off by at most 2^-39 of the largest); O is in units of 2^(E - 6).
+//                of two relative to E, the unit's largest so far (exact, since none lies below 2^(E - SPREAD)); O is in units of 2^(E - 6).
 //                Values whose powers lie more than 2^SPREAD apart: as their codes, with a unit of O per row (apart_tile), so that a token
 //                that a row does not see or gives no weight takes nothing from it, however large it is.
 //
@@ -27,6 +27,8 @@
 // added row by row (never in normal use).  All waits are bounded (status word on timeout).
 #include "attn_common.cuh"
 #include "tree_attn.cuh"
+
+static_assert(tree::SPREAD <= 20, "factors of values are normal f16 numbers; codes times them are exact");
 
 namespace {
 
@@ -533,10 +535,10 @@ tree_tile_kernel(const TreeParams p) {
             const uint32_t vword = mt.valid[warp - W_VAL];
             uint8_t* op = sV + vs * L::VT;
             if constexpr (FP8) {
-                // the token's factor, an f16 power of two of at most 2^6 (twice); none where the probabilities carry it
+                // the token's factor, an f16 power of two from 2^(6 - SPREAD) to 2^6 (twice); none where the probabilities carry it
                 const uint8_t* raw = sR + rst * L::KT;
-                const int ev = exps[rst * 2 * TT + TT + t], w = ev == 255 || mt.E == APART ? 0 : min(ev - mt.E, 0) + 6;
-                const uint32_t one = !(vword >> lane & 1u) || w < -24 ? 0u : w >= -14 ? (uint32_t)(w + 15) << 10 : 1u << (w + 24);
+                const int ev = exps[rst * 2 * TT + TT + t], w = ev == 255 || mt.E == APART ? 0 : ev - mt.E + 6;
+                const uint32_t one = vword >> lane & 1u ? (uint32_t)(w + 15) << 10 : 0u;
                 const uint32_t mine = one | one << 16;
                 // codes -> f16: a warp takes whole rows, 16 codes per lane, so that loads and stores use all banks
                 constexpr int CH = HD / 16, RPW = 32 / CH;     // chunks per row, rows per warp step
