@@ -9,10 +9,10 @@
 // which bf16 holds.  A row that holds an infinity or a NaN is stored as exponent 255 with NaN codes; it reads back as NaN.
 // Compiled without fast-math (denormal results are kept).
 //
-// Append is bound by instructions (about 100 per warp and two rows of 128 each of keys and values; 8191 tokens x 8 heads x 128: 10.7 us, 4.7 TB/s; the 50 MB would take 7.8), since a
-// row's largest magnitude is needed before its first code; two bf16 magnitudes share a word on the way (one at a time: 22 us).  The rows are
-// fetched beside their slot: the two loads' latencies do not add up.  Reading back is bound by the memory: 16 x 4096 tokens x 8 heads x 128 in
-// 50.7 us, 6.1 TB/s (66 us with 16-byte stores).
+// Append: 8191 tokens x 8 heads x 128 in 10.7 us, 4.7 TB/s (the 50 MB would take 7.8).  About 107 instructions per warp and two rows of 128 each of keys and
+// values, in 66 % of the issue slots with 81 % of the warps there: between a row's loads and its first code lies the search for its largest
+// magnitude.  Two bf16 magnitudes share a word on the way (one at a time: 22 us).  The rows are fetched beside their slot: the two loads'
+// latencies do not add up.  Reading back is bound by the memory: 16 x 4096 tokens x 8 heads x 128 in 51 us, 6.0 TB/s (66 us with 16-byte stores).
 #include <cuda_fp8.h>
 
 #include "vec.cuh"

@@ -12,8 +12,9 @@
 // groups of inputs and meet in shared memory once per step of up to four tiles.  Every warp streams its blocks - a block of each tile, the tokens' inputs
 // for them, the scales - through a ring of its own by 16-byte asynchronous copies, across the steps, so that no load waits for arithmetic.
 //
-// What bounds it: instructions.  Of about 80 per 512 bytes 36 widen the codes, 4 multiply; the rest is copies, addresses, sums.  At 8 x 28672 x 4096
-// the schedulers issue in 56 % of the cycles and the ALU is half busy (18 us, 3.4 TB/s); the 64 MB alone would take 9.5 us.  Tried: registers instead
+// What bounds it: no unit alone.  Of about 80 instructions per 512 bytes 36 widen the codes, 4 multiply; the rest is copies, addresses, sums.  At
+// 8 x 28672 x 4096 the schedulers issue in 56 % of the cycles, the ALU is half busy, and 16 warps per SM do not cover the latencies in between (18 us,
+// 3.4 TB/s; the 64 MB alone would take 9.5 us).  Tried: registers instead
 // of the ring (23 us: fewer loads in flight), x straight from the L1 cache (27 us: it does not fit beside the rings), more and smaller
 // blocks of threads (20 to 25 us), 8 warps (20 us).
 #include <stddef.h>

@@ -12,7 +12,7 @@
 // into just that.  For step k lane q takes word q of the packed lane k of its row, so that the operand has the inputs in x's order.  The words are
 // read from shared memory one by one; the copies' places there are exchanged (by the row's bits 1 and 2) so that no two meet in a bank.
 //
-// What bounds it: the length of a turn's way from codes to sums, and instructions.  A turn of 64 tokens takes about 900 clocks, of which the products
+// What bounds it: the length of a turn's way from codes to sums.  A turn of 64 tokens takes about 900 clocks, of which the products
 // need 256: each role works 500 to 600 and waits for another the rest of the time, with the schedulers issuing in 54 % of the cycles (64 x 4096 x 14336:
 // 18.2 us, of which the bytes would take 5.2).  At 1024 x 6144 x 4096 it reaches 910 TFLOP/s, 0.54 of the library's bf16 product, because
 // every group's sums go through registers once.  Tried: x by 8-byte copies in the order that the store gives (30 us: issuing them), 16 widening warps

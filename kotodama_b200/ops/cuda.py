@@ -569,7 +569,7 @@ class CudaOps(TorchOps):
     def qknorm_rope_fwd(self, qkv, qw, kw, cos, sin, seq_len, n_q, n_kv, hd, eps, pos_offset=0, positions=None,
                         append=None):
         """``append=(k_pages, v_pages, slots)``: the same launch also writes the rotated keys and the values of
-        every token into its cache slot (what ``kv_append`` does as a launch of its own)."""
+        every token into its cache slot (what ``kv_append`` does as a launch of its own, and does here for 8-bit pages)."""
         N = qkv.shape[0]
         out = torch.empty(N, (n_q + n_kv) * hd, device=qkv.device, dtype=qkv.dtype)
         rstd = torch.empty(N, n_q + n_kv, device=qkv.device, dtype=torch.float32)

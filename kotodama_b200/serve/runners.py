@@ -113,7 +113,7 @@ class LlamaRunner:
                 committed = committed + [partial]
                 partial = None
             qkv = ops.gemm_nt(xn, lw["wqkv"])
-            # QK-norm + RoPE; the same launch puts the new keys and values into their cache slots
+            # QK-norm + RoPE; the same launch (an 8-bit cache: a second one) puts the new keys and values into their cache slots
             qk, _ = ops.qknorm_rope_fwd(qkv, lw["qn"], lw["kn"], cos, sin, N, H, KV, hd, eps, positions=b.positions,
                                         append=(self.cache.k[i], self.cache.v[i], b.slots))
             k_rows = qk[:, H * hd:]
