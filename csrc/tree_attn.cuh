@@ -10,10 +10,12 @@ typedef __nv_bfloat16 bf16;
 namespace tree {
 
 constexpr int PAGE = 16, MAX_B = 1024;
-// 8-bit pages: most binary orders of magnitude between the powers of two of a unit's values for one unit of the output for all rows, so that
-// a probability near the maximum keeps f16's eleven bits beside the smallest of them.  Values further apart (hidden tokens count: what they
-// hold is not known to be small) have a unit per row, which depends on nothing that the row does not see or gives no weight.
-constexpr int SPREAD = 16;
+// 8-bit pages: most binary orders of magnitude between the powers of two of a unit's values for one unit of the output, in which 16-bit operands
+// carry them: a row's terms are then off by at most 2^-17 of its largest, whatever tokens it does not see or gives no weight (2^-25 where it sees the
+// largest values).  Values further apart (hidden ones count: what they hold is not known to be small) are added in fp32 where rows are few,
+// or have a unit per row that follows the row's own terms.  (Normal numbers times lognormal factors of e^0.7 lie within 2^9 in a part of a thousand
+// tokens.  The rare path takes 7 and 2.5 times as long.)
+constexpr int SPREAD = 12;
 constexpr float NO_UNIT = -1e30f;                      // log2 of the unit of an output without a term
 
 struct TreeParams {

@@ -19,8 +19,8 @@
 // Values: the probability is scaled by the token's power of two relative to E, the largest seen so far by the warp, times 2^4, and
 // rounded to f16; the output is kept in units of 2^(E - 4).  Maxima are renewed when a score exceeds them by 2^11, so f16's largest is
 // 2^15; a scaled probability keeps eleven bits down to 2^-18 and is off by at most 2^-29 below.
-// Values whose powers lie more than 2^SPREAD apart: a unit per row in E's place (apart_step), so that a token that a row does not see or gives no
-// weight takes nothing from it, however large it is.  (64 x 1 tokens over 2048: 53.6 us a call without that code in the kernel, 55.3 with it.)
+// Values whose powers lie more than 2^SPREAD apart: added in fp32 like values that are not finite, so that a token that a row does not see or gives
+// no weight takes nothing from it, however large it is.
 // Queries become f16 with a power of two per row taken out, which brings the largest number to [1, 2): exact from 2^-17 on, off by at most 2^-25 below.
 // bf16 pages: queries as they are, probabilities rounded to bf16, since both operands of a product have one type (16 x 16 tokens over 4000: off by 0.0023
 // of the result in 64 bits, where rounding the result alone leaves 0.0017).  Scores, maxima, sums and outputs are fp32.
@@ -87,54 +87,15 @@ __device__ __forceinline__ void zero_rows(const TreeParams& p, int c0, int n, in
     }
 }
 
-// A step's softmax with a unit of the output per row, 2^D times that of the sums (SPREAD in tree_attn.cuh): scores s become probabilities that
-// carry their value's power of two (w: its exponent) relative to it.  D follows the row's largest term by steps of at least 2^GROW, the maximum
-// is taken as it is.  ml: maxima and sums of the lane's two rows; o: their output, [OT][4].
-constexpr int UP = 4, GROW8 = 11;                      // 8-bit pages: probabilities carry 2^UP, at most 2^(GROW8 + UP)
-template <int NT, int OT>
-__device__ __noinline__ void apart_step(float* o, float* s, float* ml, const float* w, float* units, float2 rs) {
-#pragma unroll 1
-    for (int hf = 0; hf < 2; ++hf) {
-        const float r = hf ? rs.y : rs.x;
-        float mx = -INFINITY, y = -INFINITY, sum = 0.f;
-#pragma unroll 1
-        for (int i = 0; i < 2 * NT; ++i) {
-            float& v = s[(i >> 1) * 4 + 2 * hf + (i & 1)];
-            v *= r;
-            mx = fmaxf(mx, v);
-            y = fmaxf(y, v + w[(i >> 1) * 8 + (i & 1)]);
-        }
-#pragma unroll
-        for (int d = 1; d < 4; d <<= 1) {
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, d));
-        }
-        const float was = ml[hf], m = fmaxf(was, mx), at = m == -INFINITY ? 0.f : m;
-        float D = fmaxf(units[hf * THREADS] + (was - m), NO_UNIT);             // (also where the difference is NaN: no maximum yet)
-        const float to = y - at > D + GROW8 ? y - at - UP : D, f = exp2f(D - to);
-        units[hf * THREADS] = D = to;
-        if (f != 1.f)
-#pragma unroll 1
-            for (int i = 0; i < 2 * OT; ++i) o[(i >> 1) * 4 + 2 * hf + (i & 1)] *= f;
-#pragma unroll 1
-        for (int i = 0; i < 2 * NT; ++i) {
-            float& v = s[(i >> 1) * 4 + 2 * hf + (i & 1)];
-            const float t = v - at;
-            sum += exp2f(t);
-            v = exp2f(t + (w[(i >> 1) * 8 + (i & 1)] - D));
-        }
-        ml[hf] = m;
-        ml[2 + hf] = (m == -INFINITY ? ml[2 + hf] : ml[2 + hf] * exp2f(was - m)) + sum;
-    }
-}
-
 // DIRECT: a block of threads per unit, whose tiles its warps share; nothing is left for a merge.  Else the line of tiles of all units.
 template <bool FP8, int HD, bool DIRECT>
 __global__ void __launch_bounds__(THREADS, CTAS)
 tree_attn_kernel(const TreeParams p) {
     using C = Cfg<FP8, HD>;
     constexpr int TILE = C::TILE, NT = TILE / 8, KS = HD / 16;
-    constexpr float GROW = FP8 ? GROW8 : 20.f;         // log2 units: when a maximum is renewed; 8-bit pages: f16 holds 2^(GROW + UP)
+    // log2 units: when a maximum is renewed; 8-bit pages: probabilities carry 2^UP, and f16 holds 2^(GROW + UP)
+    constexpr int UP = 4;
+    constexpr float GROW = FP8 ? 11.f : 20.f;
     extern __shared__ __align__(128) uint8_t ring_all[];
     uint8_t* exps_all = ring_all + C::RING;
     float* fact_all = reinterpret_cast<float*>(exps_all + C::EXPS);
@@ -142,7 +103,6 @@ tree_attn_kernel(const TreeParams p) {
     __shared__ int wsum[WARPS];
     __shared__ uint32_t there[WARPS][C::NST];          // bit per page of a stage: loaded
     __shared__ float2 wml[WARPS][C::ROWS];
-    __shared__ float units[FP8 ? 2 * THREADS : 1];     // (E == APART)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = lane >> 2, qd = lane & 3;
     kb_dep_wait();
     kb_dep_trigger();
@@ -282,7 +242,7 @@ tree_attn_kernel(const TreeParams p) {
         }
         float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
         int E = 0, low = 255;                          // biased exponent of the output's unit; the smallest of the values so far
-        constexpr int APART = -1;                      // for E: a unit per row, 2^D times that of the sums (D in shared memory, two rows per lane)
+        constexpr int APART = -1;                      // for E: the output is in units of one, values are added in fp32
 #pragma unroll
         for (int j = 0; j < HD / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
         for (int t = sg.t0; t < sg.t1; ++t, ++x) {
@@ -307,8 +267,7 @@ tree_attn_kernel(const TreeParams p) {
                     const int top = (int)__reduce_max_sync(0xffffffffu, counts ? (unsigned)ev : 0u);
                     low = min(low, (int)__reduce_min_sync(0xffffffffu, counts ? (unsigned)ev : 255u));
                     if (E != APART && max(top, E) - low > SPREAD) {
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) units[hf * THREADS + threadIdx.x] = m[hf] == -INFINITY ? NO_UNIT : (float)(E - 127 - UP);
+                        grow = exp2f((float)(E - 127 - UP));               // (zero ahead of the first token: so is the output)
                         E = APART;
                     }
                     if (E != APART && top > E) {
@@ -316,7 +275,7 @@ tree_attn_kernel(const TreeParams p) {
                         E = top;
                     }
                     fk[lane] = pow2_biased(ek) * p.scale_log2;
-                    fk[TILE + lane] = E == APART ? (float)(ev - 127) : counts ? __uint_as_float((uint32_t)(ev - E + UP + 127) << 23) : 1.f;
+                    fk[TILE + lane] = counts && E != APART ? __uint_as_float((uint32_t)(ev - E + UP + 127) << 23) : 1.f;
                     __syncwarp();
                 }
                 // ---- scores
@@ -363,8 +322,8 @@ tree_attn_kernel(const TreeParams p) {
                     s[j][3] *= f.y;
                 }
                 // ---- what is not seen: places that hold no token, and drafted tokens the row's mask does not name
-                uint32_t odd = 0;                      // drafted tokens whose values are not finite: kept out of the product
-                uint32_t seen[2] = {0u, 0u};           // bit t: the row sees token t of the step (only where something is hidden)
+                uint32_t odd = FP8 && E == APART ? valid : 0u;             // tokens kept out of the product: drafted ones whose values are not finite, or all
+                uint32_t seen[2] = {~0u, ~0u};         // bit t: the row sees token t of the step
                 if (!whole || drafts) {
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
@@ -390,7 +349,7 @@ tree_attn_kernel(const TreeParams p) {
                                     bad |= FP8 ? __vcmpeq4(w[q] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0u : __vcmpeq2(w[q] & 0x7f807f80u, 0x7f807f80u) != 0u;
                             }
                         }
-                        odd = __ballot_sync(0xffffffffu, bad);
+                        odd |= __ballot_sync(0xffffffffu, bad);
                     }
                 }
                 // ---- softmax against a maximum that is renewed only when a score exceeds it by more than GROW
@@ -402,69 +361,48 @@ tree_attn_kernel(const TreeParams p) {
                     for (int j = 1; j < NT; ++j) mx[hf] = fmaxf(mx[hf], fmaxf(s[j][2 * hf], s[j][2 * hf + 1]));
                     if constexpr (FP8) mx[hf] *= rs[hf];
                 }
-                if (FP8 && E == APART) {
-                    float os[HD / 2], ss[NT * 4], ml[4] = {m[0], m[1], l[0], l[1]};        // (in local memory, here only)
-#pragma unroll
-                    for (int i = 0; i < HD / 2; ++i) os[i] = o[i >> 2][i & 3];
-#pragma unroll
-                    for (int i = 0; i < NT * 4; ++i) ss[i] = s[i >> 2][i & 3];
-                    apart_step<NT, HD / 8>(os, ss, ml, fk + TILE + 2 * qd, units + threadIdx.x, make_float2(rs[0], rs[1]));
-#pragma unroll
-                    for (int i = 0; i < HD / 2; ++i) o[i >> 2][i & 3] = os[i];
-#pragma unroll
-                    for (int i = 0; i < NT * 4; ++i) s[i >> 2][i & 3] = ss[i];
-                    m[0] = ml[0];
-                    m[1] = ml[1];
-                    l[0] = ml[2];
-                    l[1] = ml[3];
-                } else {
-                    if (__any_sync(0xffffffffu, mx[0] > m[0] + GROW || mx[1] > m[1] + GROW || (FP8 && grow != 1.f))) {
-                        float f[2];
-#pragma unroll
-                        for (int hf = 0; hf < 2; ++hf) {
-                            mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
-                            mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
-                            const float mn = fmaxf(m[hf], mx[hf]);
-                            f[hf] = mn == -INFINITY ? 1.f : exp2f(m[hf] - mn);
-                            m[hf] = mn;
-                            l[hf] *= f[hf];
-                            f[hf] *= grow;
-                        }
-#pragma unroll
-                        for (int j = 0; j < HD / 8; ++j) {
-                            o[j][0] *= f[0];
-                            o[j][1] *= f[0];
-                            o[j][2] *= f[1];
-                            o[j][3] *= f[1];
-                        }
-                    }
+                if (__any_sync(0xffffffffu, mx[0] > m[0] + GROW || mx[1] > m[1] + GROW || (FP8 && grow != 1.f))) {
+                    float f[2];
 #pragma unroll
                     for (int hf = 0; hf < 2; ++hf) {
-                        const float at = m[hf] == -INFINITY ? 0.f : m[hf];
+                        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 1));
+                        mx[hf] = fmaxf(mx[hf], __shfl_xor_sync(0xffffffffu, mx[hf], 2));
+                        const float mn = fmaxf(m[hf], mx[hf]);
+                        f[hf] = mn == -INFINITY ? 1.f : exp2f(m[hf] - mn);
+                        m[hf] = mn;
+                        l[hf] *= f[hf];
+                        f[hf] *= grow;
+                    }
 #pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            float a = exp2f(FP8 ? fmaf(s[j][2 * hf], rs[hf], -at) : s[j][2 * hf] - at);
-                            float z = exp2f(FP8 ? fmaf(s[j][2 * hf + 1], rs[hf], -at) : s[j][2 * hf + 1] - at);
-                            l[hf] += a + z;
-                            if constexpr (FP8) {
-                                const float2 w = *reinterpret_cast<const float2*>(fk + TILE + 8 * j + 2 * qd);
-                                a *= w.x;
-                                z *= w.y;
-                            }
-                            s[j][2 * hf] = a;
-                            s[j][2 * hf + 1] = z;
-                        }
+                    for (int j = 0; j < HD / 8; ++j) {
+                        o[j][0] *= f[0];
+                        o[j][1] *= f[0];
+                        o[j][2] *= f[1];
+                        o[j][3] *= f[1];
                     }
                 }
                 uint32_t pa[TILE / 16][4];
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf)
+                for (int hf = 0; hf < 2; ++hf) {
+                    const float at = m[hf] == -INFINITY ? 0.f : m[hf];
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        pa[j >> 1][(j & 1) * 2 + hf] = FP8 ? pack_f16(s[j][2 * hf], s[j][2 * hf + 1]) : pack_bf16(s[j][2 * hf], s[j][2 * hf + 1]);
+                    for (int j = 0; j < NT; ++j) {
+                        float a = exp2f(FP8 ? fmaf(s[j][2 * hf], rs[hf], -at) : s[j][2 * hf] - at);
+                        float z = exp2f(FP8 ? fmaf(s[j][2 * hf + 1], rs[hf], -at) : s[j][2 * hf + 1] - at);
+                        l[hf] += a + z;
+                        if constexpr (FP8) {
+                            const float2 w = *reinterpret_cast<const float2*>(fk + TILE + 8 * j + 2 * qd);
+                            a *= w.x;
+                            z *= w.y;
+                        }
+                        s[j][2 * hf] = a;
+                        s[j][2 * hf + 1] = z;
+                        pa[j >> 1][(j & 1) * 2 + hf] = FP8 ? pack_f16(a, z) : pack_bf16(a, z);
+                    }
+                }
                 if (!whole || odd) {
-                    // Values that must not enter the product: what the cache holds in places without a token, and drafted tokens that
-                    // are not finite - those are added row by row (never in normal use)
+                    // Values that must not enter the product: what the cache holds in places without a token, and the odd tokens, which are
+                    // added row by row (never in normal use)
                     uint8_t* pages = ring + (size_t)st * C::STAGE + C::PAGES * C::PAGE_BYTES;
                     volatile float kept[NT][4];        // (indexed by the token: in local memory, here only)
                     if (odd)
@@ -476,6 +414,7 @@ tree_attn_kernel(const TreeParams p) {
                     for (uint32_t left = odd; left; left &= left - 1u) {
                         const int tk = __ffs(left) - 1, src = (lane & ~3) | ((tk & 7) >> 1), tr = tk % PAGE;
                         const uint8_t* page = pages + (tk / PAGE) * C::PAGE_BYTES;
+                        const float unit = FP8 && E == APART ? pow2_biased(exps[st * 2 * TILE + TILE + tk]) : 1.f;
                         float pv[2];
 #pragma unroll
                         for (int hf = 0; hf < 2; ++hf) pv[hf] = __shfl_sync(0xffffffffu, kept[tk >> 3][2 * hf + (tk & 1)], src);
@@ -485,7 +424,7 @@ tree_attn_kernel(const TreeParams p) {
                             for (int e = 0; e < 2; ++e) {
                                 const int d = FP8 ? (j >> 1) * 16 + 4 * qd + 2 * e + (j & 1) : 8 * j + 2 * qd + e, byte = FP8 ? d : 2 * d;
                                 const uint8_t* at = page + C::place(tr * (C::ROW_BYTES / 16) + byte / 16) + byte % 16;
-                                const float v = FP8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(*at, __NV_E4M3))) : __bfloat162float(*reinterpret_cast<const bf16*>(at));
+                                const float v = FP8 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(*at, __NV_E4M3))) * unit : __bfloat162float(*reinterpret_cast<const bf16*>(at));
                                 if (seen[0] >> tk & 1u) o[j][e] += pv[0] * v;
                                 if (seen[1] >> tk & 1u) o[j][2 + e] += pv[1] * v;
                             }
@@ -548,7 +487,7 @@ tree_attn_kernel(const TreeParams p) {
             l[hf] += __shfl_xor_sync(0xffffffffu, l[hf], 2);
             const int row = hf * 8 + r, R = row0 + row;
             if (R >= M) continue;
-            float g = FP8 ? E == APART ? exp2f(units[hf * THREADS + threadIdx.x]) : pow2_biased(E) * (1.f / (1 << UP)) : 1.f;       // 2^(E - 127 - UP)
+            float g = FP8 && E != APART ? pow2_biased(E) * (1.f / (1 << UP)) : 1.f;    // 2^(E - 127 - UP)
             if (done) g *= l[hf] == 0.f ? 0.f : 1.f / l[hf];
             bf16* dst = p.out + (long long)(c0 + R / p.G) * p.out_stride + (long long)(sg.h * p.G + R % p.G) * HD;
 #pragma unroll

@@ -74,6 +74,14 @@ def test_values_of_every_size(hd, H, bound):
     get_ops("cuda").check_status()
 
 
+@pytest.mark.parametrize("H,G,hd,sizes,lens,masked,seed,spread,bound", [
+    (32, 4, 128, [5, 5], [548, 6], False, 540258, 6.0, 3000),
+    (8, 8, 128, [11, 31, 19, 19, 15, 25, 27, 4, 32, 33, 23, 8, 16, 27, 31, 31, 31], [96, 32, 20, 50, 15, 25, 27, 5, 32, 69, 24, 70, 17, 27, 43, 40, 47], True, 267427, 1.0, None)])
+def test_elements_without_the_large_tokens(H, G, hd, sizes, lens, masked, seed, spread, bound):
+    """Elements in which a row's large tokens hold exact zeros live on its small ones."""
+    cases.check_tree(get_ops("cuda"), "cuda", H, G, hd, sizes, lens, True, torch.bfloat16, masked, seed=seed, spread=spread, bound=bound)
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("H", [4, 64])

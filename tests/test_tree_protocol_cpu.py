@@ -19,9 +19,10 @@ KST, VST, SLOTS = 2, 2, 8
 
 class Part:
     """The roles' programs for a part whose segments have the given numbers of tiles.  ``idle_groups_wait``: a softmax group waits for a unit's
-    queries at the unit's start, even if it has no tile of it."""
+    queries at the unit's start, even if it has no tile of it.  ``by_hand``: the softmax groups read every value tile themselves (values far
+    apart, or not finite)."""
 
-    def __init__(self, segments: list[int], fp8: bool, idle_groups_wait: bool = False) -> None:
+    def __init__(self, segments: list[int], fp8: bool, idle_groups_wait: bool = False, by_hand: bool = False) -> None:
         self.fp8, rst = fp8, 3 if fp8 else 2
         seg_of = [s for s, n in enumerate(segments) for _ in range(n)]
         begin = [sum(segments[:s]) for s in range(len(segments) + 1)]
@@ -71,7 +72,7 @@ class Part:
                     step(f"g{g}", [(("q_ready", s & 1), s >> 1)], read=("q", s))
                 for j in mine:
                     step(f"g{g}", [(("s_full", g), j >> 1), (("f_ready", j % SLOTS), j // SLOTS)])
-                    step(f"g{g}", arrives=[("p_ready", g)])
+                    step(f"g{g}", [(("v_ready", j % VST), j // VST)] if by_hand else [], [("p_ready", g)])
                 step(f"g{g}", arrives=[("xch", 0)])
                 last = begin[s + 1] - 1
                 step(f"g{g}", [(("xch", 0), turn), (("pv_done", last % VST), last // VST)], read=("o", s))
@@ -140,10 +141,11 @@ class Part:
 SEGMENTS = [[1], [2], [1, 1, 1], [2, 1, 1], [1, 2, 1], [1, 1, 2], [3, 1]]
 
 
+@pytest.mark.parametrize("by_hand", [False, True])
 @pytest.mark.parametrize("fp8", [False, True])
 @pytest.mark.parametrize("segments", SEGMENTS, ids=str)
-def test_no_role_overruns_another(segments, fp8):
-    assert Part(segments, fp8).explore() is None
+def test_no_role_overruns_another(segments, fp8, by_hand):
+    assert Part(segments, fp8, by_hand=by_hand).explore() is None
 
 
 def test_a_group_without_a_tile_must_not_wait_for_the_queries():
