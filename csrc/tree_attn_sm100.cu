@@ -5,7 +5,7 @@
 // cache's bytes bound the call, and above ~100 rows the tensor cores do.  Each (sequence, KV head) has its n * G query rows as the
 // M side of `mma.sync.m16n8k16` tiles (16 of them per unit of work), cached tokens are the N side of the score product and the K side of
 // the output product; probabilities go from accumulators to operands in registers.  Calls with more rows per KV head
-// (`plan_for` below) take tree_attn_tile_sm100.cu.  Measured: 64 x 1 tokens over 2048, 8 bits, 24 query and 8 KV heads, 52 us, 3.9 TB/s, with the issue slots at
+// (`plan_for` below) take tree_attn_tile_sm100.cu.  Measured: 64 x 1 tokens over 2048, 8 bits, 24 query and 8 KV heads, 51 us, 4.0 TB/s, with the issue slots at
 // 44 %, DRAM at 50 and the tensor cores at 27 %: 12 warps per SM, what 168 registers admit, do not cover a step's latencies.
 //
 // Work.  A unit is (sequence, KV head, block of rows); its tiles are TILE tokens of the context.  All units' tiles form one line

@@ -19,7 +19,8 @@
 //                2^11 of lazy maxima: eleven bits down to 2^-18, off by at most 2^-29 below); the values' f16 carry the token's power
 //                of two relative to E, the unit's largest so far (exact, since none lies below 2^(E - SPREAD)); O is in units of 2^(E - 6).
 //                Values whose powers lie more than 2^SPREAD apart: as their codes, with a unit of O per row (apart_tile), so that a token
-//                that a row does not see or gives no weight takes nothing from it, however large it is.
+//                that a row does not see or gives no weight takes nothing from it, however large it is.  (64 rows over 131000 tokens: 245 us a call
+//                without that code in the kernel, 251 with it, 2.5 times that where it runs; fp32 sums in its place 256 and 16 times.)
 //
 // The groups run out of step: one computes while the products of the other run.  Query rows are double-buffered by unit.
 // Tokens that do not exist are masked in S and zeroed in the value tile (whatever the cache holds there).  Values of drafted tokens that
