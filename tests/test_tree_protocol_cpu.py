@@ -1,8 +1,8 @@
 """Interleaving check of the barriers of the tree attention kernel with 128-row tiles (csrc/tree_attn_tile_sm100.cu).
 
 Every role of the kernel is a program of steps; a step waits for phases of barriers, then arrives on others.  A barrier's wait knows the
-parity of a phase only, as on the GPU: it passes when the phase in progress has the other parity.  The checker walks every interleaving of
-a part's roles (the tensor core, which runs products in order some time after their issue, is a role of its own) and reports
+parity of a phase only, as on the GPU: it passes when the phase in progress has the other parity.  Every interleaving of a part's roles is
+walked (the tensor core, which runs products in order some time after their issue, is a role of its own); reported are
 
 * an *overrun* - a wait that passed on another phase than its own,
 * a *stale* read - query scales of another unit, an output that the next unit has begun to overwrite, and
@@ -19,8 +19,8 @@ KST, VST, SLOTS = 2, 2, 8
 
 class Part:
     """The roles' programs for a part whose segments have the given numbers of tiles.  ``idle_groups_wait``: a softmax group waits for a unit's
-    queries at the unit's start, even if it has no tile of it.  ``by_hand``: the softmax groups read every value tile themselves (values far
-    apart, or not finite)."""
+    queries at the unit's start, even if it has no tile of it.  ``by_hand``: the softmax groups read every value tile themselves (values
+    that are not finite)."""
 
     def __init__(self, segments: list[int], fp8: bool, idle_groups_wait: bool = False, by_hand: bool = False) -> None:
         self.fp8, rst = fp8, 3 if fp8 else 2
